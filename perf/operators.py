@@ -101,7 +101,8 @@ def _activations(rows, cols, seed, stream):
 
 def _codes(x):
     a = x.abs().amax(dim=-1, keepdim=True).clamp(min=FLOOR)
-    return torch.round(x * (127.0 / a)).to(torch.int8), (a / 127.0).squeeze(-1)
+    most = torch.full_like(a, 127.0)
+    return torch.round(x * (most / a)).to(torch.int8), (a / most).squeeze(-1)
 
 
 def prepare(case, seed):
@@ -156,7 +157,8 @@ def _run_own(state):
 def _round(x):
     """x as 8-bit codes (held in 32 bits) and the scale of each row (last dimension)."""
     a = torch.clamp(torch.amax(torch.abs(x), dim=-1, keepdim=True), min=FLOOR)
-    return torch.round(x * (127.0 / a)), a / 127.0
+    most = torch.full_like(a, 127.0)  # a tensor: with a number, torch multiplies by a rounded reciprocal
+    return torch.round(x * (most / a)), a / most
 
 
 def _plain_rows(state):
@@ -232,7 +234,7 @@ def work(case):
 
 def _step_of(largest):
     """The step (scale) of groups whose largest magnitudes are given, as the format defines it."""
-    return torch.maximum(largest, torch.full_like(largest, FLOOR)).div(127)
+    return torch.maximum(largest, torch.full_like(largest, FLOOR)).div(torch.full_like(largest, 127.0))
 
 
 def _read_back(values, factor=None):
