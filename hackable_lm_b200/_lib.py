@@ -63,6 +63,14 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "hlm_attention_bwd_workspace_bytes": ([_I64, _I64, _I64, _I64], c_size_t),
     "hlm_attention_bwd": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _I64, _I64, _I64, _I64, _I64, _I64,
                            c_float, _P], c_int),
+    "hlm_quantize_rows": ([_P, _P, _P, _I64, _I64, c_int, _P], c_int),
+    "hlm_dequantize_rows": ([_P, _P, _P, _I64, _I64, c_int, _P], c_int),
+    "hlm_residual_rms_norm_q8": ([_P, _P, _P, _P, _P, _P, _I64, _I64, c_float, c_int, _P], c_int),
+    "hlm_linear_q8": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, c_int, _P], c_int),
+    "hlm_swiglu_ckpt8_fwd": ([_P, _P, _P, _P, _I64, _I64, c_int, _P], c_int),
+    "hlm_swiglu_ckpt8_bwd": ([_P, _P, _P, _P, _I64, _I64, c_int, _P], c_int),
+    "hlm_weight_grad_q8": ([_P, _P, _P, _P, _P, c_size_t, _I64, _I64, _I64, c_int, _P], c_int),
+    "hlm_weight_grad_q8_workspace_bytes": ([_I64, _I64, _I64], c_size_t),
     "hlm_gemm_bf16": (
         [_P, _P, _P, _I64, _I64, _I64, c_int, c_int, _I64, _I64, _I64, c_int, c_int, _P], c_int),
 }
@@ -143,6 +151,8 @@ KERNEL_IDS = {
     "qkv_dx": 7, "qkv_dw": 8, "swiglu_fwd": 9, "swiglu_bwd": 10, "rmsnorm_fwd": 11,
     "rmsnorm_bwd": 12, "qk_rope_fwd": 13, "qk_rope_bwd": 14, "gemm": 15, "gate_up": 16,
     "swiglu_down_bwd": 17, "proj_norm": 18, "attn_fwd": 19, "attn_bwd": 20,
+    "quant_rows": 21, "dequant_rows": 22, "norm_q8": 23, "linear_q8": 24, "swiglu_ckpt8_fwd": 25,
+    "swiglu_ckpt8_bwd": 26, "weight_grad_q8": 27,
 }
 
 

@@ -1,0 +1,65 @@
+// The 8-bit format shared by the quantising operators and their readers.
+//
+// A group of values v (a whole row, or 128 columns of a checkpoint) is held as
+// int8 codes and one fp32 scale:
+//
+//   a = max(max|v|, 2^-110),  q = rint(v * (127 / a)),  scale = a / 127,  v ~ q * scale
+//
+// with IEEE fp32 divisions and product, so the codes of a group do not depend
+// on how the group is split over threads.  |q| <= 127: 127 / a and the product
+// are each at most (1 + 2^-24) too large, and 127 (1 + 2^-24)^2 rounds to 127.
+// The floor 2^-110 keeps 127 / a and a / 127 normal numbers; smaller groups
+// read back as multiples of 2^-110 / 127.  A group that holds an infinity or a
+// NaN has scale NaN and codes 0: everything read back from it is NaN.
+#pragma once
+
+#include "hlm_common.cuh"
+
+namespace hlm {
+
+constexpr float kQuantFloor = 7.7037197775489434e-34f;  // 2^-110
+constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr int kCkptGroup = 128;  // columns of one checkpoint group
+
+// Magnitude of v as bits: ordered like the magnitudes, with infinities above
+// every finite value and NaNs above infinity, so an integer maximum keeps both.
+HLM_DEVICE uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct QuantStep {
+  float inv;    // 127 / a, or 0 for a group that is not finite
+  float scale;  // a / 127, or NaN
+};
+HLM_DEVICE QuantStep quant_step(uint32_t max_bits) {
+  QuantStep s;
+  if (max_bits >= kInfBits) {
+    s.inv = 0.0f;
+    s.scale = __uint_as_float(0x7fc00000u);
+  } else {
+    const float a = fmaxf(__uint_as_float(max_bits), kQuantFloor);
+    s.inv = __fdiv_rn(127.0f, a);
+    s.scale = __fdiv_rn(a, 127.0f);
+  }
+  return s;
+}
+
+// Code of v.  rint through the fp32 magic number 1.5 * 2^23: for |v * inv| <= 127.0001
+// the sum's low mantissa bits are the rounded (half to even) integer in two's
+// complement, so the low byte of the sum is the code.  The product is rounded
+// to fp32 first (no fused multiply-add), as the format defines it.  With inv = 0,
+// an infinity or NaN in v gives NaN bits whose low byte is replaced by 0.
+HLM_DEVICE uint32_t quant_bits(float v, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f));
+}
+HLM_DEVICE int8_t quant_code(float v, const QuantStep& s) {
+  return s.inv == 0.0f ? static_cast<int8_t>(0) : static_cast<int8_t>(quant_bits(v, s.inv) & 0xffu);
+}
+// Four codes packed low byte first.
+HLM_DEVICE uint32_t quant_pack4(float v0, float v1, float v2, float v3, float inv) {
+  const uint32_t lo = __byte_perm(quant_bits(v0, inv), quant_bits(v1, inv), 0x0040);
+  const uint32_t hi = __byte_perm(quant_bits(v2, inv), quant_bits(v3, inv), 0x0040);
+  return inv == 0.0f ? 0u : __byte_perm(lo, hi, 0x5410);
+}
+
+HLM_DEVICE uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+}  // namespace hlm

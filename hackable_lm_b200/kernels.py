@@ -250,6 +250,66 @@ def fused_linear_cross_entropy_with_weight(hidden: torch.Tensor, weight: torch.T
     return _B200FusedLinearCrossEntropy.apply(hidden_flat, weight, targets_flat, ignore_index, chunk_size)
 
 
+# ---------------------------------------------------------------------------
+# 8-bit operators: int8 inference projections and 8-bit activation checkpoints
+# ---------------------------------------------------------------------------
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., C] as int8 codes [..., C] and one fp32 scale for each row [...]: x ~ q * scale,
+    off by at most half a scale (the row's largest magnitude / 254).  Also how a weight [N, K]
+    gets its codes and its scale for each output channel."""
+    _cuda_only(x, "quantize_rows")
+    return ops.quantize_rows(x)
+
+
+def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values q * scale that the codes stand for, rounded to ``dtype``."""
+    _cuda_only(q, "dequantize_rows")
+    return ops.dequantize_rows(q, scale, dtype)
+
+
+def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor | None, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rms_norm`` with its output in 8 bits: (q, scale by rows).  Not differentiable."""
+    _cuda_only(x, "rms_norm_q8")
+    return ops.rms_norm_q8(x, weight, eps)
+
+
+def residual_rms_norm_q8(residual: torch.Tensor, branch: torch.Tensor, eps: float,
+                         weight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``residual_rms_norm`` with the norm in 8 bits: (residual + branch, q, scale by rows).
+    Not differentiable."""
+    _cuda_only(branch, "residual_rms_norm_q8")
+    return ops.residual_rms_norm_q8(residual, branch, weight, eps)
+
+
+def linear_q8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(q * scale) @ (weight * weight_scale)^T on 8-bit integers: q int8 [..., K] with a scale for
+    each token [...], weight int8 [N, K] with a scale for each output channel [N], K a multiple
+    of 16 up to 131056; the sums are exact, the result [..., N] is rounded once to ``out_dtype``.
+    Not differentiable."""
+    _cuda_only(q, "linear_q8")
+    return ops.linear_q8(q, scale, weight, weight_scale, out_dtype)
+
+
+def swiglu_ckpt8(gate_up: torch.Tensor) -> torch.Tensor:
+    """``swiglu_triton`` that keeps gate_up [..., 2H] for the backward pass in 8 bits (one scale
+    for each 128 hidden units of the gate and of the up half) instead of whole: the output is the
+    same, the gradient is taken at the values the codes stand for."""
+    if gate_up.shape[-1] % 2:
+        raise RuntimeError(f"SwiGLU input last dimension must be even, got {gate_up.shape[-1]}")
+    _cuda_only(gate_up, "swiglu_ckpt8")
+    return ops.swiglu_ckpt8(gate_up)[0]
+
+
+def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """x @ weight^T (bf16 or fp16; weight [N, K], N a multiple of 8, K of 16) that keeps x for the
+    weight gradient in 8 bits by rows; the output and the gradient of x are those of F.linear."""
+    _cuda_only(x, "linear_ckpt8")
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        return F.linear(x, weight)  # no weight gradient: nothing of x to keep
+    return ops.linear_ckpt8(x, weight)[0]
+
+
 @dataclass(frozen=True)
 class WindowBlockMask:
     """What ``flex_attention_block_mask`` returns on this path: the causal

@@ -909,3 +909,13 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn_major: bool = False, b_mn_maj
         b.shape[1], out.stride(0), _code(out.dtype), int(accumulate), _stream(dev)),
         "hlm_gemm_bf16")
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit operators (their own module; imported last, it uses the helpers above)
+# ---------------------------------------------------------------------------
+from . import ops_q8 as _q8  # noqa: E402
+from .ops_q8 import (  # noqa: E402
+    dequantize_rows, linear_ckpt8, linear_ckpt8_supported, linear_q8, quantize_rows, residual_rms_norm_q8,
+    rms_norm_q8, swiglu_ckpt8, swiglu_ckpt8_backward, weight_grad_q8,
+)

@@ -104,7 +104,14 @@ uint64_t hlm_launch_count(void);
 #define HLM_KERNEL_PROJ_NORM 18    /* o_proj / down GEMM + residual add + RMSNorm epilogue */
 #define HLM_KERNEL_ATTN_FWD 19     /* attention forward (causal / sliding window) */
 #define HLM_KERNEL_ATTN_BWD 20     /* attention backward (its three launches) */
-#define HLM_KERNEL_MAX 21
+#define HLM_KERNEL_QUANT_ROWS 21   /* rows to 8 bits */
+#define HLM_KERNEL_DEQUANT_ROWS 22 /* rows read back from 8 bits */
+#define HLM_KERNEL_NORM_Q8 23      /* residual add + RMSNorm with an 8-bit output */
+#define HLM_KERNEL_LINEAR_Q8 24    /* 8-bit integer projection */
+#define HLM_KERNEL_SWIGLU_CKPT8_FWD 25 /* SwiGLU keeping its input in 8 bits */
+#define HLM_KERNEL_SWIGLU_CKPT8_BWD 26 /* its backward */
+#define HLM_KERNEL_WEIGHT_GRAD_Q8 27   /* weight gradient from an 8-bit input */
+#define HLM_KERNEL_MAX 28
 
 /* Start timing every launch of kernel `kernel_id`: launch i records
  * start_events[i] immediately before and stop_events[i] immediately after
@@ -357,6 +364,68 @@ int hlm_attention_bwd(const void* grad_out, const void* q, const void* k, const 
                       const float* lse, void* dq, void* dk, void* dv, void* workspace,
                       size_t workspace_bytes, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
                       int64_t window, float scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit operators
+ * ------------------------------------------------------------------------
+ *
+ * Format.  A group of values v is held as int8 codes and one fp32 scale:
+ *   a = max(max|v|, 2^-110),  q = rint(v * (127 / a)),  scale = a / 127,
+ * the divisions and the product in IEEE fp32 (rint: half to even), so the codes
+ * are the same wherever they are computed; v ~ q * scale with an error of at
+ * most scale / 2 and a few fp32 roundings.  A group holding an infinity or a
+ * NaN has scale NaN and codes 0.  A group is a whole row, except in the SwiGLU
+ * checkpoint.  All tensors are row-major contiguous.  No counterpart in the
+ * reference, whose operators are bf16. */
+
+/* x [rows, cols] (any dtype code) -> q int8 [rows, cols], scale fp32 [rows].
+ * cols >= 1. */
+int hlm_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int dtype,
+                      void* stream);
+
+/* out[r, c] = q[r, c] * scale[r], rounded to dtype. */
+int hlm_dequantize_rows(const void* q, const float* scale, void* out, int64_t rows, int64_t cols,
+                        int dtype, void* stream);
+
+/* hlm_residual_rms_norm_fwd with the norm in 8 bits: out = residual + branch
+ * (rounded to dtype), then the codes of v = out [* weight] and
+ * scale = a / 127 * rsqrt(mean(out^2) + eps).  1/rms is common to a row, so it
+ * cancels from the codes.  residual may be NULL (x = branch, `out` not
+ * written); weight may be NULL. */
+int hlm_residual_rms_norm_q8(const void* residual, const void* branch, const void* weight, void* out,
+                             void* q, float* scale, int64_t rows, int64_t cols, float eps, int dtype,
+                             void* stream);
+
+/* out[m, n] = (sum_k q[m, k] * w[n, k]) * scale[m] * w_scale[n]: exact int32 sums,
+ * then fp32, rounded to out_dtype (any code).  q [M, K] and w [N, K] int8,
+ * 16-byte aligned; scale [M], w_scale [N] fp32; out [M, N].  M and N are free,
+ * K a multiple of 16 up to HLM_LINEAR_Q8_MAX_K (any int8 sums stay within
+ * int32); other K return HLM_ERR_UNSUPPORTED. */
+#define HLM_LINEAR_Q8_MAX_K 131056
+int hlm_linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, void* out,
+                  int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
+
+/* SwiGLU that keeps its input in 8 bits for the backward pass.  Forward:
+ * h = silu(gate) * up (as hlm_swiglu_fwd) and the codes of gate_up, in groups of
+ * 128 hidden units of the gate half and of the up half (the last group of a
+ * half may be shorter): gate_up [rows, 2*hidden]; q int8 [rows, 2*hidden];
+ * scale fp32 [rows, 2*G], G = ceil(hidden / 128), gate groups first.
+ * Backward: the gradient of hlm_swiglu_bwd at the values that the codes stand
+ * for; grad_h [rows, hidden], grad_gate_up [rows, 2*hidden]. */
+int hlm_swiglu_ckpt8_fwd(const void* gate_up, void* h, void* q, float* scale, int64_t rows,
+                         int64_t hidden, int dtype, void* stream);
+int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const void* grad_h, void* grad_gate_up,
+                         int64_t rows, int64_t hidden, int dtype, void* stream);
+
+/* Weight gradient of y = x w^T from x held in 8 bits by rows:
+ * grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m]), fp32 sums in a fixed
+ * order, rounded to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16
+ * (dtype), q int8 [tokens, K], 16-byte aligned; N a multiple of 8, K of 16.
+ * tokens == 0 writes zeros.  Workspace bytes from the query, 16-byte aligned. */
+int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
+                       void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N, int64_t K,
+                       int dtype, void* stream);
+size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, int64_t K);
 
 /* ------------------------------------------------------------------------
  * Plain tcgen05 GEMM (building block; also used by tests)

@@ -1,0 +1,127 @@
+"""Host side of the 8-bit operators: refusals, shapes on meta tensors, and the oracle itself."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from hackable_lm_b200 import _lib, kernels, ops
+from oracle import quant8
+
+
+def test_c_entry_points_refuse_bad_arguments_before_any_launch():
+    lib = _lib.load()
+    V, BF, F32, F16 = ctypes.c_void_p(16), _lib.HLM_BF16, _lib.HLM_F32, _lib.HLM_F16
+    odd = ctypes.c_void_p(24)
+    assert lib.hlm_quantize_rows(V, V, V, -1, 8, BF, None) == -1
+    assert lib.hlm_quantize_rows(V, V, V, 4, 0, BF, None) == -1
+    assert lib.hlm_quantize_rows(None, V, V, 4, 8, BF, None) == -1
+    assert lib.hlm_quantize_rows(V, V, V, 4, 8, 7, None) == -2
+    assert lib.hlm_quantize_rows(None, None, None, 0, 8, BF, None) == 0
+    assert lib.hlm_dequantize_rows(V, None, V, 4, 8, BF, None) == -1
+    assert lib.hlm_dequantize_rows(V, V, V, 4, 8, 9, None) == -2
+    assert lib.hlm_residual_rms_norm_q8(V, V, None, None, V, V, 4, 8, 1e-6, BF, None) == -1  # residual without out
+    assert lib.hlm_residual_rms_norm_q8(None, V, None, None, V, V, 4, 0, 1e-6, BF, None) == -1
+    assert lib.hlm_residual_rms_norm_q8(None, V, None, None, V, V, 4, 8, 1e-6, 5, None) == -2
+    assert lib.hlm_linear_q8(V, V, V, V, V, -1, 8, 16, BF, None) == -1
+    assert lib.hlm_linear_q8(V, V, V, V, None, 1, 8, 16, BF, None) == -1
+    assert lib.hlm_linear_q8(V, V, V, V, V, 1, 8, 0, BF, None) == -2
+    assert lib.hlm_linear_q8(V, V, V, V, V, 1, 8, 24, BF, None) == -2
+    assert lib.hlm_linear_q8(V, V, V, V, V, 1, 8, 131056 + 16, BF, None) == -2
+    assert lib.hlm_linear_q8(V, V, V, V, V, 1, 8, 16, 4, None) == -2
+    assert lib.hlm_linear_q8(odd, V, V, V, V, 1, 8, 16, BF, None) == -2
+    assert lib.hlm_linear_q8(V, V, odd, V, V, 1, 8, 16, F16, None) == -2
+    assert lib.hlm_linear_q8(None, None, None, None, None, 0, 8, 16, F32, None) == 0
+    assert lib.hlm_swiglu_ckpt8_fwd(V, V, V, V, -1, 8, BF, None) == -1
+    assert lib.hlm_swiglu_ckpt8_fwd(V, V, None, V, 1, 8, BF, None) == -1
+    assert lib.hlm_swiglu_ckpt8_fwd(V, V, V, V, 1, 8, 3, None) == -2
+    assert lib.hlm_swiglu_ckpt8_bwd(V, V, V, None, 1, 8, BF, None) == -1
+    assert lib.hlm_swiglu_ckpt8_bwd(None, None, None, None, 0, 8, BF, None) == 0
+    assert lib.hlm_weight_grad_q8(V, V, V, V, None, 0, -1, 8, 16, BF, None) == -1
+    assert lib.hlm_weight_grad_q8(V, V, V, None, None, 0, 4, 8, 16, BF, None) == -1
+    assert lib.hlm_weight_grad_q8(V, V, V, V, None, 0, 4, 12, 16, BF, None) == -2
+    assert lib.hlm_weight_grad_q8(V, V, V, V, None, 0, 4, 8, 24, BF, None) == -2
+    assert lib.hlm_weight_grad_q8(V, V, V, V, None, 0, 4, 8, 16, F32, None) == -2
+    assert lib.hlm_weight_grad_q8(V, odd, V, V, None, 0, 4, 8, 16, BF, None) == -2
+
+
+def test_cpu_tensors_are_rejected():
+    x = torch.randn(4, 32, dtype=torch.bfloat16)
+    q, s = torch.zeros(4, 32, dtype=torch.int8), torch.ones(4)
+    calls = [lambda: kernels.quantize_rows(x), lambda: kernels.dequantize_rows(q, s), lambda: kernels.rms_norm_q8(x, None, 1e-6),
+             lambda: kernels.residual_rms_norm_q8(x, x, 1e-6), lambda: kernels.linear_q8(q, s, q, s),
+             lambda: kernels.swiglu_ckpt8(x), lambda: kernels.linear_ckpt8(x, x), lambda: ops.weight_grad_q8(x, q, s),
+             lambda: ops.swiglu_ckpt8_backward(q, torch.ones(4, 2), x[:, :16]), lambda: ops.quantize_rows(x)]
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_argument_checks():
+    x = torch.zeros(4, 32, dtype=torch.bfloat16)
+    q, s = torch.zeros(4, 32, dtype=torch.int8), torch.ones(4)
+    for bad in (lambda: ops._q8._linear_q8(q, s, q[:, :16], s, torch.bfloat16),            # K differs
+                lambda: ops._q8._linear_q8(q, s[:3], q, s, torch.bfloat16),                 # scales of other rows
+                lambda: ops._q8._linear_q8(x, s, q, s, torch.bfloat16),                     # not codes
+                lambda: ops._q8._linear_q8(q, s, q, s, torch.int32),                        # output type
+                lambda: ops._q8._quantize_rows(q),                                          # input type
+                lambda: ops._q8._quantize_rows(torch.zeros(4, 0)),                          # no columns
+                lambda: ops._q8._dequantize_rows(q, s.half(), torch.float32),
+                lambda: ops._q8._residual_rms_norm_q8(x, x[:2], None, 1e-6),
+                lambda: ops._q8._swiglu_ckpt8(torch.zeros(2, 7)),
+                lambda: ops._q8._swiglu_ckpt8_backward(q, torch.ones(4, 4), x[:, :16]),     # scales of another width
+                lambda: ops._q8._weight_grad_q8(x.float(), q, s),
+                lambda: ops._q8._weight_grad_q8(x[:3], q, s)):
+        with pytest.raises(RuntimeError):
+            bad()
+    w = torch.zeros(5, device="meta")
+    with pytest.raises(RuntimeError):
+        ops._q8._norm_weight("rms_norm_q8", torch.zeros(4, 32, device="meta"), w)
+
+
+def test_shapes_on_meta_tensors():
+    x = torch.empty(2, 3, 64, device="meta", dtype=torch.bfloat16)
+    q, s = kernels.quantize_rows(x)
+    assert q.shape == x.shape and q.dtype == torch.int8 and s.shape == (2, 3) and s.dtype == torch.float32
+    assert kernels.dequantize_rows(q, s, torch.float16).dtype == torch.float16
+    out, q, s = kernels.residual_rms_norm_q8(x, x, 1e-6)
+    assert out.dtype == torch.bfloat16 and q.shape == x.shape
+    w, ws = torch.empty(40, 64, device="meta", dtype=torch.int8), torch.empty(40, device="meta")
+    assert kernels.linear_q8(q, s, w, ws).shape == (2, 3, 40)
+    gu = torch.empty(2, 3, 400, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    h = kernels.swiglu_ckpt8(gu)
+    h.sum().backward()
+    assert h.shape == (2, 3, 200) and gu.grad.shape == gu.shape
+    assert ops.swiglu_ckpt8(gu)[2].shape == (2, 3, 4)
+    xw = torch.empty(2, 3, 64, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    wf = torch.empty(40, 64, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    kernels.linear_ckpt8(xw, wf).sum().backward()
+    assert xw.grad.shape == xw.shape and wf.grad.shape == wf.shape
+
+
+def test_oracle_codes_are_within_half_a_scale():
+    v = torch.randn(50, 300, generator=torch.Generator().manual_seed(0)) * 3
+    q, s = quant8.quantize(v)
+    err = (quant8.read_back(q, s) - v.double()).abs()
+    # half a scale, and the roundings of 127 / a, the product (each 127 u of a code at most) and a / 127
+    assert bool((err <= s.double().unsqueeze(-1) * (0.5 + 4 * 127 * 2.0 ** -24)).all())
+    assert int(q.abs().max()) == 127
+
+
+def test_oracle_swiglu_gradient_against_differences():
+    """The checkpoint's gradient is the derivative of silu(gate) * up at the values read back."""
+    g = torch.Generator().manual_seed(1)
+    gate_up = torch.randn(3, 2 * 200, generator=g)
+    d = torch.randn(3, 200, generator=g)
+    _, q, s = quant8.swiglu_ckpt8(gate_up)
+    grad = quant8.swiglu_ckpt8_backward(q, s, d)
+    qg, qu = q.chunk(2, dim=-1)
+    sg, su = s.chunk(2, dim=-1)
+    gate, up = quant8.group_read_back(qg, sg), quant8.group_read_back(qu, su)
+    f = lambda a, b: d.double() * a * torch.sigmoid(a) * b  # noqa: E731
+    e = 1e-5  # central differences: error e^2 / 6 * third derivative (below 1.5 |d u|) + 1e-16 / e
+    dg = (f(gate + e, up) - f(gate - e, up)) / (2 * e)
+    du = (f(gate, up + e) - f(gate, up - e)) / (2 * e)
+    tol = 1e-9 * (1 + (d.double() * up).abs().max() + (d.double() * gate).abs().max())
+    assert (grad - torch.cat((dg, du), dim=-1)).abs().max() <= tol
