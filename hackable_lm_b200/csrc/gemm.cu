@@ -26,20 +26,28 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-bool encode_bf16_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
-                     uint64_t ld, uint32_t box_outer) {
+bool encode_map(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
+                uint64_t ld, uint32_t box_outer) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return false;
-  if (!host_aligned16(base) || (ld % 8) != 0 || inner == 0 || outer == 0 || ld < inner) return false;
+  if (!host_aligned16(base) || (ld * elem_bytes) % 16 != 0 || inner == 0 || outer == 0 || ld < inner) return false;
+  const CUtensorMapDataType type = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {ld * 2};
-  cuuint32_t box[2] = {64, box_outer};
+  cuuint64_t strides[1] = {ld * elem_bytes};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem_bytes), box_outer};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+      fn(map, type, 2, const_cast<void*>(base), dims, strides, box,
          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+bool encode_bf16_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                     uint64_t ld, uint32_t box_outer) {
+  return encode_map(map, base, 2, inner, outer, ld, box_outer);
 }
 
 template <int BN, bool A_MN, bool B_MN>

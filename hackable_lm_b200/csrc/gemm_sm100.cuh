@@ -1,6 +1,7 @@
 // Persistent warp-specialised tcgen05 GEMM core for sm_100a.
 //
 //   D[M, N] (+)= A[M, K] * B[N, K]^T      bf16 operands, fp32 accumulation in TMEM
+//                                         (Kind = KindS8: int8 operands, int32 sums)
 //
 // Roles (one CTA per SM, grid = min(#tiles, #SMs)):
 //   warp 0      : one thread issues TMA loads (cp.async.bulk.tensor, 128-byte
@@ -126,7 +127,7 @@ HLM_DEVICE bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err) {
   return true;
 }
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
 __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
     gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA0,
                       const __grid_constant__ CUtensorMap tmA1,
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
           armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
           const uint32_t sa = base + stage * L::kStageBytes;
           const uint32_t sb = sa + L::kABytes;
-          const int k0 = kb * kBK;
+          const int k0 = kb * Kind::kBlockK;
           // ---- A
           if constexpr (!A_MN) {
             const CUtensorMap* mp = &tmA0;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16_f32(kBM, BN, A_MN, B_MN);
+      constexpr uint32_t idesc = Kind::idesc(kBM, BN, A_MN, B_MN);
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
                                         : make_sw128_desc(sa + kk * 32u, 16u, 1024u);
             const uint64_t bdesc = B_MN ? make_sw128_desc(sb + kk * 2048u, 8192u, 1024u)
                                         : make_sw128_desc(sb + kk * 32u, 16u, 1024u);
-            tc_mma_f16(d_tmem, adesc, bdesc, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+            Kind::mma(d_tmem, adesc, bdesc, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
           }
           tc_commit(EMPTY_BAR(stage));
           if (++stage == STAGES) {
@@ -352,7 +353,7 @@ struct PairSmem {
   static_assert(BN == 128 || BN == 256 || BN == 384, "pair tile N");
 };
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0,
                      const __grid_constant__ CUtensorMap tmA1,
@@ -435,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
           const uint32_t full = mapa_shared(FULL_BAR(stage), 0);
           const uint32_t sa = base + stage * L::kStageBytes;
           const uint32_t sb = sa + L::kABytes;
-          const int k0 = kb * kBK;
+          const int k0 = kb * Kind::kBlockK;
           if constexpr (!A_MN) {
             const CUtensorMap* mp = &tmA0;
             int kc = k0;
@@ -488,8 +489,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
   } else if (warp == 1) {
     // ------------------------------------------------------------ pair MMA issuer (even CTA)
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc0 = make_idesc_bf16_f32(2 * kBM, L::kN0, A_MN, B_MN);
-      constexpr uint32_t idesc1 = make_idesc_bf16_f32(2 * kBM, L::kN1 > 0 ? L::kN1 : 16, A_MN, B_MN);
+      constexpr uint32_t idesc0 = Kind::idesc(2 * kBM, L::kN0, A_MN, B_MN);
+      constexpr uint32_t idesc1 = Kind::idesc(2 * kBM, L::kN1 > 0 ? L::kN1 : 16, A_MN, B_MN);
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -522,13 +523,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
             const uint64_t bdesc = B_MN ? make_sw128_desc(sb + kk * 2048u, 8192u, 1024u)
                                         : make_sw128_desc(sb + kk * 32u, 16u, 1024u);
             const uint32_t accum = (kb > kb0 || kk > 0) ? 1u : 0u;
-            tc_mma_f16_pair(d_tmem, adesc, bdesc, idesc0, accum);
+            Kind::mma_pair(d_tmem, adesc, bdesc, idesc0, accum);
             if constexpr (L::kN1 > 0) {
               // second MMA: columns [256, BN); its B half starts after the first's
               constexpr uint32_t off = static_cast<uint32_t>(L::kN0 / 2) * 128u;
               const uint64_t bdesc1 = B_MN ? make_sw128_desc(sb + off + kk * 2048u, 8192u, 1024u)
                                            : make_sw128_desc(sb + off + kk * 32u, 16u, 1024u);
-              tc_mma_f16_pair(d_tmem + static_cast<uint32_t>(L::kN0), adesc, bdesc1, idesc1, accum);
+              Kind::mma_pair(d_tmem + static_cast<uint32_t>(L::kN0), adesc, bdesc1, idesc1, accum);
             }
           }
           tc_commit_pair(EMPTY_BAR(stage));
@@ -593,13 +594,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
 //   ld: row stride in elements, box = {64, box_outer}.
 bool encode_bf16_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                      uint64_t ld, uint32_t box_outer);
+// The same for elements of elem_bytes (1: bytes, 2: 16-bit, 4: fp32), box = {128 bytes, box_outer}.
+// The 16-bit map copies fp16 as well as bf16 (no arithmetic on the elements).
+bool encode_map(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
+                uint64_t ld, uint32_t box_outer);
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
 int launch_gemm_sm100(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                       const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                       cudaStream_t stream, int kernel_id) {
   using L = GemmSmem<BN, STAGES>;
-  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS>;
+  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,
                 "shared memory budget exceeded");
@@ -621,12 +626,12 @@ int launch_gemm_sm100(const CUtensorMap& a0, const CUtensorMap& a1, const CUtens
 // epilogues that exchange data across the cluster.  With p.n_tiles == cluster
 // and p.splits == 1, the CTAs of a cluster take the n tiles of one m tile
 // together (work index w = m_tile * n_tiles + n_tile, stepped by the grid).
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
 int launch_gemm_cluster(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                         const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                         int cluster, cudaStream_t stream, int kernel_id) {
   using L = GemmSmem<BN, STAGES>;
-  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS>;
+  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,
                 "shared memory budget exceeded");
@@ -665,12 +670,12 @@ int launch_gemm_cluster(const CUtensorMap& a0, const CUtensorMap& a1, const CUte
 
 // Pair launch: one cluster of two CTAs per two SMs, persistent over the
 // 256 x BN pair tiles (p.m_tiles counts pair tiles: gemm_tiling_pair).
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
 int launch_gemm_pair(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                      const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                      cudaStream_t stream, int kernel_id) {
   using L = PairSmem<BN, STAGES>;
-  auto kern = gemm_pair_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS>;
+  auto kern = gemm_pair_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,
                 "shared memory budget exceeded");
@@ -689,13 +694,13 @@ int launch_gemm_pair(const CUtensorMap& a0, const CUtensorMap& a1, const CUtenso
 }
 
 // Fill the tiling fields of GemmParams.
-inline void gemm_tiling(GemmParams& p, int M, int N, int K, int BN, int splits) {
+inline void gemm_tiling(GemmParams& p, int M, int N, int K, int BN, int splits, int block_k = kBK) {
   p.M = M;
   p.N = N;
   p.K = K;
   p.m_tiles = (M + kBM - 1) / kBM;
   p.n_tiles = (N + BN - 1) / BN;
-  p.k_blocks = (K + kBK - 1) / kBK;
+  p.k_blocks = (K + block_k - 1) / block_k;
   if (splits < 1) splits = 1;
   if (splits > p.k_blocks) splits = p.k_blocks;
   p.kb_per_split = (p.k_blocks + splits - 1) / splits;
@@ -706,8 +711,8 @@ inline void gemm_tiling(GemmParams& p, int M, int N, int K, int BN, int splits) 
 }
 
 // Same for the pair kernel: m_tiles counts 256-row pair tiles.
-inline void gemm_tiling_pair(GemmParams& p, int M, int N, int K, int BN, int splits) {
-  gemm_tiling(p, M, N, K, BN, splits);
+inline void gemm_tiling_pair(GemmParams& p, int M, int N, int K, int BN, int splits, int block_k = kBK) {
+  gemm_tiling(p, M, N, K, BN, splits, block_k);
   p.m_tiles = (M + 2 * kBM - 1) / (2 * kBM);
 }
 

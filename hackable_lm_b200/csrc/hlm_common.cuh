@@ -455,6 +455,62 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16_f32(int M, int N, bool a_
          | (static_cast<uint32_t>(M >> 4) << 24);     // M / 16
 }
 
+// The same two MMAs for 8-bit integer operands: kind::i8, signed bytes in, int32 sums.
+HLM_DEVICE void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+HLM_DEVICE void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor for kind::i8 with signed A/B (both K-major) and int32 D.
+__host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
+  return (2u << 4)                                // D format: s32
+         | (1u << 7)                              // A format: signed
+         | (1u << 10)                             // B format: signed
+         | (static_cast<uint32_t>(N >> 3) << 17)  // N / 8
+         | (static_cast<uint32_t>(M >> 4) << 24); // M / 16
+}
+
+// Operand kinds of the GEMM kernels.  A K block is one 128-byte swizzle row of
+// either (64 bf16 or 128 int8), read by four MMAs of 32 bytes of K each.
+struct KindBf16 {
+  static constexpr int kBlockK = 64;
+  static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
+    return make_idesc_bf16_f32(M, N, a_mn, b_mn);
+  }
+  static HLM_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    tc_mma_f16(d, a, b, idesc, acc);
+  }
+  static HLM_DEVICE void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    tc_mma_f16_pair(d, a, b, idesc, acc);
+  }
+};
+struct KindS8 {
+  static constexpr int kBlockK = 128;
+  static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool, bool) {
+    return make_idesc_s8_s32(M, N);
+  }
+  static HLM_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    tc_mma_i8(d, a, b, idesc, acc);
+  }
+  static HLM_DEVICE void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    tc_mma_i8_pair(d, a, b, idesc, acc);
+  }
+};
+
 // ---------------------------------------------------------------------------
 // Numeric helpers
 // ---------------------------------------------------------------------------

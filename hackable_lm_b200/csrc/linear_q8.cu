@@ -1,29 +1,461 @@
-// 8-bit integer projection: y[m, n] = (sum_k q[m, k] w[n, k]) * scale[m] * w_scale[n],
-// q and w int8 (K contiguous), exact int32 sums.
-#include "quant_common.cuh"
+// 8-bit integer projection:
+//
+//   y[m, n] = (sum_k q[m, k] w[n, k]) * scale[m] * w_scale[n]
+//
+// q [M, K] and w [N, K] int8 with K contiguous, exact int32 sums (any order gives
+// the same bits), the two scales applied in fp32, one rounding to the output type.
+// Three kernels, by M and the number of output tiles:
+//
+//  - rows kernel, M <= 8: one pass over the weights with dp4a; bound by
+//    reading w (and by launch latency at small sizes).
+//  - split kernel, fewer 128 x 128 output tiles than SMs: weights as the
+//    128-row MMA operand, tokens as the 16..128-column one, K split over a
+//    thread-block cluster whose CTAs add their int32 partial tiles through
+//    distributed shared memory (no workspace, one launch).
+//  - pair kernel, otherwise: the persistent CTA-pair GEMM of gemm_sm100.cuh with
+//    kind::i8 (256 x 256 tiles) and the scales in its epilogue.
+#include "gemm_sm100.cuh"
 
 namespace hlm {
 
 template <typename T>
-__global__ void __launch_bounds__(256) linear_q8_simple_kernel(
+HLM_DEVICE uint32_t pack2(float a, float b);
+template <>
+HLM_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  return pack_bf16x2(a, b);
+}
+template <>
+HLM_DEVICE uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+HLM_DEVICE T scaled(int acc, float row_scale, float col_scale) {
+  return from_f32<T>(static_cast<float>(acc) * row_scale * col_scale);
+}
+
+// ---------------------------------------------------------------------------
+// M <= 8: a warp per R output channels, lanes along K.
+// ---------------------------------------------------------------------------
+template <typename T, int MR, int R>
+__global__ void __launch_bounds__(128) linear_q8_rows_kernel(
     const int8_t* __restrict__ q, const float* __restrict__ scale, const int8_t* __restrict__ w,
-    const float* __restrict__ w_scale, T* __restrict__ out, int64_t M, int64_t N, int64_t K) {
-  const int64_t total = M * N;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t m = i / N, n = i - m * N;
-    const int8_t* a = q + m * K;
-    const int8_t* b = w + n * K;
-    int acc = 0;
-    for (int64_t k = 0; k < K; k += 16) {
-      const uint4 x = ld_global_v4(a + k), y = ld_global_v4(b + k);
-      acc = __dp4a(static_cast<int>(x.x), static_cast<int>(y.x), acc);
-      acc = __dp4a(static_cast<int>(x.y), static_cast<int>(y.y), acc);
-      acc = __dp4a(static_cast<int>(x.z), static_cast<int>(y.z), acc);
-      acc = __dp4a(static_cast<int>(x.w), static_cast<int>(y.w), acc);
+    const float* __restrict__ w_scale, T* __restrict__ out, int M, int N, int K) {
+  const int lane = threadIdx.x & 31;
+  const int64_t n0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * R;
+  if (n0 >= N) return;
+  int acc[R][MR];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[r][m] = 0;
+#pragma unroll 2
+  for (int k = lane * 16; k < K; k += 512) {
+    uint4 wv[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t n = n0 + r < N ? n0 + r : N - 1;  // the last warp's spare rows repeat a row
+      wv[r] = ld_global_nc_v4(w + n * K + k);
     }
-    out[i] = from_f32<T>(static_cast<float>(acc) * scale[m] * w_scale[n]);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const int mm = m < M ? m : M - 1;
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + static_cast<int64_t>(mm) * K + k));
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].x), static_cast<int>(x.x), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].y), static_cast<int>(x.y), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].z), static_cast<int>(x.z), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].w), static_cast<int>(x.w), acc[r][m]);
+      }
+    }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[r][m] = __reduce_add_sync(0xffffffffu, acc[r][m]);
+  // lane r * MR + m writes output (m, n0 + r)
+  int mine = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+      if (lane == r * MR + m) mine = acc[r][m];
+  const int r = lane / MR, m = lane - r * MR;
+  if (r < R && m < M && n0 + r < N)
+    out[static_cast<int64_t>(m) * N + n0 + r] = scaled<T>(mine, scale[m], w_scale[n0 + r]);
+}
+
+// ---------------------------------------------------------------------------
+// Few output tiles: K split over a cluster.
+// ---------------------------------------------------------------------------
+constexpr int kSplitThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
+constexpr int kMaxSplits = 8;       // portable cluster size
+
+template <int MT>
+struct SplitSmem {
+  static constexpr int kStages = MT <= 64 ? 8 : 6;
+  static constexpr int kABytes = 128 * 128;  // 128 output channels x 128 bytes of K
+  static constexpr int kBBytes = MT * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kBarOffset = kStages * kStageBytes;
+  static constexpr int kTmemSlotOffset = kBarOffset + (2 * kStages + 1) * 8;
+  static constexpr int kBytes = kTmemSlotOffset + 16 + 1024;
+  static constexpr int kTmemCols = MT < 32 ? 32 : MT;
+  static_assert(MT * 128 * 4 <= kBarOffset, "the partial tile reuses the stages");
+  static_assert(kBytes <= 232448, "shared memory budget exceeded");
+};
+
+HLM_DEVICE int ld_shared_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+HLM_DEVICE uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// One output tile (128 channels x MT tokens) per cluster; CTA `rank` sums K blocks
+// [rank * kb_per, ...).  Each CTA leaves its int32 partial tile in its own shared
+// memory as [token][channel]; after a cluster barrier, token columns rank,
+// rank + S, ... are added over the S CTAs, scaled and written (128 consecutive
+// channels of one token per warp row: coalesced).
+template <typename T, int MT>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    linear_q8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_q,
+                           const float* __restrict__ scale, const float* __restrict__ w_scale,
+                           T* __restrict__ out, int M, int N, int k_blocks, int kb_per, int* err) {
+  using L = SplitSmem<MT>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw_addr);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t bar0 = base + L::kBarOffset;
+  const uint32_t done_bar = bar0 + 8u * (2 * L::kStages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + L::kTmemSlotOffset);
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int splits = static_cast<int>(cluster_nctarank());
+  const int n0 = static_cast<int>(cluster_id_x()) * 128;
+  const int m0 = static_cast<int>(blockIdx.y) * MT;
+  const int kb0 = rank * kb_per;
+  const int kb1 = min(kb0 + kb_per, k_blocks);
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(bar0 + 8u * s, 1);
+      mbar_init(bar0 + 8u * (L::kStages + s), 1);
+    }
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_q);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, armed_mask = 0, armed_par = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(bar0 + 8u * (L::kStages + stage), phase ^ 1u, err, kDevErrTimeoutEmpty)) break;
+        const uint32_t full = bar0 + 8u * stage;
+        mbar_arrive_expect_tx(full, L::kStageBytes);
+        armed_mask |= 1u << stage;
+        armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+        const uint32_t sa = base + stage * L::kStageBytes;
+        tma_load_2d(sa, &tm_w, kb * KindS8::kBlockK, n0, full);
+        tma_load_2d(sa + L::kABytes, &tm_q, kb * KindS8::kBlockK, m0, full);
+        if (++stage == L::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      for (int s = 0; s < L::kStages; ++s)
+        if (armed_mask & (1u << s)) mbar_wait_drain(bar0 + 8u * s, (armed_par >> s) & 1u, err);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_s8_s32(128, MT);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(bar0 + 8u * stage, phase, err, kDevErrTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t sa = base + stage * L::kStageBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_i8(tmem_base, make_sw128_desc(sa + kk * 32u, 16u, 1024u),
+                    make_sw128_desc(sa + L::kABytes + kk * 32u, 16u, 1024u), idesc,
+                    (kb > kb0 || kk > 0) ? 1u : 0u);
+        tc_commit(bar0 + 8u * (L::kStages + stage));
+        if (++stage == L::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) tc_commit(done_bar);
+    }
+  } else {
+    // partial tile -> shared memory.  The MMAs are done with the stages once
+    // done_bar completes, and every load they read has landed.
+    const int quad = warp & 3;
+    if (warp_wait(done_bar, 0, err, kDevErrTimeoutTmemFull, lane)) {
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+      int* part = reinterpret_cast<int*>(base_ptr) + quad * 32 + lane;
+#pragma unroll 1
+      for (int c = 0; c < L::kTmemCols; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < MT) part[(c + j) * 128] = static_cast<int>(r[j]);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // every partial tile of the cluster is written
+  {
+    const int tokens = min(MT, M - m0);
+    const int n = n0 + static_cast<int>(threadIdx.x);
+    if (threadIdx.x < 128 && n < N) {
+      const float cs = w_scale[n];
+      const uint32_t mine = base + threadIdx.x * 4u;
+      for (int c = rank; c < tokens; c += splits) {
+        int sum = 0;
+        for (int s = 0; s < splits; ++s)
+          sum += ld_shared_cluster_s32(mapa_shared(mine + static_cast<uint32_t>(c) * 512u, static_cast<uint32_t>(s)));
+        out[static_cast<int64_t>(m0 + c) * N + n] = scaled<T>(sum, scale[m0 + c], cs);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while a peer reads its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many output tiles: CTA-pair GEMM with the scales in the epilogue.
+// ---------------------------------------------------------------------------
+// Per warp (32 rows) and group of 128 output bytes (64 or 32 columns): int32
+// columns from TMEM, scaled, staged as a 32 x 128-byte box and stored by TMA.
+// Outputs whose rows are not 16-byte multiples leave the box by rows instead
+// (one coalesced row segment per step).
+template <typename T>
+struct EpiScaleQ8 {
+  struct Params {
+    alignas(64) CUtensorMap map_out;
+    T* out;
+    const float* row_scale;
+    const float* col_scale;
+    int tma;
+  };
+  static constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a group
+  static constexpr int kBoxBytes = 32 * 128;
+  static constexpr int kBufs = 2;
+  static constexpr int kWarpBytes = kBufs * kBoxBytes + 256;  // boxes, then the group's column scales
+  template <int EPI_WARPS>
+  static constexpr int smem_bytes() {
+    return EPI_WARPS * kWarpBytes;
+  }
+
+  template <int BN, int kParts>
+  static HLM_DEVICE void run(const Params& ep, const GemmParams& p, uint8_t* smem, uint32_t taddr,
+                             int m_tile, int n_tile, int, int quad, int part, int lane) {
+    // boxes of all warps first (1024-byte aligned for the swizzle), then their column scales
+    constexpr int kWarps = 4 * kParts;
+    const int slot = part * 4 + quad;
+    uint8_t* boxes = smem + slot * kBufs * kBoxBytes;
+    float* cs_ptr = reinterpret_cast<float*>(smem + kWarps * kBufs * kBoxBytes + slot * 256);
+    const uint32_t cs_addr = smem_u32(cs_ptr);
+    const int row0 = m_tile * kBM + quad * 32;
+    const int row = row0 + lane;
+    const float rs = row < p.M ? ep.row_scale[row] : 0.0f;
+    int k = 0;
+#pragma unroll 1
+    for (int g = part; g < BN / kCols; g += kParts, ++k) {
+      const int col0 = n_tile * BN + g * kCols;
+      if (col0 >= p.N) break;  // the same for the whole warp
+      uint8_t* box = boxes + (k & 1) * kBoxBytes;
+      const uint32_t buf = smem_u32(box);
+      if (ep.tma && lane == 0) {  // this box's last store has read it (a tile starts over at box 0)
+        if (k == 0)
+          bulk_wait_group_read<0>();
+        else
+          bulk_wait_group_read<kBufs - 1>();
+      }
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const int col = col0 + 32 * i + lane;
+        cs_ptr[32 * i + lane] = col < p.N ? ep.col_scale[col] : 0.0f;
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int hs = 0; hs < kCols / 32; ++hs) {
+        uint32_t a[32];
+        tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * kCols + hs * 32), a);
+        tmem_ld_wait();
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint4 c4 = ld_shared_v4(cs_addr + static_cast<uint32_t>(hs * 128 + j * 16));
+          f[4 * j] = static_cast<float>(static_cast<int>(a[4 * j])) * rs * __uint_as_float(c4.x);
+          f[4 * j + 1] = static_cast<float>(static_cast<int>(a[4 * j + 1])) * rs * __uint_as_float(c4.y);
+          f[4 * j + 2] = static_cast<float>(static_cast<int>(a[4 * j + 2])) * rs * __uint_as_float(c4.z);
+          f[4 * j + 3] = static_cast<float>(static_cast<int>(a[4 * j + 3])) * rs * __uint_as_float(c4.w);
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + ((c ^ (lane & 7)) << 4)),
+                         make_uint4(__float_as_uint(f[4 * c]), __float_as_uint(f[4 * c + 1]),
+                                    __float_as_uint(f[4 * c + 2]), __float_as_uint(f[4 * c + 3])));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int cc = hs * 4 + c;
+            st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + ((cc ^ (lane & 7)) << 4)),
+                         make_uint4(pack2<T>(f[8 * c], f[8 * c + 1]), pack2<T>(f[8 * c + 2], f[8 * c + 3]),
+                                    pack2<T>(f[8 * c + 4], f[8 * c + 5]), pack2<T>(f[8 * c + 6], f[8 * c + 7])));
+          }
+        }
+      }
+      if (ep.tma) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && row0 < p.M) {
+          tma_store_2d(&ep.map_out, col0, row0, buf);
+          bulk_commit_group();
+        }
+      } else {
+        __syncwarp();
+        constexpr int kPerChunk = 16 / static_cast<int>(sizeof(T));
+        const int rows = min(32, p.M - row0);
+        for (int r = 0; r < rows; ++r) {
+#pragma unroll
+          for (int i = 0; i < kCols / 32; ++i) {
+            const int c = 32 * i + lane;
+            const T v = *reinterpret_cast<const T*>(box + r * 128 + (((c / kPerChunk) ^ (r & 7)) << 4) +
+                                                    (c % kPerChunk) * static_cast<int>(sizeof(T)));
+            if (col0 + c < p.N) ep.out[static_cast<int64_t>(row0 + r) * p.N + col0 + c] = v;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+};
+
+constexpr int kQ8Stages = 6;
+constexpr int kQ8EpiWarps = 4;
+
+template <typename T, int BN>
+static int linear_q8_pair(const void* q, const float* scale, const void* w, const float* w_scale, T* out,
+                          int64_t M, int64_t N, int64_t K, int* err, cudaStream_t s) {
+  CUtensorMap ma, mb;
+  if (!encode_map(&ma, q, 1, K, M, K, kBM) || !encode_map(&mb, w, 1, K, N, K, 64)) return HLM_ERR_DRIVER;
+  typename EpiScaleQ8<T>::Params ep;
+  ep.out = out;
+  ep.row_scale = scale;
+  ep.col_scale = w_scale;
+  ep.tma = (N * static_cast<int64_t>(sizeof(T))) % 16 == 0 && host_aligned16(out);
+  ep.map_out = mb;  // only read when ep.tma
+  if (ep.tma && !encode_map(&ep.map_out, out, sizeof(T), N, M, N, 32)) return HLM_ERR_DRIVER;
+  GemmParams p;
+  gemm_tiling_pair(p, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), BN, 1, KindS8::kBlockK);
+  p.err = err;
+  return launch_gemm_pair<BN, kQ8Stages, false, false, EpiScaleQ8<T>, kQ8EpiWarps, KindS8>(
+      ma, ma, ma, mb, p, ep, s, HLM_KERNEL_LINEAR_Q8);
+}
+
+template <typename T, int MT>
+static int linear_q8_split(const void* q, const float* scale, const void* w, const float* w_scale, T* out,
+                           int64_t M, int64_t N, int64_t K, int* err, cudaStream_t s) {
+  using L = SplitSmem<MT>;
+  CUtensorMap mw, mq;
+  if (!encode_map(&mw, w, 1, K, N, K, 128) || !encode_map(&mq, q, 1, K, M, K, MT)) return HLM_ERR_DRIVER;
+  const int n_tiles = static_cast<int>((N + 127) / 128), m_tiles = static_cast<int>((M + MT - 1) / MT);
+  const int k_blocks = static_cast<int>((K + KindS8::kBlockK - 1) / KindS8::kBlockK);
+  int splits = num_sms_of_current_device() / (n_tiles * m_tiles);
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  if (splits > k_blocks) splits = k_blocks;
+  if (splits < 1) splits = 1;
+  const int kb_per = (k_blocks + splits - 1) / splits;
+  splits = (k_blocks + kb_per - 1) / kb_per;
+  auto kern = linear_q8_split_kernel<T, MT>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+    return HLM_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles), 1);
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  {
+    LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
+    if (cudaLaunchKernelEx(&cfg, kern, mw, mq, scale, w_scale, out, static_cast<int>(M), static_cast<int>(N),
+                           k_blocks, kb_per, err) != cudaSuccess)
+      return HLM_ERR_LAUNCH;
+  }
+  return launch_status();
+}
+
+template <typename T, int MR>
+static int linear_q8_rows(const void* q, const float* scale, const void* w, const float* w_scale, T* out,
+                          int64_t M, int64_t N, int64_t K, cudaStream_t s) {
+  constexpr int R = 2;
+  constexpr int kWarps = 4;
+  const int64_t blocks = (N + R * kWarps - 1) / (R * kWarps);
+  LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
+  linear_q8_rows_kernel<T, MR, R><<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(
+      static_cast<const int8_t*>(q), scale, static_cast<const int8_t*>(w), w_scale, out, static_cast<int>(M),
+      static_cast<int>(N), static_cast<int>(K));
+  return launch_status();
+}
+
+template <typename T>
+static int linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, T* out, int64_t M,
+                     int64_t N, int64_t K, cudaStream_t s) {
+  if (M == 1) return linear_q8_rows<T, 1>(q, scale, w, w_scale, out, M, N, K, s);
+  if (M <= 4) return linear_q8_rows<T, 4>(q, scale, w, w_scale, out, M, N, K, s);
+  if (M <= 8) return linear_q8_rows<T, 8>(q, scale, w, w_scale, out, M, N, K, s);
+  int* err = device_error_ptr();
+  if (err == nullptr) return HLM_ERR_LAUNCH;
+  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  if (M <= 128 || tiles <= num_sms_of_current_device()) {
+    if (M <= 16) return linear_q8_split<T, 16>(q, scale, w, w_scale, out, M, N, K, err, s);
+    if (M <= 32) return linear_q8_split<T, 32>(q, scale, w, w_scale, out, M, N, K, err, s);
+    if (M <= 64) return linear_q8_split<T, 64>(q, scale, w, w_scale, out, M, N, K, err, s);
+    return linear_q8_split<T, 128>(q, scale, w, w_scale, out, M, N, K, err, s);
+  }
+  return linear_q8_pair<T, 256>(q, scale, w, w_scale, out, M, N, K, err, s);
 }
 
 }  // namespace hlm
@@ -43,20 +475,12 @@ extern "C" int hlm_linear_q8(const void* q, const float* scale, const void* w, c
   if (M > (1ll << 31) - 512 || N > (1ll << 31) - 512) return HLM_ERR_UNSUPPORTED;
   if (!host_aligned16(q) || !host_aligned16(w)) return HLM_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t blocks64 = (M * N + 255) / 256;
-  const int64_t cap = static_cast<int64_t>(num_sms_of_current_device()) * 64;
-  const int blocks = static_cast<int>(blocks64 < cap ? blocks64 : cap);
-  LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
-  const int8_t* qp = static_cast<const int8_t*>(q);
-  const int8_t* wp = static_cast<const int8_t*>(w);
-  if (out_dtype == HLM_BF16)
-    linear_q8_simple_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(
-        qp, scale, wp, w_scale, static_cast<__nv_bfloat16*>(out), M, N, K);
-  else if (out_dtype == HLM_F16)
-    linear_q8_simple_kernel<__half><<<blocks, 256, 0, s>>>(qp, scale, wp, w_scale,
-                                                           static_cast<__half*>(out), M, N, K);
-  else
-    linear_q8_simple_kernel<float><<<blocks, 256, 0, s>>>(qp, scale, wp, w_scale,
-                                                          static_cast<float*>(out), M, N, K);
-  return launch_status();
+  switch (out_dtype) {
+    case HLM_BF16:
+      return linear_q8<__nv_bfloat16>(q, scale, w, w_scale, static_cast<__nv_bfloat16*>(out), M, N, K, s);
+    case HLM_F16:
+      return linear_q8<__half>(q, scale, w, w_scale, static_cast<__half*>(out), M, N, K, s);
+    default:
+      return linear_q8<float>(q, scale, w, w_scale, static_cast<float*>(out), M, N, K, s);
+  }
 }
