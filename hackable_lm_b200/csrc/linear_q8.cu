@@ -95,22 +95,23 @@ constexpr int kMaxSplits = 8;       // portable cluster size
 
 template <int MT>
 struct SplitSmem {
-  static constexpr int kStages = MT <= 64 ? 8 : 6;
+  static constexpr int kStages = MT <= 64 ? 6 : 4;
   static constexpr int kABytes = 128 * 128;  // 128 output channels x 128 bytes of K
   static constexpr int kBBytes = MT * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kBarOffset = kStages * kStageBytes;
+  // partial sums from every CTA of the cluster for the token columns that this one
+  // owns: [CTA][owned column][channel] int32; at most MT + 7 columns in all
+  static constexpr int kPartOffset = kStages * kStageBytes;
+  static constexpr int kPartBytes = (MT + kMaxSplits) * 128 * 4;
+  static constexpr int kBarOffset = kPartOffset + kPartBytes;
   static constexpr int kTmemSlotOffset = kBarOffset + (2 * kStages + 1) * 8;
   static constexpr int kBytes = kTmemSlotOffset + 16 + 1024;
   static constexpr int kTmemCols = MT < 32 ? 32 : MT;
-  static_assert(MT * 128 * 4 <= kBarOffset, "the partial tile reuses the stages");
   static_assert(kBytes <= 232448, "shared memory budget exceeded");
 };
 
-HLM_DEVICE int ld_shared_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+HLM_DEVICE void st_shared_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 HLM_DEVICE uint32_t cluster_nctarank() {
   uint32_t r;
@@ -119,15 +120,16 @@ HLM_DEVICE uint32_t cluster_nctarank() {
 }
 
 // One output tile (128 channels x MT tokens) per cluster; CTA `rank` sums K blocks
-// [rank * kb_per, ...).  Each CTA leaves its int32 partial tile in its own shared
-// memory as [token][channel]; after a cluster barrier, token columns rank,
-// rank + S, ... are added over the S CTAs, scaled and written (128 consecutive
-// channels of one token per warp row: coalesced).
+// [rank * kb_per, ...).  Token column c belongs to CTA c mod S: every CTA writes its
+// int32 partial of that column (128 channels) into the owner's shared memory, and
+// after one cluster barrier the owner adds the S partials, scales and writes them.
+// Nothing is read remotely (such loads, one latency after the other, cost 16 us at
+// 128 tokens), and no CTA touches a peer's memory after the barrier.
 template <typename T, int MT>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     linear_q8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_q,
                            const float* __restrict__ scale, const float* __restrict__ w_scale,
-                           T* __restrict__ out, int M, int N, int k_blocks, int kb_per, int* err) {
+                           T* __restrict__ out, int M, int N, int k_blocks, int kb_per, int vec, int* err) {
   using L = SplitSmem<MT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -144,6 +146,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   const int m0 = static_cast<int>(blockIdx.y) * MT;
   const int kb0 = rank * kb_per;
   const int kb1 = min(kb0 + kb_per, k_blocks);
+  const int tokens = min(MT, M - m0);
+  const int per = (tokens + splits - 1) / splits;  // columns that one CTA owns, at most
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < L::kStages; ++s) {
@@ -160,7 +164,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();  // barriers are set up, and every CTA of the cluster runs (its memory may be written)
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
@@ -212,43 +217,66 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       if (ok) tc_commit(done_bar);
     }
   } else {
-    // partial tile -> shared memory.  The MMAs are done with the stages once
-    // done_bar completes, and every load they read has landed.
     const int quad = warp & 3;
     if (warp_wait(done_bar, 0, err, kDevErrTimeoutTmemFull, lane)) {
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-      int* part = reinterpret_cast<int*>(base_ptr) + quad * 32 + lane;
+      // slot of column c: CTA c % splits, row rank * per + c / splits
+      const uint32_t mine = base + L::kPartOffset + static_cast<uint32_t>((rank * per * 128 + quad * 32 + lane) * 4);
+      int owner = 0;
+      uint32_t slot = 0;
 #pragma unroll 1
-      for (int c = 0; c < L::kTmemCols; c += 32) {
+      for (int c = 0; c < tokens; c += 32) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(c), r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < MT) part[(c + j) * 128] = static_cast<int>(r[j]);
+        for (int j = 0; j < 32; ++j) {
+          if (c + j < tokens) st_shared_cluster_u32(mapa_shared(mine + slot, static_cast<uint32_t>(owner)), r[j]);
+          if (++owner == splits) {
+            owner = 0;
+            slot += 512u;
+          }
+        }
       }
       tc_fence_before();
     }
   }
   __syncwarp();
-  cluster_sync_all();  // every partial tile of the cluster is written
+  cluster_sync_all();  // every partial of this CTA's columns has arrived
   {
-    const int tokens = min(MT, M - m0);
-    const int n = n0 + static_cast<int>(threadIdx.x);
-    if (threadIdx.x < 128 && n < N) {
-      const float cs = w_scale[n];
-      const uint32_t mine = base + threadIdx.x * 4u;
-      for (int c = rank; c < tokens; c += splits) {
-        int sum = 0;
-        for (int s = 0; s < splits; ++s)
-          sum += ld_shared_cluster_s32(mapa_shared(mine + static_cast<uint32_t>(c) * 512u, static_cast<uint32_t>(s)));
-        out[static_cast<int64_t>(m0 + c) * N + n] = scaled<T>(sum, scale[m0 + c], cs);
+    // a warp per owned column, four channels per lane
+    const int n = n0 + 4 * lane;
+    float cs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = n + i < N ? w_scale[n + i] : 0.0f;
+    for (int i = warp; rank + i * splits < tokens; i += kSplitThreads / 32) {
+      const int m = m0 + rank + i * splits;
+      int4 sum = make_int4(0, 0, 0, 0);
+      uint32_t addr = base + L::kPartOffset + static_cast<uint32_t>(i * 512 + lane * 16);
+      for (int s = 0; s < splits; ++s, addr += static_cast<uint32_t>(per) * 512u) {
+        const uint4 v = ld_shared_v4(addr);
+        sum.x += static_cast<int>(v.x);
+        sum.y += static_cast<int>(v.y);
+        sum.z += static_cast<int>(v.z);
+        sum.w += static_cast<int>(v.w);
+      }
+      const float rs = scale[m];
+      alignas(16) const T y[4] = {scaled<T>(sum.x, rs, cs[0]), scaled<T>(sum.y, rs, cs[1]), scaled<T>(sum.z, rs, cs[2]),
+                      scaled<T>(sum.w, rs, cs[3])};
+      T* dst = out + static_cast<int64_t>(m) * N + n;
+      if (vec && n + 4 <= N) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+        else
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + k < N) dst[k] = y[k];
       }
     }
   }
-  __syncwarp();
-  cluster_sync_all();  // no CTA leaves while a peer reads its shared memory
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
@@ -259,22 +287,24 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // Many output tiles: CTA-pair GEMM with the scales in the epilogue.
 // ---------------------------------------------------------------------------
 // Per warp (32 rows) and group of 128 output bytes (64 or 32 columns): int32
-// columns from TMEM, scaled, staged as a 32 x 128-byte box and stored by TMA.
-// Outputs whose rows are not 16-byte multiples leave the box by rows instead
-// (one coalesced row segment per step).
+// columns from TMEM (one row per lane), scaled, staged as a 32 x 128-byte box
+// (16-byte chunks swizzled by row) and written out with 16-byte stores, four
+// whole 128-byte row segments per instruction.  Plain stores and not TMA: nothing
+// waits for them, while TMA stores of the two boxes that fit per warp held the
+// epilogue at 3 TB/s.  Outputs whose rows are not 16-byte multiples leave the box
+// element by element, a row segment per step.
 template <typename T>
 struct EpiScaleQ8 {
   struct Params {
-    alignas(64) CUtensorMap map_out;
     T* out;
     const float* row_scale;
     const float* col_scale;
-    int tma;
+    int vec;  // rows of the output are 16-byte aligned
   };
   static constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a group
+  static constexpr int kPerChunk = 16 / static_cast<int>(sizeof(T));
   static constexpr int kBoxBytes = 32 * 128;
-  static constexpr int kBufs = 2;
-  static constexpr int kWarpBytes = kBufs * kBoxBytes + 256;  // boxes, then the group's column scales
+  static constexpr int kWarpBytes = kBoxBytes + 256;  // box, then the group's column scales
   template <int EPI_WARPS>
   static constexpr int smem_bytes() {
     return EPI_WARPS * kWarpBytes;
@@ -283,35 +313,25 @@ struct EpiScaleQ8 {
   template <int BN, int kParts>
   static HLM_DEVICE void run(const Params& ep, const GemmParams& p, uint8_t* smem, uint32_t taddr,
                              int m_tile, int n_tile, int, int quad, int part, int lane) {
-    // boxes of all warps first (1024-byte aligned for the swizzle), then their column scales
-    constexpr int kWarps = 4 * kParts;
-    const int slot = part * 4 + quad;
-    uint8_t* boxes = smem + slot * kBufs * kBoxBytes;
-    float* cs_ptr = reinterpret_cast<float*>(smem + kWarps * kBufs * kBoxBytes + slot * 256);
-    const uint32_t cs_addr = smem_u32(cs_ptr);
+    uint8_t* box = smem + (part * 4 + quad) * kWarpBytes;
+    const uint32_t buf = smem_u32(box);
+    float* cs_ptr = reinterpret_cast<float*>(box + kBoxBytes);
+    const uint32_t cs_addr = buf + kBoxBytes;
     const int row0 = m_tile * kBM + quad * 32;
     const int row = row0 + lane;
     const float rs = row < p.M ? ep.row_scale[row] : 0.0f;
-    int k = 0;
 #pragma unroll 1
-    for (int g = part; g < BN / kCols; g += kParts, ++k) {
+    for (int g = part; g < BN / kCols; g += kParts) {
       const int col0 = n_tile * BN + g * kCols;
       if (col0 >= p.N) break;  // the same for the whole warp
-      uint8_t* box = boxes + (k & 1) * kBoxBytes;
-      const uint32_t buf = smem_u32(box);
-      if (ep.tma && lane == 0) {  // this box's last store has read it (a tile starts over at box 0)
-        if (k == 0)
-          bulk_wait_group_read<0>();
-        else
-          bulk_wait_group_read<kBufs - 1>();
-      }
+      __syncwarp();            // the box's last group has been read
 #pragma unroll
       for (int i = 0; i < kCols / 32; ++i) {
         const int col = col0 + 32 * i + lane;
         cs_ptr[32 * i + lane] = col < p.N ? ep.col_scale[col] : 0.0f;
       }
       __syncwarp();
-#pragma unroll 1
+#pragma unroll
       for (int hs = 0; hs < kCols / 32; ++hs) {
         uint32_t a[32];
         tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * kCols + hs * 32), a);
@@ -341,16 +361,18 @@ struct EpiScaleQ8 {
           }
         }
       }
-      if (ep.tma) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && row0 < p.M) {
-          tma_store_2d(&ep.map_out, col0, row0, buf);
-          bulk_commit_group();
+      __syncwarp();
+      if (ep.vec) {
+        const int chunk = lane & 7;
+        const bool col_ok = col0 + chunk * kPerChunk < p.N;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          const uint4 v = ld_shared_v4(buf + static_cast<uint32_t>(r * 128 + ((chunk ^ (r & 7)) << 4)));
+          if (col_ok && row0 + r < p.M)
+            st_global_v4(ep.out + static_cast<int64_t>(row0 + r) * p.N + col0 + chunk * kPerChunk, v);
         }
       } else {
-        __syncwarp();
-        constexpr int kPerChunk = 16 / static_cast<int>(sizeof(T));
         const int rows = min(32, p.M - row0);
         for (int r = 0; r < rows; ++r) {
 #pragma unroll
@@ -362,13 +384,12 @@ struct EpiScaleQ8 {
           }
         }
       }
-      __syncwarp();
     }
   }
 };
 
-constexpr int kQ8Stages = 6;
-constexpr int kQ8EpiWarps = 4;
+constexpr int kQ8Stages = 5;
+constexpr int kQ8EpiWarps = 8;
 
 template <typename T, int BN>
 static int linear_q8_pair(const void* q, const float* scale, const void* w, const float* w_scale, T* out,
@@ -379,9 +400,7 @@ static int linear_q8_pair(const void* q, const float* scale, const void* w, cons
   ep.out = out;
   ep.row_scale = scale;
   ep.col_scale = w_scale;
-  ep.tma = (N * static_cast<int64_t>(sizeof(T))) % 16 == 0 && host_aligned16(out);
-  ep.map_out = mb;  // only read when ep.tma
-  if (ep.tma && !encode_map(&ep.map_out, out, sizeof(T), N, M, N, 32)) return HLM_ERR_DRIVER;
+  ep.vec = (N * static_cast<int64_t>(sizeof(T))) % 16 == 0 && host_aligned16(out);
   GemmParams p;
   gemm_tiling_pair(p, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), BN, 1, KindS8::kBlockK);
   p.err = err;
@@ -412,6 +431,8 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  // four outputs of a lane as one store
+  const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
   cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles), 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
   cfg.dynamicSmemBytes = L::kBytes;
@@ -421,7 +442,7 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   {
     LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
     if (cudaLaunchKernelEx(&cfg, kern, mw, mq, scale, w_scale, out, static_cast<int>(M), static_cast<int>(N),
-                           k_blocks, kb_per, err) != cudaSuccess)
+                           k_blocks, kb_per, vec, err) != cudaSuccess)
       return HLM_ERR_LAUNCH;
   }
   return launch_status();
