@@ -53,6 +53,17 @@ template <class E>
 struct epi_cluster_exchange<E, std::void_t<decltype(E::kClusterExchange)>>
     : std::integral_constant<bool, E::kClusterExchange> {};
 
+// Epilogues that write their results with plain global stores declare
+// `static constexpr bool kRelaxedRelease = true`: the pair kernel then hands the
+// accumulator back without a release, which would wait for those stores to land.
+// What the MMA issuer may overwrite is the accumulator alone, and its tcgen05.ld
+// have completed (tcgen05.wait::ld) before the arrive.
+template <class E, class = void>
+struct epi_relaxed_release : std::false_type {};
+template <class E>
+struct epi_relaxed_release<E, std::void_t<decltype(E::kRelaxedRelease)>>
+    : std::integral_constant<bool, E::kRelaxedRelease> {};
+
 constexpr int kBM = 128;
 constexpr int kBK = 64;  // 64 bf16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
@@ -564,7 +575,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
                                     lane);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(TEMPTY_BAR(acc), 0));
+      if (lane == 0) {
+        if constexpr (epi_relaxed_release<Epi>::value)
+          mbar_arrive_cluster_relaxed(mapa_shared(TEMPTY_BAR(acc), 0));
+        else
+          mbar_arrive_cluster(mapa_shared(TEMPTY_BAR(acc), 0));
+      }
     }
     if (lane == 0) bulk_wait_group_all();
     __syncwarp();

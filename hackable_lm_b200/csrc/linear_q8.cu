@@ -301,6 +301,7 @@ struct EpiScaleQ8 {
     const float* col_scale;
     int vec;  // rows of the output are 16-byte aligned
   };
+  static constexpr bool kRelaxedRelease = true;
   static constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a group
   static constexpr int kPerChunk = 16 / static_cast<int>(sizeof(T));
   static constexpr int kBoxBytes = 32 * 128;
