@@ -38,17 +38,36 @@ def _direct(*tensors: Optional[torch.Tensor]) -> bool:
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
-def _call(dev: torch.device, name: str, *args) -> None:
-    """Library call on the current stream of ``dev``, with ``dev`` current for its duration."""
-    fn = getattr(_lib.load(), name)
-    idx = dev.index
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() builds an object around it (1.2 us)
+
+
+def _device_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the CUDA device that all the tensors are on (raises where there is none)."""
+    idx = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            idx = -1
+    if idx < 0 or not first.is_cuda:
+        _require_cuda(first, *(t for t in others if t is not None))
+        raise RuntimeError("hackable_lm_b200: all tensors must be on the same device")
+    return idx
+
+
+def _call(idx: int, name: str, *args) -> None:
+    """Library call on the current stream of device ``idx``, with it current for the call's duration."""
+    fn = _FNS.get(name)
+    if fn is None:
+        fn = _FNS[name] = getattr(_lib.load(), name)
     if torch.cuda.current_device() == idx:
-        rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+        rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+            rc = fn(*args, _raw_stream(idx))
     if rc:
         check(rc, name)
+
+
+_FNS: dict = {}
 
 
 def _packed(t: torch.Tensor) -> torch.Tensor:
@@ -74,11 +93,11 @@ def _check_cols(what: str, x: torch.Tensor) -> None:
 # ---------------------------------------------------------------------------
 def _quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     _check_cols("quantize_rows", x)
-    dev = _require_cuda(x)
+    dev = _device_of(x)
     x = x.contiguous()
     cols = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _call(dev, "hlm_quantize_rows", x.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(), cols,
           _DTYPE_CODE[x.dtype])
     return q, scale
@@ -100,10 +119,10 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     _check_rows("dequantize_rows", q, scale)
-    dev = _require_cuda(q, scale)
+    dev = _device_of(q, scale)
     code = _code(dtype)
     q, scale = q.contiguous(), scale.contiguous()
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
+    out = q.new_empty(q.shape, dtype=dtype)
     if q.numel():
         _call(dev, "hlm_dequantize_rows", q.data_ptr(), scale.data_ptr(), out.data_ptr(), scale.numel(),
               q.shape[-1], code)
@@ -132,17 +151,17 @@ def _norm_weight(what: str, x: torch.Tensor, weight: Optional[torch.Tensor]) -> 
         return None
     if weight.shape != x.shape[-1:]:
         raise RuntimeError(f"{what}: weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
-    _require_cuda(x, weight)
+    _device_of(x, weight)
     return weight.to(x.dtype).contiguous()
 
 
 def _rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     _check_cols("rms_norm_q8", x)
-    dev = _require_cuda(x)
+    dev = _device_of(x)
     w = _norm_weight("rms_norm_q8", x, weight)
     x = x.contiguous()
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _call(dev, "hlm_residual_rms_norm_q8", None, x.data_ptr(), None if w is None else w.data_ptr(), None,
           q.data_ptr(), scale.data_ptr(), scale.numel(), x.shape[-1], float(eps), _DTYPE_CODE[x.dtype])
     return q, scale
@@ -164,14 +183,14 @@ def rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float) -> 
 def _residual_rms_norm_q8(residual: torch.Tensor, branch: torch.Tensor, weight: Optional[torch.Tensor],
                           eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     _check_cols("residual_rms_norm_q8", branch)
-    dev = _require_cuda(residual, branch)
+    dev = _device_of(residual, branch)
     if residual.shape != branch.shape or residual.dtype != branch.dtype:
         raise RuntimeError("residual_rms_norm_q8: residual and branch must match in shape and dtype")
     w = _norm_weight("residual_rms_norm_q8", branch, weight)
     residual, branch = residual.contiguous(), branch.contiguous()
-    out = torch.empty(branch.shape, dtype=branch.dtype, device=dev)
-    q = torch.empty(branch.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(branch.shape[:-1], dtype=torch.float32, device=dev)
+    out = branch.new_empty(branch.shape)
+    q = branch.new_empty(branch.shape, dtype=torch.int8)
+    scale = branch.new_empty(branch.shape[:-1], dtype=torch.float32)
     _call(dev, "hlm_residual_rms_norm_q8", residual.data_ptr(), branch.data_ptr(),
           None if w is None else w.data_ptr(), out.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(),
           branch.shape[-1], float(eps), _DTYPE_CODE[branch.dtype])
@@ -204,10 +223,10 @@ def _linear_q8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weigh
     code = _code(out_dtype)
     if weight.dim() != 2 or weight.shape[1] != q.shape[-1]:
         raise RuntimeError(f"linear_q8: weight must be [N, {q.shape[-1]}], got {tuple(weight.shape)}")
-    dev = _require_cuda(q, scale, weight, weight_scale)
+    dev = _device_of(q, scale, weight, weight_scale)
     N, K = weight.shape
     q, weight, scale, weight_scale = _packed(q), _packed(weight), scale.contiguous(), weight_scale.contiguous()
-    out = torch.empty((*q.shape[:-1], N), dtype=out_dtype, device=dev)
+    out = q.new_empty((*q.shape[:-1], N), dtype=out_dtype)
     _call(dev, "hlm_linear_q8", q.data_ptr(), scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
           out.data_ptr(), scale.numel(), N, K, code)
     return out
@@ -244,14 +263,14 @@ def _check_gate_up(what: str, width: int) -> int:
 
 
 def _swiglu_ckpt8(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    dev = _require_cuda(gate_up)
+    dev = _device_of(gate_up)
     code = _code(gate_up.dtype)
     hidden = _check_gate_up("swiglu_ckpt8", gate_up.shape[-1])
     gate_up = gate_up.contiguous()
     lead = gate_up.shape[:-1]
-    h = torch.empty((*lead, hidden), dtype=gate_up.dtype, device=dev)
-    q = torch.empty(gate_up.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty((*lead, _ckpt_scale_cols(hidden)), dtype=torch.float32, device=dev)
+    h = gate_up.new_empty((*lead, hidden))
+    q = gate_up.new_empty(gate_up.shape, dtype=torch.int8)
+    scale = gate_up.new_empty((*lead, _ckpt_scale_cols(hidden)), dtype=torch.float32)
     if hidden:
         _call(dev, "hlm_swiglu_ckpt8_fwd", gate_up.data_ptr(), h.data_ptr(), q.data_ptr(), scale.data_ptr(),
               h.numel() // hidden, hidden, code)
@@ -277,9 +296,9 @@ def _swiglu_ckpt8_backward(q: torch.Tensor, scale: torch.Tensor, grad_h: torch.T
             or scale.shape != (*lead, _ckpt_scale_cols(hidden))):
         raise RuntimeError("swiglu_ckpt8_backward: needs the codes and scales of swiglu_ckpt8 and a gradient "
                            f"[..., {hidden}], got {tuple(q.shape)}, {tuple(scale.shape)}, {tuple(grad_h.shape)}")
-    dev = _require_cuda(q, scale, grad_h)
+    dev = _device_of(q, scale, grad_h)
     q, scale, grad_h = q.contiguous(), scale.contiguous(), grad_h.contiguous()
-    grad = torch.empty(q.shape, dtype=grad_h.dtype, device=dev)
+    grad = grad_h.new_empty(q.shape)
     if hidden:
         _call(dev, "hlm_swiglu_ckpt8_bwd", q.data_ptr(), scale.data_ptr(), grad_h.data_ptr(), grad.data_ptr(),
               grad_h.numel() // hidden, hidden, code)
@@ -335,12 +354,12 @@ def _weight_grad_q8(grad: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) ->
     if grad.dim() < 1 or grad.shape[:-1] != q.shape[:-1]:
         raise RuntimeError("weight_grad_q8: grad [..., N] and the codes [..., K] must have the same rows, got "
                            f"{tuple(grad.shape)} and {tuple(q.shape)}")
-    dev = _require_cuda(grad, q, scale)
+    dev = _device_of(grad, q, scale)
     grad, q, scale = _packed(grad), _packed(q), scale.contiguous()
     tokens, N, K = scale.numel(), grad.shape[-1], q.shape[-1]
-    out = torch.empty((N, K), dtype=grad.dtype, device=dev)
+    out = grad.new_empty((N, K))
     nbytes = _lib.load().hlm_weight_grad_q8_workspace_bytes(tokens, N, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = grad.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(dev, "hlm_weight_grad_q8", grad.data_ptr(), q.data_ptr(), scale.data_ptr(), out.data_ptr(),
           None if ws is None else ws.data_ptr(), nbytes, tokens, N, K, _DTYPE_CODE[grad.dtype])
     return out
@@ -371,7 +390,7 @@ def linear_ckpt8_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
 def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, q, scale): y = x @ weight^T, and x in 8 bits by rows, kept for the weight gradient
     in place of x."""
-    _require_cuda(x, weight)
+    _device_of(x, weight)
     if not linear_ckpt8_supported(x, weight):
         raise RuntimeError("linear_ckpt8: needs bf16 or fp16 x [..., K] and weight [N, K] of one dtype with N a "
                            f"multiple of 8 and K of 16, got {x.dtype} {tuple(x.shape)}, {weight.dtype} "
