@@ -171,6 +171,437 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
   }
 }
 
+// ---------------------------------------------------------------------------
+// Rows, vectorised: TPR threads per row, up to NV 16-byte vectors per thread, the row
+// kept in registers between the maximum (and the sum of squares) and the codes.
+//
+// A row starts anywhere in its 16-byte vector when cols is not a multiple of the
+// vector (SHIFT): threads then load the aligned vectors that cover the row, elements
+// outside the row count as zeros, and the codes go through shared memory so that
+// they too leave in 16-byte stores.  Only the row's first and last vectors, whose
+// other elements belong to the neighbouring rows, are read and written by elements.
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+template <int TPR>
+HLM_DEVICE uint32_t row_max(uint32_t v, uint32_t* sh, int t) {
+  v = warp_max_u32(v);
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int w0 = (threadIdx.x / TPR) * W;
+    if ((t & 31) == 0) sh[w0 + (t >> 5)] = v;
+    __syncthreads();
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max(m, sh[w0 + i]);
+    v = m;
+  }
+  return v;
+}
+
+template <typename T, int TPR, int NV, bool NORM, bool SHIFT>
+__global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
+    const T* __restrict__ residual, const T* __restrict__ x, const T* __restrict__ weight,
+    T* __restrict__ out, int8_t* __restrict__ q, float* __restrict__ scale, int64_t rows, int cols,
+    float eps) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  constexpr int RPB = kRowThreads / TPR;
+  constexpr int kStage = SHIFT ? TPR * NV * VEC + 16 : 16;  // bytes of one row's codes
+  __shared__ uint32_t sh_max[kRowThreads / 32];
+  __shared__ float sh_sum[kRowThreads / 32];
+  __shared__ alignas(16) int8_t stage[SHIFT ? RPB * kStage : 16];
+  const int t = threadIdx.x % TPR;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool row_ok = row < rows;  // the same for the row's threads
+    const int64_t base = row * cols;
+    // elements of x that lie before the row in its first vector
+    const int head = SHIFT ? static_cast<int>((reinterpret_cast<uintptr_t>(x + base) & 15) / sizeof(T)) : 0;
+    uint4 v[NV], rr[NORM ? NV : 1];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      v[j] = make_uint4(0, 0, 0, 0);
+      if constexpr (NORM) rr[j] = make_uint4(0, 0, 0, 0);
+      const int c = (t + TPR * j) * VEC - head;  // column of the vector's first element
+      if (!row_ok || c >= cols) continue;
+      if (!SHIFT || (c >= 0 && c + VEC <= cols)) {
+        v[j] = ld_global_nc_v4(x + base + c);
+        if (NORM && residual != nullptr) rr[j] = ld_global_nc_v4(residual + base + c);
+      } else {
+        T* e = reinterpret_cast<T*>(&v[j]);
+        T* f = reinterpret_cast<T*>(&rr[NORM ? j : 0]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (c + i >= 0 && c + i < cols) {
+            e[i] = x[base + c + i];
+            if (NORM && residual != nullptr) f[i] = residual[base + c + i];
+          }
+      }
+    }
+    // the sum, rounded to T once, back in v; squares and magnitudes of it
+    float ss = 0.0f;
+    uint32_t mp = 0;
+    uint32_t mw = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (t + TPR * j) * VEC - head;
+      if constexpr (NORM) {
+        Vec16<T> a;
+        a.raw = v[j];
+        float f[VEC];
+        a.to_float(f);
+        if (residual != nullptr) {
+          Vec16<T> b;
+          b.raw = rr[j];
+          float g[VEC];
+          b.to_float(g);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] += g[i];
+          a.from_float(f);
+          v[j] = a.raw;
+          a.to_float(f);
+          if (row_ok && c < cols) {
+            if (!SHIFT || (c >= 0 && c + VEC <= cols)) {
+              st_global_v4(out + base + c, a.raw);
+            } else {
+              const T* e = reinterpret_cast<const T*>(&a.raw);
+#pragma unroll
+              for (int i = 0; i < VEC; ++i)
+                if (c + i >= 0 && c + i < cols) out[base + c + i] = e[i];
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) ss += f[i] * f[i];
+        if (weight != nullptr) {
+          if (!SHIFT) {
+            if (c < cols) {
+              Vec16<T> w;
+              w.raw = ld_global_v4(weight + c);
+              float g[VEC];
+              w.to_float(g);
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) mw = max(mw, mag_bits(__fmul_rn(f[i], g[i])));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              if (c + i >= 0 && c + i < cols) mw = max(mw, mag_bits(__fmul_rn(f[i], to_f32(weight[c + i]))));
+          }
+        }
+      }
+      mp = max_packed<T>(mp, max16_packed<T>(v[j]));
+    }
+    uint32_t m = unpack_max<T>(mp);
+    if (NORM && weight != nullptr) m = mw;
+    m = row_max<TPR>(m, sh_max, t);
+    const QuantStep st = quant_step(m);
+    if constexpr (NORM) {
+      ss = warp_sum(ss);
+      if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int w0 = (threadIdx.x / TPR) * W;
+        if ((t & 31) == 0) sh_sum[w0 + (t >> 5)] = ss;
+        __syncthreads();
+        ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) ss += sh_sum[w0 + i];
+      }
+    }
+    int8_t* row_stage = stage + (SHIFT ? (threadIdx.x / TPR) * kStage : 0);
+    // codes are bytes: the row's first code lies `qhead` bytes into its 16-byte vector
+    const int qhead = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(q + base) & 15) : 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (t + TPR * j) * VEC - head;
+      if (!row_ok || c >= cols) continue;
+      Vec16<T> a;
+      a.raw = v[j];
+      float f[VEC];
+      a.to_float(f);
+      if (NORM && weight != nullptr) {
+        if (!SHIFT) {
+          Vec16<T> w;
+          w.raw = ld_global_v4(weight + c);
+          float g[VEC];
+          w.to_float(g);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] = __fmul_rn(f[i], g[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (c + i >= 0 && c + i < cols) f[i] = __fmul_rn(f[i], to_f32(weight[c + i]));
+        }
+      }
+      if constexpr (!SHIFT) {
+        if constexpr (VEC == 8)
+          *reinterpret_cast<uint2*>(q + base + c) = make_uint2(quant_pack4(f[0], f[1], f[2], f[3], st.inv),
+                                                               quant_pack4(f[4], f[5], f[6], f[7], st.inv));
+        else
+          *reinterpret_cast<uint32_t*>(q + base + c) = quant_pack4(f[0], f[1], f[2], f[3], st.inv);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (c + i >= 0 && c + i < cols) row_stage[qhead + c + i] = quant_code(f[i], st);
+      }
+    }
+    if constexpr (SHIFT) {
+      if constexpr (TPR > 32)
+        __syncthreads();
+      else
+        __syncwarp();
+      if (row_ok) {
+        for (int b = t * 16; b < qhead + cols; b += TPR * 16) {
+          int8_t* dst = q + base - qhead + b;
+          if (b >= qhead && b + 16 <= qhead + cols) {
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(row_stage + b);
+          } else {
+            for (int i = 0; i < 16; ++i)
+              if (b + i >= qhead && b + i < qhead + cols) dst[i] = row_stage[b + i];
+          }
+        }
+      }
+    }
+    if (row_ok && t == 0) {
+      if constexpr (NORM)
+        scale[row] = st.scale * rsqrtf(ss / static_cast<float>(cols) + eps);
+      else
+        scale[row] = st.scale;
+    }
+    // shared memory is rewritten by the block's next rows
+    if constexpr (TPR > 32)
+      __syncthreads();
+    else if constexpr (SHIFT)
+      __syncwarp();
+  }
+}
+
+// Launch of the vector kernel that holds a row of `cols`, or false when the row is too
+// wide (or its tensors are aligned differently): the scalar kernel takes those.
+template <typename T, bool NORM>
+static bool launch_quant_rows_vec(const T* residual, const T* x, const T* weight, T* out, int8_t* q,
+                                  float* scale, int64_t rows, int cols, float eps, cudaStream_t s) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  auto mod16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & 15u; };
+  const bool same = residual == nullptr || (mod16(residual) == mod16(x) && mod16(out) == mod16(x));
+  if (!same || mod16(x) % sizeof(T) != 0) return false;
+  const bool aligned = cols % VEC == 0 && mod16(x) == 0 && reinterpret_cast<uintptr_t>(q) % VEC == 0 &&
+                       (weight == nullptr || mod16(weight) == 0);
+  // vectors that cover a row, at most
+  const int64_t nv = aligned ? cols / VEC : (cols + VEC - 1) / VEC + 1;
+#define HLM_ROWS_LAUNCH(TPR, NV, SHIFT)                                                                     \
+  do {                                                                                                      \
+    quant_rows_vec_kernel<T, TPR, NV, NORM, SHIFT><<<quant_grid(rows, kRowThreads / TPR), kRowThreads, 0, s>>>( \
+        residual, x, weight, out, q, scale, rows, cols, eps);                                               \
+    return true;                                                                                            \
+  } while (0)
+  if (aligned) {
+    if (nv <= 32) HLM_ROWS_LAUNCH(32, 1, false);
+    if (nv <= 64) HLM_ROWS_LAUNCH(32, 2, false);
+    if (nv <= 96) HLM_ROWS_LAUNCH(32, 3, false);
+    if (nv <= 128) HLM_ROWS_LAUNCH(32, 4, false);
+    if (nv <= 256) HLM_ROWS_LAUNCH(64, 4, false);
+    if (nv <= 512) HLM_ROWS_LAUNCH(128, 4, false);
+    if (nv <= 1024) HLM_ROWS_LAUNCH(256, 4, false);
+    if (nv <= 2048) HLM_ROWS_LAUNCH(256, 8, false);
+    return false;
+  }
+  if (nv <= 128) HLM_ROWS_LAUNCH(32, 4, true);
+  if (nv <= 256) HLM_ROWS_LAUNCH(64, 4, true);
+  if (nv <= 512) HLM_ROWS_LAUNCH(128, 4, true);
+  if (nv <= 1024) HLM_ROWS_LAUNCH(256, 4, true);
+  if (nv <= 2048) HLM_ROWS_LAUNCH(256, 8, true);
+#undef HLM_ROWS_LAUNCH
+  return false;
+}
+
+// Read back, over the flat tensor: a thread takes 16 codes at a time whatever the row
+// length, since 16 consecutive codes lie in at most two rows of 16 or more columns.
+// One division finds the row.
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* __restrict__ q,
+                                                          const float* __restrict__ scale,
+                                                          T* __restrict__ out, I total, I cols) {
+  const I step = static_cast<I>(gridDim.x) * blockDim.x * 16;
+  for (I e = (static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x) * 16; e < total; e += step) {
+    const I row = e / cols;
+    const I next = (row + 1) * cols - e;  // codes from here on belong to the next row
+    const float s0 = scale[row];
+    if (e + 16 <= total) {
+      const uint4 raw = ld_global_nc_v4(q + e);
+      const float s1 = next < 16 ? scale[row + 1] : s0;
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      float f[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float c[4];
+        codes_to_float(w[k], c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * k + i] = c[i] * (static_cast<I>(4 * k + i) < next ? s0 : s1);
+      }
+      constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+      for (int k = 0; k < 16 / VEC; ++k) {
+        Vec16<T> o;
+        float g[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[i] = f[k * VEC + i];
+        o.from_float(g);
+        st_global_v4(out + e + k * VEC, o.raw);
+      }
+    } else {
+      for (I i = 0; e + i < total; ++i) {
+        const I r = (e + i) / cols;
+        out[e + i] = from_f32<T>(static_cast<float>(q[e + i]) * scale[r]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// SwiGLU checkpoint, vectorised: a thread owns one 16-byte vector of gate and the
+// matching one of up in R consecutive rows; the 128 / VEC threads of a group (half a
+// warp for 16-bit types, a warp for fp32) find its two maxima by shuffles, both in
+// one packed word for the 16-bit types.
+// ---------------------------------------------------------------------------
+template <typename T>
+HLM_DEVICE void group_maxima(uint4 g, uint4 u, uint32_t& mg, uint32_t& mu) {
+  if constexpr (sizeof(T) == 4) {
+    mg = warp_max_u32(max16_packed<T>(g));
+    mu = warp_max_u32(max16_packed<T>(u));
+  } else {
+    const uint32_t a = max16_packed<T>(g), b = max16_packed<T>(u);
+    // one 16-bit maximum of each, gate low and up high
+    uint32_t m = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    mg = unpack_max<T>(m & 0xffffu);
+    mu = unpack_max<T>(m >> 16);
+  }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_vec_kernel(
+    const T* __restrict__ gate_up, T* __restrict__ h, int8_t* __restrict__ q,
+    float* __restrict__ scale, int64_t rows, int hv, int groups) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  constexpr int GT = kCkptGroup / VEC;  // threads of a group
+  const int64_t hidden = static_cast<int64_t>(hv) * VEC;
+  const int hv_pad = groups * GT;  // a group's threads stay together past the last vector
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < rows;
+       r0 += static_cast<int64_t>(gridDim.x) * R) {
+    for (int c0 = 0; c0 < hv_pad; c0 += blockDim.x) {
+      const int cv = c0 + threadIdx.x;
+      uint4 gr[R], ur[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        gr[r] = ur[r] = make_uint4(0, 0, 0, 0);
+        if (r0 + r < rows && cv < hv) {
+          const T* src = gate_up + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
+          gr[r] = ld_global_nc_v4(src);
+          ur[r] = ld_global_nc_v4(src + hidden);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        uint32_t mg, mu;
+        group_maxima<T>(gr[r], ur[r], mg, mu);  // all threads: shuffles
+        if (r0 + r >= rows || cv >= hv) continue;
+        const QuantStep sg = quant_step(mg), su = quant_step(mu);
+        Vec16<T> gv, uv, ov;
+        gv.raw = gr[r];
+        uv.raw = ur[r];
+        float g[VEC], u[VEC], o[VEC];
+        gv.to_float(g);
+        uv.to_float(u);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = g[i] * sigmoid_fast(g[i]) * u[i];
+        ov.from_float(o);
+        st_global_v4(h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC, ov.raw);
+        int8_t* qg = q + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
+        if constexpr (VEC == 8) {
+          *reinterpret_cast<uint2*>(qg) =
+              make_uint2(quant_pack4(g[0], g[1], g[2], g[3], sg.inv), quant_pack4(g[4], g[5], g[6], g[7], sg.inv));
+          *reinterpret_cast<uint2*>(qg + hidden) =
+              make_uint2(quant_pack4(u[0], u[1], u[2], u[3], su.inv), quant_pack4(u[4], u[5], u[6], u[7], su.inv));
+        } else {
+          *reinterpret_cast<uint32_t*>(qg) = quant_pack4(g[0], g[1], g[2], g[3], sg.inv);
+          *reinterpret_cast<uint32_t*>(qg + hidden) = quant_pack4(u[0], u[1], u[2], u[3], su.inv);
+        }
+        if (cv % GT == 0) {
+          float* sp = scale + (r0 + r) * 2 * groups + cv / GT;
+          sp[0] = sg.scale;
+          sp[groups] = su.scale;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_vec_kernel(
+    const int8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ grad_h,
+    T* __restrict__ grad_gate_up, int64_t rows, int hv, int groups) {
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  constexpr int GT = kCkptGroup / VEC;
+  const int64_t hidden = static_cast<int64_t>(hv) * VEC;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * R; r0 < rows;
+       r0 += static_cast<int64_t>(gridDim.x) * R) {
+    for (int cv = threadIdx.x; cv < hv; cv += blockDim.x) {
+      uint32_t qg[R][VEC / 4], qu[R][VEC / 4];
+      uint4 dr[R];
+      float sg[R], su[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r0 + r < rows) {
+          const int8_t* src = q + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
+          if constexpr (VEC == 8) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(src));
+            const uint2 b = __ldg(reinterpret_cast<const uint2*>(src + hidden));
+            qg[r][0] = a.x;
+            qg[r][1] = a.y;
+            qu[r][0] = b.x;
+            qu[r][1] = b.y;
+          } else {
+            qg[r][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+            qu[r][0] = __ldg(reinterpret_cast<const uint32_t*>(src + hidden));
+          }
+          dr[r] = ld_global_nc_v4(grad_h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC);
+          const float* sp = scale + (r0 + r) * 2 * groups + cv / GT;
+          sg[r] = __ldg(sp);
+          su[r] = __ldg(sp + groups);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r0 + r >= rows) continue;
+        Vec16<T> dv, og, ou;
+        dv.raw = dr[r];
+        float d[VEC], rg[VEC], ru[VEC];
+        dv.to_float(d);
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) {
+          float g[4], u[4];
+          codes_to_float(qg[r][k], g);
+          codes_to_float(qu[r][k], u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float gv = g[i] * sg[r], uv = u[i] * su[r], dd = d[4 * k + i];
+            const float s = sigmoid_fast(gv);
+            rg[4 * k + i] = dd * uv * (s * (1.0f + gv * (1.0f - s)));
+            ru[4 * k + i] = dd * (gv * s);
+          }
+        }
+        og.from_float(rg);
+        ou.from_float(ru);
+        T* dst = grad_gate_up + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
+        st_global_v4(dst, og.raw);
+        st_global_v4(dst + hidden, ou.raw);
+      }
+    }
+  }
+}
+
 }  // namespace hlm
 
 using namespace hlm;
@@ -183,7 +614,9 @@ extern "C" int hlm_quantize_rows(const void* x, void* q, float* scale, int64_t r
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_QUANT_ROWS, s);
-    quant_rows_scalar_kernel<T, false><<<quant_grid(rows, 8), 256, 0, s>>>(
+    if (!launch_quant_rows_vec<T, false>(nullptr, static_cast<const T*>(x), nullptr, nullptr,
+                                         static_cast<int8_t*>(q), scale, rows, static_cast<int>(cols), 0.0f, s))
+      quant_rows_scalar_kernel<T, false><<<quant_grid(rows, 8), 256, 0, s>>>(
         nullptr, static_cast<const T*>(x), nullptr, nullptr, static_cast<int8_t*>(q), scale, rows,
         static_cast<int>(cols), 0.0f);
   });
@@ -198,7 +631,19 @@ extern "C" int hlm_dequantize_rows(const void* q, const float* scale, void* out,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_DEQUANT_ROWS, s);
-    dequant_rows_scalar_kernel<T><<<quant_grid(rows, 8), 256, 0, s>>>(
+    const int64_t total = rows * cols;
+    const int grid = quant_grid((total + 15) / 16, 256);
+    if (cols >= 16 && host_aligned16(q) && host_aligned16(out)) {
+      if (total < (1ll << 31))  // 32-bit division; the stride past the end stays below 2^32
+        dequant_flat_kernel<T, uint32_t><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(q), scale,
+                                                              static_cast<T*>(out), static_cast<uint32_t>(total),
+                                                              static_cast<uint32_t>(cols));
+      else
+        dequant_flat_kernel<T, uint64_t><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(q), scale,
+                                                              static_cast<T*>(out), static_cast<uint64_t>(total),
+                                                              static_cast<uint64_t>(cols));
+    } else
+      dequant_rows_scalar_kernel<T><<<quant_grid(rows, 8), 256, 0, s>>>(
         static_cast<const int8_t*>(q), scale, static_cast<T*>(out), rows, static_cast<int>(cols));
   });
   return launch_status();
@@ -214,7 +659,10 @@ extern "C" int hlm_residual_rms_norm_q8(const void* residual, const void* branch
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_NORM_Q8, s);
-    quant_rows_scalar_kernel<T, true><<<quant_grid(rows, 8), 256, 0, s>>>(
+    if (!launch_quant_rows_vec<T, true>(static_cast<const T*>(residual), static_cast<const T*>(branch),
+                                        static_cast<const T*>(weight), static_cast<T*>(out),
+                                        static_cast<int8_t*>(q), scale, rows, static_cast<int>(cols), eps, s))
+      quant_rows_scalar_kernel<T, true><<<quant_grid(rows, 8), 256, 0, s>>>(
         static_cast<const T*>(residual), static_cast<const T*>(branch),
         static_cast<const T*>(weight), static_cast<T*>(out), static_cast<int8_t*>(q), scale, rows,
         static_cast<int>(cols), eps);
@@ -232,7 +680,14 @@ extern "C" int hlm_swiglu_ckpt8_fwd(const void* gate_up, void* h, void* q, float
   const int groups = static_cast<int>((hidden + kCkptGroup - 1) / kCkptGroup);
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_SWIGLU_CKPT8_FWD, s);
-    swiglu_ckpt8_fwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
+    constexpr int VEC = 16 / sizeof(T);
+    if (hidden % VEC == 0 && host_aligned16(gate_up) && host_aligned16(h) && host_aligned16(q)) {
+      constexpr int R = 2;
+      swiglu_ckpt8_fwd_vec_kernel<T, R><<<quant_grid(rows, R), 256, 0, s>>>(
+          static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
+          static_cast<int>(hidden / VEC), groups);
+    } else
+      swiglu_ckpt8_fwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
         static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
         hidden, groups);
   });
@@ -250,7 +705,14 @@ extern "C" int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const voi
   const int groups = static_cast<int>((hidden + kCkptGroup - 1) / kCkptGroup);
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_SWIGLU_CKPT8_BWD, s);
-    swiglu_ckpt8_bwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
+    constexpr int VEC = 16 / sizeof(T);
+    if (hidden % VEC == 0 && host_aligned16(grad_h) && host_aligned16(grad_gate_up) && host_aligned16(q)) {
+      constexpr int R = 2;
+      swiglu_ckpt8_bwd_vec_kernel<T, R><<<quant_grid(rows, R), 256, 0, s>>>(
+          static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
+          static_cast<T*>(grad_gate_up), rows, static_cast<int>(hidden / VEC), groups);
+    } else
+      swiglu_ckpt8_bwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
         static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
         static_cast<T*>(grad_gate_up), rows, hidden, groups);
   });

@@ -60,6 +60,56 @@ HLM_DEVICE uint32_t quant_pack4(float v0, float v1, float v2, float v3, float in
   return inv == 0.0f ? 0u : __byte_perm(lo, hi, 0x5410);
 }
 
+// Four codes back as floats: each byte, offset by 128, becomes the low mantissa
+// byte of 2^23, from which 2^23 + 128 is subtracted: exact.
+HLM_DEVICE void codes_to_float(uint32_t packed, float (&f)[4]) {
+  const uint32_t b = packed ^ 0x80808080u;
+  f[0] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440)) - 8388736.0f;
+  f[1] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7441)) - 8388736.0f;
+  f[2] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7442)) - 8388736.0f;
+  f[3] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7443)) - 8388736.0f;
+}
+
+// Largest magnitude among the elements of a 16-byte vector, as fp32 bits.  The
+// 16-bit types compare as packed pairs of 15-bit integers: ordered like the
+// magnitudes, infinities above finite values, NaNs above infinities.
+template <typename T>
+HLM_DEVICE uint32_t max16_packed(uint4 v);  // packed pair (16-bit types) or fp32 bits
+template <>
+HLM_DEVICE uint32_t max16_packed<float>(uint4 v) {
+  constexpr uint32_t k = 0x7fffffffu;
+  return max(max(v.x & k, v.y & k), max(v.z & k, v.w & k));
+}
+template <>
+HLM_DEVICE uint32_t max16_packed<__nv_bfloat16>(uint4 v) {
+  constexpr uint32_t k = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(v.x & k, v.y & k), __vmaxu2(v.z & k, v.w & k));
+}
+template <>
+HLM_DEVICE uint32_t max16_packed<__half>(uint4 v) {
+  return max16_packed<__nv_bfloat16>(v);
+}
+template <typename T>
+HLM_DEVICE uint32_t max_packed(uint32_t a, uint32_t b) {
+  return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
+}
+// fp32 magnitude bits of a packed maximum.
+template <typename T>
+HLM_DEVICE uint32_t unpack_max(uint32_t m);
+template <>
+HLM_DEVICE uint32_t unpack_max<float>(uint32_t m) {
+  return m;
+}
+template <>
+HLM_DEVICE uint32_t unpack_max<__nv_bfloat16>(uint32_t m) {
+  return max(m & 0xffffu, m >> 16) << 16;
+}
+template <>
+HLM_DEVICE uint32_t unpack_max<__half>(uint32_t m) {
+  const uint16_t h = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+  return mag_bits(__half2float(__ushort_as_half(h)));
+}
+
 HLM_DEVICE uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 }  // namespace hlm
