@@ -98,19 +98,17 @@ __global__ void __launch_bounds__(256) dequant_rows_scalar_kernel(const int8_t* 
   }
 }
 
-// SwiGLU checkpoint, one warp per row and group of 128 hidden units: the gate
-// group and the up group each get their own scale.
+// SwiGLU checkpoint for halves that are not 16-byte multiples: a block per row, a warp
+// per group of 128 hidden units, of which the gate part and the up part each get their
+// own scale.
 template <typename T>
 __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_scalar_kernel(
     const T* __restrict__ gate_up, T* __restrict__ h, int8_t* __restrict__ q,
     float* __restrict__ scale, int64_t rows, int64_t hidden, int groups) {
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
-  const int64_t items = rows * groups;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * wpb + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * wpb) {
-    const int64_t row = it / groups;
-    const int grp = static_cast<int>(it - row * groups);
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+  for (int grp = threadIdx.x >> 5; grp < groups; grp += wpb) {
     const int64_t gbase = row * 2 * hidden;
     float g[4], u[4];
     uint32_t mg = 0, mu = 0;
@@ -149,11 +147,8 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
     T* __restrict__ grad_gate_up, int64_t rows, int64_t hidden, int groups) {
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
-  const int64_t items = rows * groups;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * wpb + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * wpb) {
-    const int64_t row = it / groups;
-    const int grp = static_cast<int>(it - row * groups);
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+  for (int grp = threadIdx.x >> 5; grp < groups; grp += wpb) {
     const int64_t gbase = row * 2 * hidden;
     const float sg = scale[row * 2 * groups + grp];
     const float su = scale[row * 2 * groups + groups + grp];
@@ -183,6 +178,17 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
+// Barrier of one row's threads (a block holds several rows; they do not wait for each other).
+template <int TPR>
+HLM_DEVICE void row_sync() {
+  if constexpr (TPR == 32)
+    __syncwarp();
+  else if constexpr (TPR == kRowThreads)
+    __syncthreads();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / TPR), "n"(TPR) : "memory");
+}
+
 template <int TPR>
 HLM_DEVICE uint32_t row_max(uint32_t v, uint32_t* sh, int t) {
   v = warp_max_u32(v);
@@ -190,7 +196,7 @@ HLM_DEVICE uint32_t row_max(uint32_t v, uint32_t* sh, int t) {
     constexpr int W = TPR / 32;
     const int w0 = (threadIdx.x / TPR) * W;
     if ((t & 31) == 0) sh[w0 + (t >> 5)] = v;
-    __syncthreads();
+    row_sync<TPR>();
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) m = max(m, sh[w0 + i]);
@@ -211,6 +217,7 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
   __shared__ float sh_sum[kRowThreads / 32];
   __shared__ alignas(16) int8_t stage[SHIFT ? RPB * kStage : 16];
   const int t = threadIdx.x % TPR;
+  const int64_t total = rows * cols;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
     const int64_t row = r0 + threadIdx.x / TPR;
     const bool row_ok = row < rows;  // the same for the row's threads
@@ -224,10 +231,10 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
       if constexpr (NORM) rr[j] = make_uint4(0, 0, 0, 0);
       const int c = (t + TPR * j) * VEC - head;  // column of the vector's first element
       if (!row_ok || c >= cols) continue;
-      if (!SHIFT || (c >= 0 && c + VEC <= cols)) {
+      if (!SHIFT || (base + c >= 0 && base + c + VEC <= total)) {
         v[j] = ld_global_nc_v4(x + base + c);
         if (NORM && residual != nullptr) rr[j] = ld_global_nc_v4(residual + base + c);
-      } else {
+      } else {  // the tensor's own first or last vector
         T* e = reinterpret_cast<T*>(&v[j]);
         T* f = reinterpret_cast<T*>(&rr[NORM ? j : 0]);
 #pragma unroll
@@ -235,6 +242,21 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
           if (c + i >= 0 && c + i < cols) {
             e[i] = x[base + c + i];
             if (NORM && residual != nullptr) f[i] = residual[base + c + i];
+          }
+      }
+    }
+    // elements of the neighbouring rows (after every load has been issued)
+#pragma unroll
+    for (int j = 0; j < (SHIFT ? NV : 0); ++j) {
+      const int c = (t + TPR * j) * VEC - head;
+      if (row_ok && c < cols && (c < 0 || c + VEC > cols)) {
+        T* e = reinterpret_cast<T*>(&v[j]);
+        T* f = reinterpret_cast<T*>(&rr[NORM ? j : 0]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (c + i < 0 || c + i >= cols) {
+            e[i] = from_f32<T>(0.0f);
+            if (NORM) f[i] = from_f32<T>(0.0f);
           }
       }
     }
@@ -302,15 +324,16 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
         constexpr int W = TPR / 32;
         const int w0 = (threadIdx.x / TPR) * W;
         if ((t & 31) == 0) sh_sum[w0 + (t >> 5)] = ss;
-        __syncthreads();
+        row_sync<TPR>();
         ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; ++i) ss += sh_sum[w0 + i];
       }
     }
     int8_t* row_stage = stage + (SHIFT ? (threadIdx.x / TPR) * kStage : 0);
-    // codes are bytes: the row's first code lies `qhead` bytes into its 16-byte vector
-    const int qhead = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(q + base) & 15) : 0;
+    // the row's first code lies `qhead` bytes into its word of q; the stage holds the codes of
+    // the row's vectors one after the other, so its first code is at byte `head`
+    const int qhead = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(q + base) & 3) : 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (t + TPR * j) * VEC - head;
@@ -333,31 +356,27 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
             if (c + i >= 0 && c + i < cols) f[i] = __fmul_rn(f[i], to_f32(weight[c + i]));
         }
       }
-      if constexpr (!SHIFT) {
-        if constexpr (VEC == 8)
-          *reinterpret_cast<uint2*>(q + base + c) = make_uint2(quant_pack4(f[0], f[1], f[2], f[3], st.inv),
-                                                               quant_pack4(f[4], f[5], f[6], f[7], st.inv));
-        else
-          *reinterpret_cast<uint32_t*>(q + base + c) = quant_pack4(f[0], f[1], f[2], f[3], st.inv);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (c + i >= 0 && c + i < cols) row_stage[qhead + c + i] = quant_code(f[i], st);
-      }
+      int8_t* dst = SHIFT ? row_stage + c + head : q + base + c;
+      if constexpr (VEC == 8)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(quant_pack4(f[0], f[1], f[2], f[3], st.inv),
+                                                    quant_pack4(f[4], f[5], f[6], f[7], st.inv));
+      else
+        *reinterpret_cast<uint32_t*>(dst) = quant_pack4(f[0], f[1], f[2], f[3], st.inv);
     }
     if constexpr (SHIFT) {
-      if constexpr (TPR > 32)
-        __syncthreads();
-      else
-        __syncwarp();
+      row_sync<TPR>();
       if (row_ok) {
-        for (int b = t * 16; b < qhead + cols; b += TPR * 16) {
+        // aligned words of q: word b holds columns b - qhead ..., staged from byte head + b - qhead on
+        const int delta = head - qhead;
+        for (int b = t * 4; b < qhead + cols; b += TPR * 4) {
           int8_t* dst = q + base - qhead + b;
-          if (b >= qhead && b + 16 <= qhead + cols) {
-            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(row_stage + b);
+          if (b >= qhead && b + 4 <= qhead + cols) {
+            const int o = b + delta;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(row_stage) + (o >> 2);
+            *reinterpret_cast<uint32_t*>(dst) = __funnelshift_r(w[0], w[1], (o & 3) * 8);
           } else {
-            for (int i = 0; i < 16; ++i)
-              if (b + i >= qhead && b + i < qhead + cols) dst[i] = row_stage[b + i];
+            for (int i = 0; i < 4; ++i)
+              if (b + i >= qhead && b + i < qhead + cols) dst[i] = row_stage[b + delta + i];
           }
         }
       }
@@ -369,10 +388,7 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
         scale[row] = st.scale;
     }
     // shared memory is rewritten by the block's next rows
-    if constexpr (TPR > 32)
-      __syncthreads();
-    else if constexpr (SHIFT)
-      __syncwarp();
+    if constexpr (TPR > 32 || SHIFT) row_sync<TPR>();
   }
 }
 
@@ -406,53 +422,66 @@ static bool launch_quant_rows_vec(const T* residual, const T* x, const T* weight
     if (nv <= 2048) HLM_ROWS_LAUNCH(256, 8, false);
     return false;
   }
-  if (nv <= 128) HLM_ROWS_LAUNCH(32, 4, true);
-  if (nv <= 256) HLM_ROWS_LAUNCH(64, 4, true);
-  if (nv <= 512) HLM_ROWS_LAUNCH(128, 4, true);
-  if (nv <= 1024) HLM_ROWS_LAUNCH(256, 4, true);
-  if (nv <= 2048) HLM_ROWS_LAUNCH(256, 8, true);
+  // five vectors, since a row of a power of two plus or minus a few columns spans one more
+  if (nv <= 64) HLM_ROWS_LAUNCH(32, 2, true);
+  if (nv <= 160) HLM_ROWS_LAUNCH(32, 5, true);
+  if (nv <= 320) HLM_ROWS_LAUNCH(64, 5, true);
+  if (nv <= 640) HLM_ROWS_LAUNCH(128, 5, true);
+  if (nv <= 1280) HLM_ROWS_LAUNCH(256, 5, true);
+  if (nv <= 2304) HLM_ROWS_LAUNCH(256, 9, true);
 #undef HLM_ROWS_LAUNCH
   return false;
 }
 
-// Read back, over the flat tensor: a thread takes 16 codes at a time whatever the row
-// length, since 16 consecutive codes lie in at most two rows of 16 or more columns.
-// One division finds the row.
+// Read back, over the flat tensor: a thread takes VEC consecutive codes (one 16-byte
+// store) whatever the row length, since so few lie in at most two rows of 16 or more
+// columns; one division finds the row.  Four such steps of a block in flight.
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* __restrict__ q,
                                                           const float* __restrict__ scale,
                                                           T* __restrict__ out, I total, I cols) {
-  const I step = static_cast<I>(gridDim.x) * blockDim.x * 16;
-  for (I e = (static_cast<I>(blockIdx.x) * blockDim.x + threadIdx.x) * 16; e < total; e += step) {
-    const I row = e / cols;
-    const I next = (row + 1) * cols - e;  // codes from here on belong to the next row
-    const float s0 = scale[row];
-    if (e + 16 <= total) {
-      const uint4 raw = ld_global_nc_v4(q + e);
-      const float s1 = next < 16 ? scale[row + 1] : s0;
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      float f[16];
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+  constexpr int U = 4;
+  constexpr I kSpan = 256 * VEC;  // codes of one step of the block
+  for (I e0 = static_cast<I>(blockIdx.x) * (U * kSpan) + threadIdx.x * VEC; e0 < total;
+       e0 += static_cast<I>(gridDim.x) * (U * kSpan)) {
+    uint32_t w[U][VEC / 4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float c[4];
-        codes_to_float(w[k], c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[4 * k + i] = c[i] * (static_cast<I>(4 * k + i) < next ? s0 : s1);
+    for (int u = 0; u < U; ++u) {
+      const I e = e0 + u * kSpan;
+      if (e + VEC <= total) {
+        if constexpr (VEC == 8) {
+          const uint2 a = __ldg(reinterpret_cast<const uint2*>(q + e));
+          w[u][0] = a.x;
+          w[u][1] = a.y;
+        } else {
+          w[u][0] = __ldg(reinterpret_cast<const uint32_t*>(q + e));
+        }
       }
-      constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+    }
 #pragma unroll
-      for (int k = 0; k < 16 / VEC; ++k) {
+    for (int u = 0; u < U; ++u) {
+      const I e = e0 + u * kSpan;
+      if (e >= total) break;
+      const I row = e / cols;
+      const I next = (row + 1) * cols - e;  // codes from here on belong to the next row
+      const float s0 = scale[row];
+      if (e + VEC <= total) {
+        const float s1 = next < VEC ? scale[row + 1] : s0;
+        float f[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) {
+          float c[4];
+          codes_to_float(w[u][k], c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[4 * k + i] = c[i] * (static_cast<I>(4 * k + i) < next ? s0 : s1);
+        }
         Vec16<T> o;
-        float g[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) g[i] = f[k * VEC + i];
-        o.from_float(g);
-        st_global_v4(out + e + k * VEC, o.raw);
-      }
-    } else {
-      for (I i = 0; e + i < total; ++i) {
-        const I r = (e + i) / cols;
-        out[e + i] = from_f32<T>(static_cast<float>(q[e + i]) * scale[r]);
+        o.from_float(f);
+        st_global_v4(out + e, o.raw);
+      } else {
+        for (I i = 0; e + i < total; ++i)
+          out[e + i] = from_f32<T>(static_cast<float>(q[e + i]) * (i < next ? s0 : scale[row + 1]));
       }
     }
   }
@@ -478,6 +507,12 @@ HLM_DEVICE void group_maxima(uint4 g, uint4 u, uint32_t& mg, uint32_t& mu) {
     mg = unpack_max<T>(m & 0xffffu);
     mu = unpack_max<T>(m >> 16);
   }
+}
+
+// Threads of a block that walks rows of `n` vectors: the fewest steps of at most 256, evenly filled.
+static inline int row_block(int64_t n) {
+  const int64_t steps = (n + 255) / 256;
+  return static_cast<int>(((n + steps - 1) / steps + 31) / 32 * 32);
 }
 
 template <typename T, int R>
@@ -632,9 +667,9 @@ extern "C" int hlm_dequantize_rows(const void* q, const float* scale, void* out,
   HLM_QUANT_DISPATCH(dtype, T, {
     LaunchScope scope(HLM_KERNEL_DEQUANT_ROWS, s);
     const int64_t total = rows * cols;
-    const int grid = quant_grid((total + 15) / 16, 256);
+    const int grid = quant_grid((total + 16 / sizeof(T) - 1) / (16 / sizeof(T)), 4 * 256);
     if (cols >= 16 && host_aligned16(q) && host_aligned16(out)) {
-      if (total < (1ll << 31))  // 32-bit division; the stride past the end stays below 2^32
+      if (total < (1ll << 31))  // 32-bit division; a step past the end stays below 2^32
         dequant_flat_kernel<T, uint32_t><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(q), scale,
                                                               static_cast<T*>(out), static_cast<uint32_t>(total),
                                                               static_cast<uint32_t>(cols));
@@ -683,11 +718,11 @@ extern "C" int hlm_swiglu_ckpt8_fwd(const void* gate_up, void* h, void* q, float
     constexpr int VEC = 16 / sizeof(T);
     if (hidden % VEC == 0 && host_aligned16(gate_up) && host_aligned16(h) && host_aligned16(q)) {
       constexpr int R = 2;
-      swiglu_ckpt8_fwd_vec_kernel<T, R><<<quant_grid(rows, R), 256, 0, s>>>(
+      swiglu_ckpt8_fwd_vec_kernel<T, R><<<quant_grid(rows, R), row_block(hidden / VEC), 0, s>>>(
           static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
           static_cast<int>(hidden / VEC), groups);
     } else
-      swiglu_ckpt8_fwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
+      swiglu_ckpt8_fwd_scalar_kernel<T><<<quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), 0, s>>>(
         static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
         hidden, groups);
   });
@@ -708,11 +743,11 @@ extern "C" int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const voi
     constexpr int VEC = 16 / sizeof(T);
     if (hidden % VEC == 0 && host_aligned16(grad_h) && host_aligned16(grad_gate_up) && host_aligned16(q)) {
       constexpr int R = 2;
-      swiglu_ckpt8_bwd_vec_kernel<T, R><<<quant_grid(rows, R), 256, 0, s>>>(
+      swiglu_ckpt8_bwd_vec_kernel<T, R><<<quant_grid(rows, R), row_block(hidden / VEC), 0, s>>>(
           static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
           static_cast<T*>(grad_gate_up), rows, static_cast<int>(hidden / VEC), groups);
     } else
-      swiglu_ckpt8_bwd_scalar_kernel<T><<<quant_grid(rows * groups, 8), 256, 0, s>>>(
+      swiglu_ckpt8_bwd_scalar_kernel<T><<<quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), 0, s>>>(
         static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
         static_cast<T*>(grad_gate_up), rows, hidden, groups);
   });
