@@ -1,29 +1,474 @@
 // Weight gradient of a projection whose input was kept in 8 bits:
+//
 //   grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m])
+//
+// One CTA-pair tcgen05 GEMM (256 x 256 tiles of grad_w, tokens as the reduction),
+// whose B operand is made in the kernel: TMA brings the int8 codes of 64 tokens x
+// 128 input features per CTA, eight converter warps read them back to the gradient's
+// type (q * scale in fp32, rounded once: the MMA takes one 16-bit type for both
+// operands) and write the swizzled MN-major tile that the MMA reads.  The codes are
+// half the bytes of the activations, and no read-back tensor goes to memory.
+//
+// Per 64 tokens the pair's MMA takes about 370 ns at the measured bf16 rate; the
+// converters need about 280 issue slots of each SM quarter for the 8192 codes of a
+// CTA, so the tensor cores stay the bound.
+//
+// Few tiles: the tokens are split and each split writes an fp32 partial to the
+// workspace; a second kernel adds the partials in the order of the splits (the same
+// bits every time) and rounds.
+#include "gemm_sm100.cuh"
 #include "quant_common.cuh"
 
 namespace hlm {
 
+constexpr int kWgStages = 6;
+constexpr int kWgBStages = 3;
+constexpr int kWgConvWarps = 8;
+constexpr int kWgEpiWarps = 4;
+constexpr int kWgConvWarp0 = kEpiWarp0 + kWgEpiWarps;
+constexpr int kWgThreads = 32 * (kWgConvWarp0 + kWgConvWarps);
+
+struct WgSmem {
+  static constexpr int kABytes = kBM * kBK * 2;  // 128 output features x 64 tokens, 16-bit
+  static constexpr int kRawBytes = 128 * kBK;    // 128 input features x 64 tokens, codes
+  static constexpr int kStageBytes = kABytes + kRawBytes;
+  static constexpr int kBBytes = 128 * kBK * 2;  // the same, read back
+  static constexpr int kBOffset = kWgStages * kStageBytes;
+  static constexpr int kBoxOffset = kBOffset + kWgBStages * kBBytes;  // epilogue boxes, 4 KB per warp
+  static constexpr int kBarOffset = kBoxOffset + kWgEpiWarps * 4096;
+  static constexpr int kNumBars = 4 * kWgStages + 2 * kWgBStages + 4;
+  static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
+  static constexpr int kBytes = kTmemSlotOffset + 16 + 1024;
+  static_assert(kBytes <= 232448, "shared memory budget exceeded");
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) weight_grad_q8_simple_kernel(
-    const T* __restrict__ grad, const int8_t* __restrict__ q, const float* __restrict__ scale,
-    T* __restrict__ grad_w, int64_t tokens, int64_t N, int64_t K) {
-  const int64_t total = N * K;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t n = i / K, k = i - n * K;
-    float acc = 0.0f;
-    for (int64_t m = 0; m < tokens; ++m)
-      acc += to_f32(grad[m * N + n]) * (static_cast<float>(q[m * K + k]) * scale[m]);
-    grad_w[i] = from_f32<T>(acc);
+HLM_DEVICE uint32_t pack2_16(float a, float b);
+template <>
+HLM_DEVICE uint32_t pack2_16<__nv_bfloat16>(float a, float b) {
+  return pack_bf16x2(a, b);
+}
+template <>
+HLM_DEVICE uint32_t pack2_16<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Instruction descriptor for kind::f16 with MN-major operands of type T and fp32 D.
+template <typename T>
+constexpr uint32_t wg_idesc() {
+  constexpr uint32_t type = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;  // bf16 or f16
+  return (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+}
+
+// Write a 32-row x 32-column fp32 block per lane-row as rows of O (fp32 partial or the
+// 16-bit result): staged in a 32 x 128-byte box, out in 16-byte row segments.
+template <typename O>
+HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, int cols, uint32_t taddr,
+                              uint32_t buf, int lane) {
+  constexpr int kCols = 128 / static_cast<int>(sizeof(O));
+  constexpr int kPerChunk = 16 / static_cast<int>(sizeof(O));
+#pragma unroll 1
+  for (int g = 0; g < 256 / kCols; ++g) {
+    const int c0 = col0 + g * kCols;
+    if (c0 >= cols) break;
+    __syncwarp();  // the box's last group has been read
+#pragma unroll
+    for (int hs = 0; hs < kCols / 32; ++hs) {
+      uint32_t a[32];
+      tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * kCols + hs * 32), a);
+      tmem_ld_wait();
+      if constexpr (sizeof(O) == 4) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + ((c ^ (lane & 7)) << 4)),
+                       make_uint4(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = pack2_16<O>(__uint_as_float(a[8 * c + 2 * i]), __uint_as_float(a[8 * c + 2 * i + 1]));
+          st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + (((hs * 4 + c) ^ (lane & 7)) << 4)),
+                       make_uint4(w[0], w[1], w[2], w[3]));
+        }
+      }
+    }
+    __syncwarp();
+    const int chunk = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      const uint4 v = ld_shared_v4(buf + static_cast<uint32_t>(r * 128 + ((chunk ^ (r & 7)) << 4)));
+      if (row0 + r < rows && c0 + chunk * kPerChunk < cols)
+        st_global_v4(dst + static_cast<int64_t>(row0 + r) * ld + c0 + chunk * kPerChunk, v);
+    }
   }
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
+    weight_grad_q8_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_constant__ CUtensorMap tm_q,
+                          const float* __restrict__ scale, T* __restrict__ grad_w, float* __restrict__ partial,
+                          int tokens, const GemmParams p) {
+  using L = WgSmem;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw_addr);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t bar0 = base + L::kBarOffset;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + L::kTmemSlotOffset);
+  int* err = p.err;
+#define FULL_BAR(s) (bar0 + 8u * (s))                                // even CTA: both halves of A landed
+#define EMPTY_BAR(s) (bar0 + 8u * (kWgStages + (s)))                 // pair MMAs done with A
+#define RAWF_BAR(s) (bar0 + 8u * (2 * kWgStages + (s)))              // this CTA's codes landed
+#define RAWE_BAR(s) (bar0 + 8u * (3 * kWgStages + (s)))              // converters have read them
+#define BRDY_BAR(b) (bar0 + 8u * (4 * kWgStages + (b)))              // even CTA: both CTAs' B tiles written
+#define BEMP_BAR(b) (bar0 + 8u * (4 * kWgStages + kWgBStages + (b)))  // pair MMAs done with B
+#define TFULL_BAR(a) (bar0 + 8u * (4 * kWgStages + 2 * kWgBStages + (a)))
+#define TEMPTY_BAR(a) (bar0 + 8u * (4 * kWgStages + 2 * kWgBStages + 2 + (a)))
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kWgStages; ++s) {
+      mbar_init(FULL_BAR(s), 1);
+      mbar_init(EMPTY_BAR(s), 1);
+      mbar_init(RAWF_BAR(s), 1);
+      mbar_init(RAWE_BAR(s), kWgConvWarps);
+    }
+    for (int b = 0; b < kWgBStages; ++b) {
+      mbar_init(BRDY_BAR(b), 2 * kWgConvWarps);
+      mbar_init(BEMP_BAR(b), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(TFULL_BAR(a), 1);
+      mbar_init(TEMPTY_BAR(a), 2 * kWgEpiWarps);
+    }
+    fence_mbar_init();
+    prefetch_tensormap(&tm_g);
+    prefetch_tensormap(&tm_q);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // both CTAs' barriers initialised before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  const int total = p.m_tiles * p.n_tiles * p.splits;
+  const int w_first = static_cast<int>(cluster_id_x());
+  const int w_step = static_cast<int>(num_clusters_x());
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t armed = 0, armed_par = 0;  // stages whose loads are in flight, and their parity
+      bool ok = true;
+      for (int w = w_first; w < total && ok; w += w_step) {
+        int m_pair, n_tile, split;
+        decode_work(w, p, m_pair, n_tile, split);
+        const int n0 = (2 * m_pair + static_cast<int>(rank)) * kBM;
+        const int k0 = n_tile * 256 + static_cast<int>(rank) * 128;
+        const int kb0 = split * p.kb_per_split;
+        const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(EMPTY_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty) ||
+              !mbar_wait(RAWE_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(FULL_BAR(stage), 2 * L::kABytes);
+          mbar_arrive_expect_tx(RAWF_BAR(stage), L::kRawBytes);
+          armed |= 1u << stage;
+          armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+          const uint32_t full = mapa_shared(FULL_BAR(stage), 0);
+          const uint32_t sa = base + stage * L::kStageBytes;
+          tma_load_2d(sa + L::kABytes, &tm_q, k0, kb * kBK, RAWF_BAR(stage));
+          tma_load_2d_pair(sa, &tm_g, n0, kb * kBK, full);
+          tma_load_2d_pair(sa + 8192u, &tm_g, n0 + 64, kb * kBK, full);
+          if (++stage == kWgStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Every armed stage has landed before shared memory is released.
+      for (int s = 0; s < kWgStages; ++s) {
+        if (!(armed & (1u << s))) continue;
+        mbar_wait_drain(RAWF_BAR(s), (armed_par >> s) & 1u, err);
+        if (rank == 0) mbar_wait_drain(FULL_BAR(s), (armed_par >> s) & 1u, err);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ pair MMA issuer (even CTA)
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = wg_idesc<T>();
+      int stage = 0, bs = 0;
+      uint32_t phase = 0, bphase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int w = w_first; w < total && ok; w += w_step, ++it) {
+        int m_pair, n_tile, split;
+        decode_work(w, p, m_pair, n_tile, split);
+        const int kb0 = split * p.kb_per_split;
+        const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        const int acc = it & 1;
+        if (!mbar_wait_cluster(TEMPTY_BAR(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, err,
+                               kDevErrTimeoutTmemEmpty)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_cluster(FULL_BAR(stage), phase, err, kDevErrTimeoutFull) ||
+              !mbar_wait_cluster(BRDY_BAR(bs), bphase, err, kDevErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = base + stage * L::kStageBytes;
+          const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
+#pragma unroll
+          for (int kk = 0; kk < kBK / kUmmaK; ++kk)
+            tc_mma_f16_pair(d_tmem, make_sw128_desc(sa + kk * 2048u, 8192u, 1024u),
+                            make_sw128_desc(sb + kk * 2048u, 8192u, 1024u), idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+          tc_commit_pair(EMPTY_BAR(stage));
+          tc_commit_pair(mapa_shared(EMPTY_BAR(stage), 1));
+          tc_commit_pair(BEMP_BAR(bs));
+          tc_commit_pair(mapa_shared(BEMP_BAR(bs), 1));
+          if (++stage == kWgStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++bs == kWgBStages) {
+            bs = 0;
+            bphase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(TFULL_BAR(acc));
+        tc_commit_pair(mapa_shared(TFULL_BAR(acc), 1));
+      }
+    }
+  } else if (warp < kWgConvWarp0) {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quad = warp & 3;
+    const uint32_t buf = base + L::kBoxOffset + static_cast<uint32_t>(quad) * 4096u;
+    int it = 0;
+    for (int w = w_first; w < total; w += w_step, ++it) {
+      int m_pair, n_tile, split;
+      decode_work(w, p, m_pair, n_tile, split);
+      const int acc = it & 1;
+      if (!warp_wait(TFULL_BAR(acc), static_cast<uint32_t>(it >> 1) & 1u, err, kDevErrTimeoutTmemFull, lane)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * 256);
+      const int row0 = (2 * m_pair + static_cast<int>(rank)) * kBM + quad * 32;
+      if (partial != nullptr)
+        wg_store_tile<float>(partial + static_cast<int64_t>(split) * p.M * p.N, p.N, row0, p.M, n_tile * 256, p.N,
+                             taddr, buf, lane);
+      else
+        wg_store_tile<T>(grad_w, p.N, row0, p.M, n_tile * 256, p.N, taddr, buf, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(TEMPTY_BAR(acc), 0));
+    }
+  } else {
+    // ------------------------------------------------------------ converters (both CTAs)
+    // Two 16-byte pieces of codes per thread and block: token m = i / 8, piece c = i % 8 of its
+    // 128 features.  A piece becomes two 16-byte chunks of the read-back tile; pieces 0-3 (first
+    // box) write their even chunk first and pieces 4-7 (second box) their odd one, so that the
+    // eight lanes of a token fill eight different banks groups.
+    const int i0 = (warp - kWgConvWarp0) * 32 + lane;
+    int stage = 0, bs = 0;
+    uint32_t phase = 0, bphase = 0;
+    bool ok = true;
+    for (int w = w_first; w < total && ok; w += w_step) {
+      int m_pair, n_tile, split;
+      decode_work(w, p, m_pair, n_tile, split);
+      const int kb0 = split * p.kb_per_split;
+      const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        float sc[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int tok = kb * kBK + ((i0 + 256 * j) >> 3);
+          sc[j] = tok < tokens ? __ldg(scale + tok) : 0.0f;  // tokens past the end: codes and gradients are zeros
+        }
+        if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane)) {
+          ok = false;
+          break;
+        }
+        const uint32_t raw = base + stage * L::kStageBytes + L::kABytes;
+        uint4 v[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = i0 + 256 * j, m = i >> 3, c = i & 7;
+          v[j] = ld_shared_v4(raw + static_cast<uint32_t>(m * 128 + ((c ^ (m & 7)) << 4)));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(RAWE_BAR(stage));
+        uint4 o[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float f[4];
+            codes_to_float(words[k], f);
+            h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
+            h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
+          }
+          o[j][0] = make_uint4(h[0], h[1], h[2], h[3]);
+          o[j][1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        if (!warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
+          ok = false;
+          break;
+        }
+        const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = i0 + 256 * j, m = i >> 3, c = i & 7;
+          const uint32_t row = sb + static_cast<uint32_t>((c >> 2) * 8192 + m * 128);
+          const int first = c >> 2, ch = 2 * (c & 3);
+          st_shared_v4(row + static_cast<uint32_t>(((ch + first) ^ (m & 7)) << 4), first ? o[j][1] : o[j][0]);
+          st_shared_v4(row + static_cast<uint32_t>(((ch + 1 - first) ^ (m & 7)) << 4), first ? o[j][0] : o[j][1]);
+        }
+        fence_proxy_async_smem();  // the tensor cores read the tile
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(BRDY_BAR(bs), 0));
+        if (++stage == kWgStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        if (++bs == kWgBStages) {
+          bs = 0;
+          bphase ^= 1u;
+        }
+      }
+    }
+  }
+
+  // Neither CTA may leave while the other can still signal its barriers or the
+  // pair MMAs can still read its shared memory.
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+#undef FULL_BAR
+#undef EMPTY_BAR
+#undef RAWF_BAR
+#undef RAWE_BAR
+#undef BRDY_BAR
+#undef BEMP_BAR
+#undef TFULL_BAR
+#undef TEMPTY_BAR
+}
+
+// Sum of the splits' partials in their order, rounded to T; eight elements per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float* __restrict__ partial,
+                                                                   T* __restrict__ grad_w, int64_t n, int splits) {
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < n;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x * 8) {
+    float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(partial + s * n + i));
+      const float4 b = __ldcs(reinterpret_cast<const float4*>(partial + s * n + i + 4));
+      f[0] += a.x;
+      f[1] += a.y;
+      f[2] += a.z;
+      f[3] += a.w;
+      f[4] += b.x;
+      f[5] += b.y;
+      f[6] += b.z;
+      f[7] += b.w;
+    }
+    Vec16<T> o;
+    o.from_float(f);
+    st_global_v4(grad_w + i, o.raw);
+  }
+}
+
+// Splits of the tokens: the number that the cost in microseconds is least for, of
+// rounds of pair tiles at 0.4 us per 64 tokens, and, with partials, a second launch
+// (3 us) and 8 bytes per partial element at 6 TB/s.
+static int weight_grad_q8_splits(int64_t tokens, int64_t N, int64_t K) {
+  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
+  const int64_t pairs = num_sms_of_current_device() / 2;
+  const int64_t kb = (tokens + kBK - 1) / kBK;
+  int best = 1;
+  double best_us = 1e30;
+  for (int s = 1; s <= 32 && s <= kb; ++s) {
+    const int64_t per = (kb + s - 1) / s;
+    if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
+    double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (0.4 * static_cast<double>(per) + 2.0);
+    if (s > 1) us += 3.0 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 6.0e6;
+    if (us < best_us) {
+      best_us = us;
+      best = s;
+    }
+  }
+  return best;
+}
+
+template <typename T>
+static int weight_grad_q8(const void* grad, const void* q, const float* scale, T* grad_w, float* partial,
+                          int64_t tokens, int64_t N, int64_t K, int splits, cudaStream_t s) {
+  CUtensorMap mg, mq;
+  // g [tokens][N]: boxes of 64 output features x 64 tokens; q [tokens][K]: 128 features x 64 tokens
+  if (!encode_map(&mg, grad, 2, N, tokens, N, kBK) || !encode_map(&mq, q, 1, K, tokens, K, kBK))
+    return HLM_ERR_DRIVER;
+  GemmParams p;
+  gemm_tiling_pair(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), 256, splits);
+  p.err = device_error_ptr();
+  if (p.err == nullptr) return HLM_ERR_LAUNCH;
+  auto kern = weight_grad_q8_kernel<T>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WgSmem::kBytes) != cudaSuccess)
+    return HLM_ERR_LAUNCH;
+  const int64_t total = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
+  if (total > (1ll << 30)) return HLM_ERR_UNSUPPORTED;
+  int pairs = num_sms_of_current_device() / 2;
+  if (pairs > total) pairs = static_cast<int>(total);
+  {
+    LaunchScope scope(HLM_KERNEL_WEIGHT_GRAD_Q8, s);
+    kern<<<2 * pairs, kWgThreads, WgSmem::kBytes, s>>>(mg, mq, scale, grad_w, p.splits > 1 ? partial : nullptr,
+                                                       static_cast<int>(tokens), p);
+  }
+  const int rc = launch_status();
+  if (rc != HLM_OK || p.splits == 1) return rc;
+  const int64_t n = N * K;
+  const int64_t blocks = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms_of_current_device()) * 16;
+  {
+    LaunchScope scope(0, s);
+    weight_grad_q8_reduce_kernel<T><<<static_cast<int>(blocks < cap ? blocks : cap), 256, 0, s>>>(partial, grad_w, n,
+                                                                                               p.splits);
+  }
+  return launch_status();
 }
 
 }  // namespace hlm
 
 using namespace hlm;
 
-extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, int64_t K) {
+  if (tokens <= 0 || N <= 0 || K <= 0) return 0;
+  const int splits = weight_grad_q8_splits(tokens, N, K);
+  return splits > 1 ? static_cast<size_t>(splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * sizeof(float) : 0;
+}
 
 extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
                                   void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N,
@@ -43,19 +488,13 @@ extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* 
   }
   if (grad == nullptr || q == nullptr || scale == nullptr) return HLM_ERR_INVALID_ARG;
   if (!host_aligned16(grad) || !host_aligned16(q)) return HLM_ERR_UNSUPPORTED;
+  const int splits = weight_grad_q8_splits(tokens, N, K);
   const size_t need = hlm_weight_grad_q8_workspace_bytes(tokens, N, K);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return HLM_ERR_WORKSPACE;
-  const int64_t blocks64 = (N * K + 255) / 256;
-  const int64_t cap = static_cast<int64_t>(num_sms_of_current_device()) * 64;
-  const int blocks = static_cast<int>(blocks64 < cap ? blocks64 : cap);
-  LaunchScope scope(HLM_KERNEL_WEIGHT_GRAD_Q8, s);
+  if (need > 0 && !host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
   if (dtype == HLM_BF16)
-    weight_grad_q8_simple_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(grad), static_cast<const int8_t*>(q), scale,
-        static_cast<__nv_bfloat16*>(grad_w), tokens, N, K);
-  else
-    weight_grad_q8_simple_kernel<__half><<<blocks, 256, 0, s>>>(
-        static_cast<const __half*>(grad), static_cast<const int8_t*>(q), scale,
-        static_cast<__half*>(grad_w), tokens, N, K);
-  return launch_status();
+    return weight_grad_q8<__nv_bfloat16>(grad, q, scale, static_cast<__nv_bfloat16*>(grad_w),
+                                         static_cast<float*>(workspace), tokens, N, K, splits, s);
+  return weight_grad_q8<__half>(grad, q, scale, static_cast<__half*>(grad_w), static_cast<float*>(workspace), tokens,
+                                N, K, splits, s);
 }
