@@ -21,9 +21,11 @@
 
 namespace hlm {
 
-constexpr int kWgStages = 6;
-constexpr int kWgBStages = 3;
-constexpr int kWgConvWarps = 8;
+constexpr int kWgStages = 5;
+constexpr int kWgBStages = 5;
+constexpr int kWgGroups = 4;     // converter groups: group g makes every fourth block's tile
+constexpr int kWgGroupWarps = 2;
+constexpr int kWgConvWarps = kWgGroups * kWgGroupWarps;
 constexpr int kWgEpiWarps = 4;
 constexpr int kWgConvWarp0 = kEpiWarp0 + kWgEpiWarps;
 constexpr int kWgThreads = 32 * (kWgConvWarp0 + kWgConvWarps);
@@ -137,10 +139,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       mbar_init(FULL_BAR(s), 1);
       mbar_init(EMPTY_BAR(s), 1);
       mbar_init(RAWF_BAR(s), 1);
-      mbar_init(RAWE_BAR(s), kWgConvWarps);
+      mbar_init(RAWE_BAR(s), kWgGroupWarps);
     }
     for (int b = 0; b < kWgBStages; ++b) {
-      mbar_init(BRDY_BAR(b), 2 * kWgConvWarps);
+      mbar_init(BRDY_BAR(b), 2 * kWgGroupWarps);
       mbar_init(BEMP_BAR(b), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -282,12 +284,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ converters (both CTAs)
-    // Two 16-byte pieces of codes per thread and block: token m = i / 8, piece c = i % 8 of its
-    // 128 features.  A piece becomes two 16-byte chunks of the read-back tile; pieces 0-3 (first
-    // box) write their even chunk first and pieces 4-7 (second box) their odd one, so that the
-    // eight lanes of a token fill eight different banks groups.
-    const int i0 = (warp - kWgConvWarp0) * 32 + lane;
-    int stage = 0, bs = 0;
+    // A group's 64 threads make one block's tile, eight 16-byte pieces of codes each: token
+    // m = i / 8, piece c = i % 8 of its 128 features.  A piece becomes two 16-byte chunks of the
+    // read-back tile; pieces 0-3 (first box) write their even chunk first and pieces 4-7 (second
+    // box) their odd one, so that the eight lanes of a token write to different banks.  Groups
+    // and not all warps on one block: the wait, the proxy fence and the arrive of a block are
+    // latency, which four groups overlap (one group of eight warps: 1.4 us a block).
+    constexpr int kThreads = 32 * kWgGroupWarps;
+    constexpr int kPieces = 512 / kThreads;
+    const int group = (warp - kWgConvWarp0) / kWgGroupWarps;
+    const int i0 = ((warp - kWgConvWarp0) % kWgGroupWarps) * 32 + lane;
+    const int c = i0 & 7;  // the same piece column in every step: kThreads is a multiple of 8
+    const int first = c >> 2, ch = 2 * (c & 3);
+    int stage = 0, bs = 0, turn = 0;
     uint32_t phase = 0, bphase = 0;
     bool ok = true;
     for (int w = w_first; w < total && ok; w += w_step) {
@@ -296,56 +305,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       const int kb0 = split * p.kb_per_split;
       const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
       for (int kb = kb0; kb < kb1; ++kb) {
-        float sc[2];
+        if (turn == group) {
+          float sc[kPieces];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = kb * kBK + ((i0 + 256 * j) >> 3);
-          sc[j] = tok < tokens ? __ldg(scale + tok) : 0.0f;  // tokens past the end: codes and gradients are zeros
-        }
-        if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane)) {
-          ok = false;
-          break;
-        }
-        const uint32_t raw = base + stage * L::kStageBytes + L::kABytes;
-        uint4 v[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int i = i0 + 256 * j, m = i >> 3, c = i & 7;
-          v[j] = ld_shared_v4(raw + static_cast<uint32_t>(m * 128 + ((c ^ (m & 7)) << 4)));
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(RAWE_BAR(stage));
-        uint4 o[2][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float f[4];
-            codes_to_float(words[k], f);
-            h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
-            h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
+          for (int j = 0; j < kPieces; ++j) {
+            const int tok = kb * kBK + ((i0 + kThreads * j) >> 3);
+            sc[j] = tok < tokens ? __ldg(scale + tok) : 0.0f;  // tokens past the end: codes and gradients are zeros
           }
-          o[j][0] = make_uint4(h[0], h[1], h[2], h[3]);
-          o[j][1] = make_uint4(h[4], h[5], h[6], h[7]);
-        }
-        if (!warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
-          ok = false;
-          break;
-        }
-        const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
+          if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane) ||
+              !warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
+            ok = false;
+            break;
+          }
+          const uint32_t raw = base + stage * L::kStageBytes + L::kABytes;
+          const uint32_t sb = base + L::kBOffset + bs * L::kBBytes + static_cast<uint32_t>(first * 8192);
+          uint4 v[kPieces];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int i = i0 + 256 * j, m = i >> 3, c = i & 7;
-          const uint32_t row = sb + static_cast<uint32_t>((c >> 2) * 8192 + m * 128);
-          const int first = c >> 2, ch = 2 * (c & 3);
-          st_shared_v4(row + static_cast<uint32_t>(((ch + first) ^ (m & 7)) << 4), first ? o[j][1] : o[j][0]);
-          st_shared_v4(row + static_cast<uint32_t>(((ch + 1 - first) ^ (m & 7)) << 4), first ? o[j][0] : o[j][1]);
+          for (int j = 0; j < kPieces; ++j) {
+            const int m = (i0 + kThreads * j) >> 3;
+            v[j] = ld_shared_v4(raw + static_cast<uint32_t>(m * 128 + ((c ^ (m & 7)) << 4)));
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(RAWE_BAR(stage));
+#pragma unroll
+          for (int j = 0; j < kPieces; ++j) {
+            const int m = (i0 + kThreads * j) >> 3;
+            const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float f[4];
+              codes_to_float(words[k], f);
+              h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
+              h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
+            }
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            const uint32_t row = sb + static_cast<uint32_t>(m * 128);
+            st_shared_v4(row + static_cast<uint32_t>(((ch + first) ^ (m & 7)) << 4), first ? hi : lo);
+            st_shared_v4(row + static_cast<uint32_t>(((ch + 1 - first) ^ (m & 7)) << 4), first ? lo : hi);
+          }
+          fence_proxy_async_smem();  // the tensor cores read the tile
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(BRDY_BAR(bs), 0));
         }
-        fence_proxy_async_smem();  // the tensor cores read the tile
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(BRDY_BAR(bs), 0));
+        if (++turn == kWgGroups) turn = 0;
         if (++stage == kWgStages) {
           stage = 0;
           phase ^= 1u;
