@@ -21,24 +21,26 @@
 
 namespace hlm {
 
-constexpr int kWgStages = 5;
-constexpr int kWgBStages = 5;
+constexpr int kWgStages = 5;     // A tiles
+constexpr int kWgRawStages = 6;  // codes: their own ring and producer, so that they run ahead of A
+constexpr int kWgBStages = 5;    // read-back tiles
 constexpr int kWgGroups = 4;     // converter groups: group g makes every fourth block's tile
 constexpr int kWgGroupWarps = 2;
 constexpr int kWgConvWarps = kWgGroups * kWgGroupWarps;
 constexpr int kWgEpiWarps = 4;
 constexpr int kWgConvWarp0 = kEpiWarp0 + kWgEpiWarps;
-constexpr int kWgThreads = 32 * (kWgConvWarp0 + kWgConvWarps);
+constexpr int kWgRawWarp = kWgConvWarp0 + kWgConvWarps;
+constexpr int kWgThreads = 32 * (kWgRawWarp + 1);
 
 struct WgSmem {
   static constexpr int kABytes = kBM * kBK * 2;  // 128 output features x 64 tokens, 16-bit
   static constexpr int kRawBytes = 128 * kBK;    // 128 input features x 64 tokens, codes
-  static constexpr int kStageBytes = kABytes + kRawBytes;
   static constexpr int kBBytes = 128 * kBK * 2;  // the same, read back
-  static constexpr int kBOffset = kWgStages * kStageBytes;
+  static constexpr int kRawOffset = kWgStages * kABytes;
+  static constexpr int kBOffset = kRawOffset + kWgRawStages * kRawBytes;
   static constexpr int kBoxOffset = kBOffset + kWgBStages * kBBytes;  // epilogue boxes, 4 KB per warp
   static constexpr int kBarOffset = kBoxOffset + kWgEpiWarps * 4096;
-  static constexpr int kNumBars = 4 * kWgStages + 2 * kWgBStages + 4;
+  static constexpr int kNumBars = 2 * kWgStages + 2 * kWgRawStages + 2 * kWgBStages + 4;
   static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
   static constexpr int kBytes = kTmemSlotOffset + 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory budget exceeded");
@@ -127,19 +129,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
   int* err = p.err;
 #define FULL_BAR(s) (bar0 + 8u * (s))                                // even CTA: both halves of A landed
 #define EMPTY_BAR(s) (bar0 + 8u * (kWgStages + (s)))                 // pair MMAs done with A
-#define RAWF_BAR(s) (bar0 + 8u * (2 * kWgStages + (s)))              // this CTA's codes landed
-#define RAWE_BAR(s) (bar0 + 8u * (3 * kWgStages + (s)))              // converters have read them
-#define BRDY_BAR(b) (bar0 + 8u * (4 * kWgStages + (b)))              // even CTA: both CTAs' B tiles written
-#define BEMP_BAR(b) (bar0 + 8u * (4 * kWgStages + kWgBStages + (b)))  // pair MMAs done with B
-#define TFULL_BAR(a) (bar0 + 8u * (4 * kWgStages + 2 * kWgBStages + (a)))
-#define TEMPTY_BAR(a) (bar0 + 8u * (4 * kWgStages + 2 * kWgBStages + 2 + (a)))
+#define RAWF_BAR(r) (bar0 + 8u * (2 * kWgStages + (r)))              // this CTA's codes landed
+#define RAWE_BAR(r) (bar0 + 8u * (2 * kWgStages + kWgRawStages + (r)))  // converters have read them
+#define BAR_B0 (2 * kWgStages + 2 * kWgRawStages)
+#define BRDY_BAR(b) (bar0 + 8u * (BAR_B0 + (b)))                     // even CTA: both CTAs' B tiles written
+#define BEMP_BAR(b) (bar0 + 8u * (BAR_B0 + kWgBStages + (b)))        // pair MMAs done with B
+#define TFULL_BAR(a) (bar0 + 8u * (BAR_B0 + 2 * kWgBStages + (a)))
+#define TEMPTY_BAR(a) (bar0 + 8u * (BAR_B0 + 2 * kWgBStages + 2 + (a)))
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < kWgStages; ++s) {
       mbar_init(FULL_BAR(s), 1);
       mbar_init(EMPTY_BAR(s), 1);
-      mbar_init(RAWF_BAR(s), 1);
-      mbar_init(RAWE_BAR(s), kWgGroupWarps);
+    }
+    for (int r = 0; r < kWgRawStages; ++r) {
+      mbar_init(RAWF_BAR(r), 1);
+      mbar_init(RAWE_BAR(r), kWgGroupWarps);
     }
     for (int b = 0; b < kWgBStages; ++b) {
       mbar_init(BRDY_BAR(b), 2 * kWgGroupWarps);
@@ -167,7 +172,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
   const int w_step = static_cast<int>(num_clusters_x());
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer
+    // ------------------------------------------------------------ producer of A
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
@@ -177,22 +182,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
         int m_pair, n_tile, split;
         decode_work(w, p, m_pair, n_tile, split);
         const int n0 = (2 * m_pair + static_cast<int>(rank)) * kBM;
-        const int k0 = n_tile * 256 + static_cast<int>(rank) * 128;
         const int kb0 = split * p.kb_per_split;
         const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(EMPTY_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty) ||
-              !mbar_wait(RAWE_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty)) {
+          if (!mbar_wait(EMPTY_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(FULL_BAR(stage), 2 * L::kABytes);
-          mbar_arrive_expect_tx(RAWF_BAR(stage), L::kRawBytes);
-          armed |= 1u << stage;
-          armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+          if (rank == 0) {
+            mbar_arrive_expect_tx(FULL_BAR(stage), 2 * L::kABytes);
+            armed |= 1u << stage;
+            armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+          }
           const uint32_t full = mapa_shared(FULL_BAR(stage), 0);
-          const uint32_t sa = base + stage * L::kStageBytes;
-          tma_load_2d(sa + L::kABytes, &tm_q, k0, kb * kBK, RAWF_BAR(stage));
+          const uint32_t sa = base + stage * L::kABytes;
           tma_load_2d_pair(sa, &tm_g, n0, kb * kBK, full);
           tma_load_2d_pair(sa + 8192u, &tm_g, n0 + 64, kb * kBK, full);
           if (++stage == kWgStages) {
@@ -201,12 +204,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
           }
         }
       }
-      // Every armed stage has landed before shared memory is released.
-      for (int s = 0; s < kWgStages; ++s) {
-        if (!(armed & (1u << s))) continue;
-        mbar_wait_drain(RAWF_BAR(s), (armed_par >> s) & 1u, err);
-        if (rank == 0) mbar_wait_drain(FULL_BAR(s), (armed_par >> s) & 1u, err);
+      // Drain (even CTA): every armed stage, including the peer's half, has landed before
+      // either CTA releases its shared memory.
+      for (int s = 0; s < kWgStages; ++s)
+        if (armed & (1u << s)) mbar_wait_drain(FULL_BAR(s), (armed_par >> s) & 1u, err);
+    }
+  } else if (warp == kWgRawWarp) {
+    // ------------------------------------------------------------ producer of the codes
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t armed = 0, armed_par = 0;
+      bool ok = true;
+      for (int w = w_first; w < total && ok; w += w_step) {
+        int m_pair, n_tile, split;
+        decode_work(w, p, m_pair, n_tile, split);
+        const int k0 = n_tile * 256 + static_cast<int>(rank) * 128;
+        const int kb0 = split * p.kb_per_split;
+        const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(RAWE_BAR(stage), phase ^ 1u, err, kDevErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(RAWF_BAR(stage), L::kRawBytes);
+          armed |= 1u << stage;
+          armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+          tma_load_2d(base + L::kRawOffset + stage * L::kRawBytes, &tm_q, k0, kb * kBK, RAWF_BAR(stage));
+          if (++stage == kWgRawStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
       }
+      for (int s = 0; s < kWgRawStages; ++s)
+        if (armed & (1u << s)) mbar_wait_drain(RAWF_BAR(s), (armed_par >> s) & 1u, err);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ pair MMA issuer (even CTA)
@@ -236,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t sa = base + stage * L::kStageBytes;
+          const uint32_t sa = base + stage * L::kABytes;
           const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
 #pragma unroll
           for (int kk = 0; kk < kBK / kUmmaK; ++kk)
@@ -284,18 +316,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ converters (both CTAs)
-    // A group's 64 threads make one block's tile, eight 16-byte pieces of codes each: token
-    // m = i / 8, piece c = i % 8 of its 128 features.  A piece becomes two 16-byte chunks of the
-    // read-back tile; pieces 0-3 (first box) write their even chunk first and pieces 4-7 (second
-    // box) their odd one, so that the eight lanes of a token write to different banks.  Groups
-    // and not all warps on one block: the wait, the proxy fence and the arrive of a block are
-    // latency, which four groups overlap (one group of eight warps: 1.4 us a block).
-    constexpr int kThreads = 32 * kWgGroupWarps;
-    constexpr int kPieces = 512 / kThreads;
+    // A group's two warps make one block's tile (groups and not all warps on one block: the
+    // waits, the proxy fence and the arrive of a block are latency, which four groups
+    // overlap).  Warp b of a group makes box b (64 features): in each of eight steps its
+    // lanes take eight tokens x four 16-byte pieces of codes, and a piece becomes two
+    // 16-byte chunks of the read-back box.  The eight lanes that access shared memory
+    // together hold tokens m and m ^ 5: under the 128-byte swizzle both their reads
+    // (bit 2 differs) and their writes (bit 0 differs) fall on eight different chunks.
     const int group = (warp - kWgConvWarp0) / kWgGroupWarps;
-    const int i0 = ((warp - kWgConvWarp0) % kWgGroupWarps) * 32 + lane;
-    const int c = i0 & 7;  // the same piece column in every step: kThreads is a multiple of 8
-    const int first = c >> 2, ch = 2 * (c & 3);
+    const int box = (warp - kWgConvWarp0) % kWgGroupWarps;
+    const int piece = lane & 3;
+    const int m7 = (lane >> 3) ^ ((lane & 4) ? 5 : 0);  // token within a step
+    const uint32_t rd = static_cast<uint32_t>(m7 * 128 + (((4 * box + piece) ^ m7) << 4));
+    const uint32_t wr0 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece) ^ m7) << 4));
+    const uint32_t wr1 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece + 1) ^ m7) << 4));
     int stage = 0, bs = 0, turn = 0;
     uint32_t phase = 0, bphase = 0;
     bool ok = true;
@@ -306,50 +340,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (turn == group) {
-          float sc[kPieces];
+          float sc[8];
+          const int tok = kb * kBK + m7;
+          if (tok + 56 < tokens) {
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            const int tok = kb * kBK + ((i0 + kThreads * j) >> 3);
-            sc[j] = tok < tokens ? __ldg(scale + tok) : 0.0f;  // tokens past the end: codes and gradients are zeros
+            for (int j = 0; j < 8; ++j) sc[j] = __ldg(scale + tok + 8 * j);
+          } else {  // tokens past the end: their codes and gradients arrive as zeros
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[j] = tok + 8 * j < tokens ? __ldg(scale + tok + 8 * j) : 0.0f;
           }
           if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane) ||
               !warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
             ok = false;
             break;
           }
-          const uint32_t raw = base + stage * L::kStageBytes + L::kABytes;
-          const uint32_t sb = base + L::kBOffset + bs * L::kBBytes + static_cast<uint32_t>(first * 8192);
-          uint4 v[kPieces];
+          const uint32_t raw = base + L::kRawOffset + stage * L::kRawBytes + rd;
+          const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
+          uint4 v[8];
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            const int m = (i0 + kThreads * j) >> 3;
-            v[j] = ld_shared_v4(raw + static_cast<uint32_t>(m * 128 + ((c ^ (m & 7)) << 4)));
-          }
+          for (int j = 0; j < 8; ++j) v[j] = ld_shared_v4(raw + j * 1024u);
           __syncwarp();
           if (lane == 0) mbar_arrive(RAWE_BAR(stage));
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            const int m = (i0 + kThreads * j) >> 3;
+          for (int j = 0; j < 8; ++j) {
             const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
             uint32_t h[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               float f[4];
-              codes_to_float(words[k], f);
+              codes_to_float_dp4a(words[k], f);
               h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
               h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
             }
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            const uint32_t row = sb + static_cast<uint32_t>(m * 128);
-            st_shared_v4(row + static_cast<uint32_t>(((ch + first) ^ (m & 7)) << 4), first ? hi : lo);
-            st_shared_v4(row + static_cast<uint32_t>(((ch + 1 - first) ^ (m & 7)) << 4), first ? lo : hi);
+            st_shared_v4(sb + wr0 + j * 1024u, make_uint4(h[0], h[1], h[2], h[3]));
+            st_shared_v4(sb + wr1 + j * 1024u, make_uint4(h[4], h[5], h[6], h[7]));
           }
           fence_proxy_async_smem();  // the tensor cores read the tile
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(BRDY_BAR(bs), 0));
         }
         if (++turn == kWgGroups) turn = 0;
-        if (++stage == kWgStages) {
+        if (++stage == kWgRawStages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -376,6 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
 #undef RAWE_BAR
 #undef BRDY_BAR
 #undef BEMP_BAR
+#undef BAR_B0
 #undef TFULL_BAR
 #undef TEMPTY_BAR
 }
