@@ -330,6 +330,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
     const uint32_t rd = static_cast<uint32_t>(m7 * 128 + (((4 * box + piece) ^ m7) << 4));
     const uint32_t wr0 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece) ^ m7) << 4));
     const uint32_t wr1 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece + 1) ^ m7) << 4));
+    float sc[8];     // scales of this lane's tokens in block sc_kb
+    int sc_kb = -1;
+    auto load_scales = [&](int kb) {
+      const int tok = kb * kBK + m7;
+      sc_kb = kb;
+      if (tok + 56 < tokens) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = __ldg(scale + tok + 8 * j);
+      } else {  // tokens past the end: their codes and gradients arrive as zeros
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = tok + 8 * j < tokens ? __ldg(scale + tok + 8 * j) : 0.0f;
+      }
+    };
     int stage = 0, bs = 0, turn = 0;
     uint32_t phase = 0, bphase = 0;
     bool ok = true;
@@ -340,17 +353,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (turn == group) {
-          float sc[8];
-          const int tok = kb * kBK + m7;
-          if (tok + 56 < tokens) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[j] = __ldg(scale + tok + 8 * j);
-          } else {  // tokens past the end: their codes and gradients arrive as zeros
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[j] = tok + 8 * j < tokens ? __ldg(scale + tok + 8 * j) : 0.0f;
-          }
-          if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane) ||
-              !warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
+          if (sc_kb != kb) load_scales(kb);
+          if (!warp_wait(RAWF_BAR(stage), phase, err, kDevErrTimeoutFull, lane)) {
             ok = false;
             break;
           }
@@ -361,6 +365,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
           for (int j = 0; j < 8; ++j) v[j] = ld_shared_v4(raw + j * 1024u);
           __syncwarp();
           if (lane == 0) mbar_arrive(RAWE_BAR(stage));
+          // converted in registers before the wait for the tile's previous reader: what that
+          // wait delays is only the stores
+          uint4 o[8][2];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
@@ -372,8 +379,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
               h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
               h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
             }
-            st_shared_v4(sb + wr0 + j * 1024u, make_uint4(h[0], h[1], h[2], h[3]));
-            st_shared_v4(sb + wr1 + j * 1024u, make_uint4(h[4], h[5], h[6], h[7]));
+            o[j][0] = make_uint4(h[0], h[1], h[2], h[3]);
+            o[j][1] = make_uint4(h[4], h[5], h[6], h[7]);
+          }
+          // the group's next block in this split: its scales, a global load away
+          if (kb + kWgGroups < kb1) load_scales(kb + kWgGroups);
+          if (!warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            st_shared_v4(sb + wr0 + j * 1024u, o[j][0]);
+            st_shared_v4(sb + wr1 + j * 1024u, o[j][1]);
           }
           fence_proxy_async_smem();  // the tensor cores read the tile
           __syncwarp();
