@@ -2,16 +2,17 @@
 //
 //   grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m])
 //
-// One CTA-pair tcgen05 GEMM (256 x 256 tiles of grad_w, tokens as the reduction),
+// One CTA-pair tcgen05 GEMM (512 x 256 tiles of grad_w, tokens as the reduction),
 // whose B operand is made in the kernel: TMA brings the int8 codes of 64 tokens x
 // 128 input features per CTA, eight converter warps read them back to the gradient's
 // type (q * scale in fp32, rounded once: the MMA takes one 16-bit type for both
 // operands) and write the swizzled MN-major tile that the MMA reads.  The codes are
 // half the bytes of the activations, and no read-back tensor goes to memory.
 //
-// Per 64 tokens the pair's MMA takes about 370 ns at the measured bf16 rate; the
-// converters need about 280 issue slots of each SM quarter for the 8192 codes of a
-// CTA, so the tensor cores stay the bound.
+// A tile is two 256-row MMAs on the same B: each converted value feeds 512 rows.
+// With one 256-row MMA (two accumulators instead, the epilogue overlapped) the
+// converters' shared-memory traffic and latency held the tensor cores to 990
+// TFLOP/s at [2048 tokens, 8192, 8192].
 //
 // Few tiles: the tokens are split and each split writes an fp32 partial to the
 // workspace; a second kernel adds the partials in the order of the splits (the same
@@ -21,26 +22,34 @@
 
 namespace hlm {
 
-constexpr int kWgStages = 5;     // A tiles
-constexpr int kWgRawStages = 6;  // codes: their own ring and producer, so that they run ahead of A
-constexpr int kWgBStages = 5;    // read-back tiles
-constexpr int kWgGroups = 4;     // converter groups: group g makes every fourth block's tile
-constexpr int kWgGroupWarps = 2;
+constexpr int kWgStages = 4;     // A tiles
+constexpr int kWgRawStages = 4;  // codes: their own ring and producer, so that they run ahead of A
+constexpr int kWgBStages = 3;    // read-back tiles
+constexpr int kWgGroups = 2;     // converter groups, which take turns on the token blocks
+constexpr int kWgGroupWarps = 4;
+// A group skips the barrier phases of the other groups' blocks, and a parity wait tells
+// a phase only from its neighbours, so the phase before the awaited one must be known
+// to be over.  Read-back tiles: the group's last block n waited for the MMAs of block
+// n - kWgBStages, and n + kWgGroups - 2 kWgBStages is not after it.  Codes: block
+// n - kWgRawStages was the group's own.
+static_assert(kWgBStages >= kWgGroups && kWgRawStages % kWgGroups == 0, "unambiguous phases");
 constexpr int kWgConvWarps = kWgGroups * kWgGroupWarps;
-constexpr int kWgEpiWarps = 4;
+constexpr int kWgEpiWarps = 8;  // two per TMEM lane quadrant, one for each half of the tile's rows
 constexpr int kWgConvWarp0 = kEpiWarp0 + kWgEpiWarps;
 constexpr int kWgRawWarp = kWgConvWarp0 + kWgConvWarps;
+constexpr int kWgBM = 512;       // rows (output features) of a pair's tile
 constexpr int kWgThreads = 32 * (kWgRawWarp + 1);
 
 struct WgSmem {
-  static constexpr int kABytes = kBM * kBK * 2;  // 128 output features x 64 tokens, 16-bit
+  static constexpr int kSubBytes = kBM * kBK * 2;  // 128 output features x 64 tokens, 16-bit
+  static constexpr int kABytes = 2 * kSubBytes;  // this CTA's rows of the two MMAs
   static constexpr int kRawBytes = 128 * kBK;    // 128 input features x 64 tokens, codes
   static constexpr int kBBytes = 128 * kBK * 2;  // the same, read back
   static constexpr int kRawOffset = kWgStages * kABytes;
   static constexpr int kBOffset = kRawOffset + kWgRawStages * kRawBytes;
-  static constexpr int kBoxOffset = kBOffset + kWgBStages * kBBytes;  // epilogue boxes, 4 KB per warp
-  static constexpr int kBarOffset = kBoxOffset + kWgEpiWarps * 4096;
-  static constexpr int kNumBars = 2 * kWgStages + 2 * kWgRawStages + 2 * kWgBStages + 4;
+  static constexpr int kBoxOffset = kBOffset + kWgBStages * kBBytes;  // epilogue boxes, 2 KB per warp
+  static constexpr int kBarOffset = kBoxOffset + kWgEpiWarps * 2048;
+  static constexpr int kNumBars = 2 * kWgStages + 2 * kWgRawStages + 2 * kWgBStages + 3;
   static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
   static constexpr int kBytes = kTmemSlotOffset + 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory budget exceeded");
@@ -65,48 +74,48 @@ constexpr uint32_t wg_idesc() {
   return (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 }
 
-// Write a 32-row x 32-column fp32 block per lane-row as rows of O (fp32 partial or the
-// 16-bit result): staged in a 32 x 128-byte box, out in 16-byte row segments.
+// Write a warp's 32 rows x 256 columns of the accumulator as O (fp32 partial or the
+// 16-bit result): staged in a 32 x 64-byte box (16-byte chunks swizzled by row pairs),
+// out in 16-byte stores, eight 64-byte row segments per instruction.
 template <typename O>
 HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, int cols, uint32_t taddr,
                               uint32_t buf, int lane) {
-  constexpr int kCols = 128 / static_cast<int>(sizeof(O));
+  constexpr int kCols = 64 / static_cast<int>(sizeof(O));  // columns of a box: 16 fp32 or 32 16-bit
   constexpr int kPerChunk = 16 / static_cast<int>(sizeof(O));
+  if (row0 >= rows) return;
+  const uint32_t sw = static_cast<uint32_t>(lane >> 1) & 3u;
 #pragma unroll 1
-  for (int g = 0; g < 256 / kCols; ++g) {
-    const int c0 = col0 + g * kCols;
-    if (c0 >= cols) break;
-    __syncwarp();  // the box's last group has been read
+  for (int g = 0; g < 8; ++g) {
+    if (col0 + 32 * g >= cols) break;
+    uint32_t a[32];
+    tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * 32), a);
+    tmem_ld_wait();
 #pragma unroll
-    for (int hs = 0; hs < kCols / 32; ++hs) {
-      uint32_t a[32];
-      tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * kCols + hs * 32), a);
-      tmem_ld_wait();
-      if constexpr (sizeof(O) == 4) {
+    for (int hs = 0; hs < 32 / kCols; ++hs) {
+      __syncwarp();  // the box's last columns have been read
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + ((c ^ (lane & 7)) << 4)),
-                       make_uint4(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; ++c) {
+        uint4 v;
+        if constexpr (sizeof(O) == 4) {
+          v = make_uint4(a[16 * hs + 4 * c], a[16 * hs + 4 * c + 1], a[16 * hs + 4 * c + 2], a[16 * hs + 4 * c + 3]);
+        } else {
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             w[i] = pack2_16<O>(__uint_as_float(a[8 * c + 2 * i]), __uint_as_float(a[8 * c + 2 * i + 1]));
-          st_shared_v4(buf + static_cast<uint32_t>(lane * 128 + (((hs * 4 + c) ^ (lane & 7)) << 4)),
-                       make_uint4(w[0], w[1], w[2], w[3]));
+          v = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        st_shared_v4(buf + static_cast<uint32_t>(lane * 64) + ((static_cast<uint32_t>(c) ^ sw) << 4), v);
       }
-    }
-    __syncwarp();
-    const int chunk = lane & 7;
+      __syncwarp();
+      const int chunk = lane & 3;
+      const int c0 = col0 + 32 * g + hs * kCols + chunk * kPerChunk;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3);
-      const uint4 v = ld_shared_v4(buf + static_cast<uint32_t>(r * 128 + ((chunk ^ (r & 7)) << 4)));
-      if (row0 + r < rows && c0 + chunk * kPerChunk < cols)
-        st_global_v4(dst + static_cast<int64_t>(row0 + r) * ld + c0 + chunk * kPerChunk, v);
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        const uint4 v = ld_shared_v4(buf + static_cast<uint32_t>(r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4)));
+        if (row0 + r < rows && c0 < cols) st_global_v4(dst + static_cast<int64_t>(row0 + r) * ld + c0, v);
+      }
     }
   }
 }
@@ -134,8 +143,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
 #define BAR_B0 (2 * kWgStages + 2 * kWgRawStages)
 #define BRDY_BAR(b) (bar0 + 8u * (BAR_B0 + (b)))                     // even CTA: both CTAs' B tiles written
 #define BEMP_BAR(b) (bar0 + 8u * (BAR_B0 + kWgBStages + (b)))        // pair MMAs done with B
-#define TFULL_BAR(a) (bar0 + 8u * (BAR_B0 + 2 * kWgBStages + (a)))
-#define TEMPTY_BAR(a) (bar0 + 8u * (BAR_B0 + 2 * kWgBStages + 2 + (a)))
+#define TFULL_BAR (bar0 + 8u * (BAR_B0 + 2 * kWgBStages))
+#define TEMPTY_BAR(h) (bar0 + 8u * (BAR_B0 + 2 * kWgBStages + 1 + (h)))  // even CTA: half h of the tile drained
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < kWgStages; ++s) {
@@ -150,10 +159,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       mbar_init(BRDY_BAR(b), 2 * kWgGroupWarps);
       mbar_init(BEMP_BAR(b), 1);
     }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(TFULL_BAR(a), 1);
-      mbar_init(TEMPTY_BAR(a), 2 * kWgEpiWarps);
-    }
+    mbar_init(TFULL_BAR, 1);
+    for (int h = 0; h < 2; ++h) mbar_init(TEMPTY_BAR(h), kWgEpiWarps);  // four warps of each CTA
     fence_mbar_init();
     prefetch_tensormap(&tm_g);
     prefetch_tensormap(&tm_q);
@@ -181,7 +188,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       for (int w = w_first; w < total && ok; w += w_step) {
         int m_pair, n_tile, split;
         decode_work(w, p, m_pair, n_tile, split);
-        const int n0 = (2 * m_pair + static_cast<int>(rank)) * kBM;
+        const int n0 = m_pair * kWgBM + static_cast<int>(rank) * kBM;
+        const int subs = m_pair * kWgBM + 256 < p.M ? 2 : 1;  // 256-row MMAs with rows in them
         const int kb0 = split * p.kb_per_split;
         const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -190,14 +198,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
             break;
           }
           if (rank == 0) {
-            mbar_arrive_expect_tx(FULL_BAR(stage), 2 * L::kABytes);
+            mbar_arrive_expect_tx(FULL_BAR(stage), static_cast<uint32_t>(subs) * 2 * L::kSubBytes);
             armed |= 1u << stage;
             armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
           }
           const uint32_t full = mapa_shared(FULL_BAR(stage), 0);
           const uint32_t sa = base + stage * L::kABytes;
-          tma_load_2d_pair(sa, &tm_g, n0, kb * kBK, full);
-          tma_load_2d_pair(sa + 8192u, &tm_g, n0 + 64, kb * kBK, full);
+          for (int h = 0; h < subs; ++h) {
+            tma_load_2d_pair(sa + h * L::kSubBytes, &tm_g, n0 + 256 * h, kb * kBK, full);
+            tma_load_2d_pair(sa + h * L::kSubBytes + 8192u, &tm_g, n0 + 256 * h + 64, kb * kBK, full);
+          }
           if (++stage == kWgStages) {
             stage = 0;
             phase ^= 1u;
@@ -253,14 +263,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
         decode_work(w, p, m_pair, n_tile, split);
         const int kb0 = split * p.kb_per_split;
         const int kb1 = min(kb0 + p.kb_per_split, p.k_blocks);
-        const int acc = it & 1;
-        if (!mbar_wait_cluster(TEMPTY_BAR(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, err,
-                               kDevErrTimeoutTmemEmpty)) {
+        const int subs = m_pair * kWgBM + 256 < p.M ? 2 : 1;
+        const uint32_t free_par = (static_cast<uint32_t>(it) & 1u) ^ 1u;
+        if (!mbar_wait_cluster(TEMPTY_BAR(0), free_par, err, kDevErrTimeoutTmemEmpty) ||
+            !mbar_wait_cluster(TEMPTY_BAR(1), free_par, err, kDevErrTimeoutTmemEmpty)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait_cluster(FULL_BAR(stage), phase, err, kDevErrTimeoutFull) ||
               !mbar_wait_cluster(BRDY_BAR(bs), bphase, err, kDevErrTimeoutFull)) {
@@ -272,8 +282,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
           const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
 #pragma unroll
           for (int kk = 0; kk < kBK / kUmmaK; ++kk)
-            tc_mma_f16_pair(d_tmem, make_sw128_desc(sa + kk * 2048u, 8192u, 1024u),
+            tc_mma_f16_pair(tmem_base, make_sw128_desc(sa + kk * 2048u, 8192u, 1024u),
                             make_sw128_desc(sb + kk * 2048u, 8192u, 1024u), idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+          if (subs == 2) {
+#pragma unroll
+            for (int kk = 0; kk < kBK / kUmmaK; ++kk)
+              tc_mma_f16_pair(tmem_base + 256u, make_sw128_desc(sa + L::kSubBytes + kk * 2048u, 8192u, 1024u),
+                              make_sw128_desc(sb + kk * 2048u, 8192u, 1024u), idesc,
+                              (kb > kb0 || kk > 0) ? 1u : 0u);
+          }
           tc_commit_pair(EMPTY_BAR(stage));
           tc_commit_pair(mapa_shared(EMPTY_BAR(stage), 1));
           tc_commit_pair(BEMP_BAR(bs));
@@ -288,23 +305,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
           }
         }
         if (!ok) break;
-        tc_commit_pair(TFULL_BAR(acc));
-        tc_commit_pair(mapa_shared(TFULL_BAR(acc), 1));
+        tc_commit_pair(TFULL_BAR);
+        tc_commit_pair(mapa_shared(TFULL_BAR, 1));
       }
     }
   } else if (warp < kWgConvWarp0) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int quad = warp & 3;
-    const uint32_t buf = base + L::kBoxOffset + static_cast<uint32_t>(quad) * 4096u;
+    const int half = (warp - kEpiWarp0) >> 2;
+    const uint32_t buf = base + L::kBoxOffset + static_cast<uint32_t>(warp - kEpiWarp0) * 2048u;
     int it = 0;
     for (int w = w_first; w < total; w += w_step, ++it) {
       int m_pair, n_tile, split;
       decode_work(w, p, m_pair, n_tile, split);
-      const int acc = it & 1;
-      if (!warp_wait(TFULL_BAR(acc), static_cast<uint32_t>(it >> 1) & 1u, err, kDevErrTimeoutTmemFull, lane)) break;
+      if (!warp_wait(TFULL_BAR, static_cast<uint32_t>(it) & 1u, err, kDevErrTimeoutTmemFull, lane)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * 256);
-      const int row0 = (2 * m_pair + static_cast<int>(rank)) * kBM + quad * 32;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 256);
+      const int row0 = m_pair * kWgBM + half * 256 + static_cast<int>(rank) * kBM + quad * 32;
       if (partial != nullptr)
         wg_store_tile<float>(partial + static_cast<int64_t>(split) * p.M * p.N, p.N, row0, p.M, n_tile * 256, p.N,
                              taddr, buf, lane);
@@ -312,36 +329,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
         wg_store_tile<T>(grad_w, p.N, row0, p.M, n_tile * 256, p.N, taddr, buf, lane);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(TEMPTY_BAR(acc), 0));
+      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(TEMPTY_BAR(half), 0));
     }
   } else {
     // ------------------------------------------------------------ converters (both CTAs)
-    // A group's two warps make one block's tile (groups and not all warps on one block: the
-    // waits, the proxy fence and the arrive of a block are latency, which four groups
-    // overlap).  Warp b of a group makes box b (64 features): in each of eight steps its
-    // lanes take eight tokens x four 16-byte pieces of codes, and a piece becomes two
-    // 16-byte chunks of the read-back box.  The eight lanes that access shared memory
-    // together hold tokens m and m ^ 5: under the 128-byte swizzle both their reads
-    // (bit 2 differs) and their writes (bit 0 differs) fall on eight different chunks.
+    // A group's four warps make one block's tile (two groups: the waits, the proxy fence and
+    // the arrive of a block are latency, which they overlap).  A warp makes 32 tokens of one
+    // box (64 features): in each of four steps its lanes take eight tokens x four 16-byte
+    // pieces of codes, and a piece becomes two 16-byte chunks of the read-back box.  The
+    // eight lanes that access shared memory together hold tokens m and m ^ 5: under the
+    // 128-byte swizzle both their reads (bit 2 differs) and their writes (bit 0 differs)
+    // fall on eight different chunks.
     const int group = (warp - kWgConvWarp0) / kWgGroupWarps;
-    const int box = (warp - kWgConvWarp0) % kWgGroupWarps;
+    const int box = (warp - kWgConvWarp0) & 1;
+    const int tok0 = ((warp - kWgConvWarp0) & 2) * 16;  // the warp's first token of a block
     const int piece = lane & 3;
-    const int m7 = (lane >> 3) ^ ((lane & 4) ? 5 : 0);  // token within a step
-    const uint32_t rd = static_cast<uint32_t>(m7 * 128 + (((4 * box + piece) ^ m7) << 4));
-    const uint32_t wr0 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece) ^ m7) << 4));
-    const uint32_t wr1 = static_cast<uint32_t>(box * 8192 + m7 * 128 + (((2 * piece + 1) ^ m7) << 4));
-    float sc[8];     // scales of this lane's tokens in block sc_kb
+    const int m7 = (lane >> 3) ^ ((lane & 4) ? 5 : 0);  // token within a step's eight
+    const uint32_t rd = static_cast<uint32_t>((tok0 + m7) * 128 + (((4 * box + piece) ^ m7) << 4));
+    const uint32_t wr0 = static_cast<uint32_t>(box * 8192 + (tok0 + m7) * 128 + (((2 * piece) ^ m7) << 4));
+    const uint32_t wr1 = static_cast<uint32_t>(box * 8192 + (tok0 + m7) * 128 + (((2 * piece + 1) ^ m7) << 4));
+    float sc[4];     // scales of this lane's tokens in block sc_kb
     int sc_kb = -1;
     auto load_scales = [&](int kb) {
-      const int tok = kb * kBK + m7;
+      const int tok = kb * kBK + tok0 + m7;
       sc_kb = kb;
-      if (tok + 56 < tokens) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = __ldg(scale + tok + 8 * j);
-      } else {  // tokens past the end: their codes and gradients arrive as zeros
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = tok + 8 * j < tokens ? __ldg(scale + tok + 8 * j) : 0.0f;
-      }
+      for (int j = 0; j < 4; ++j)  // tokens past the end: their codes and gradients arrive as zeros
+        sc[j] = tok + 8 * j < tokens ? __ldg(scale + tok + 8 * j) : 0.0f;
     };
     int stage = 0, bs = 0, turn = 0;
     uint32_t phase = 0, bphase = 0;
@@ -360,16 +374,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
           }
           const uint32_t raw = base + L::kRawOffset + stage * L::kRawBytes + rd;
           const uint32_t sb = base + L::kBOffset + bs * L::kBBytes;
-          uint4 v[8];
+          if (!warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
+            ok = false;
+            break;
+          }
+          uint4 v[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = ld_shared_v4(raw + j * 1024u);
+          for (int j = 0; j < 4; ++j) v[j] = ld_shared_v4(raw + j * 1024u);
           __syncwarp();
           if (lane == 0) mbar_arrive(RAWE_BAR(stage));
-          // converted in registers before the wait for the tile's previous reader: what that
-          // wait delays is only the stores
-          uint4 o[8][2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < 4; ++j) {
             const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
             uint32_t h[8];
 #pragma unroll
@@ -379,20 +394,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
               h[2 * k] = pack2_16<T>(f[0] * sc[j], f[1] * sc[j]);
               h[2 * k + 1] = pack2_16<T>(f[2] * sc[j], f[3] * sc[j]);
             }
-            o[j][0] = make_uint4(h[0], h[1], h[2], h[3]);
-            o[j][1] = make_uint4(h[4], h[5], h[6], h[7]);
+            st_shared_v4(sb + wr0 + j * 1024u, make_uint4(h[0], h[1], h[2], h[3]));
+            st_shared_v4(sb + wr1 + j * 1024u, make_uint4(h[4], h[5], h[6], h[7]));
           }
           // the group's next block in this split: its scales, a global load away
           if (kb + kWgGroups < kb1) load_scales(kb + kWgGroups);
-          if (!warp_wait(BEMP_BAR(bs), bphase ^ 1u, err, kDevErrTimeoutEmpty, lane)) {
-            ok = false;
-            break;
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            st_shared_v4(sb + wr0 + j * 1024u, o[j][0]);
-            st_shared_v4(sb + wr1 + j * 1024u, o[j][1]);
-          }
           fence_proxy_async_smem();  // the tensor cores read the tile
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_shared(BRDY_BAR(bs), 0));
@@ -457,10 +463,12 @@ __global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float*
 }
 
 // Splits of the tokens: the number that the cost in microseconds is least for, of
-// rounds of pair tiles at 0.4 us per 64 tokens, and, with partials, a second launch
-// (3 us) and 8 bytes per partial element at 6 TB/s.
+// rounds of pair tiles at 0.8 us per 64 tokens (0.45 with one 256-row MMA) and 6 us for
+// an epilogue, and, with partials, a second launch (3 us) and 8 bytes per partial
+// element at 6 TB/s.
 static int weight_grad_q8_splits(int64_t tokens, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
+  const int64_t tiles = ((N + kWgBM - 1) / kWgBM) * ((K + 255) / 256);
+  const double block_us = N > 256 ? 0.8 : 0.45;
   const int64_t pairs = num_sms_of_current_device() / 2;
   const int64_t kb = (tokens + kBK - 1) / kBK;
   int best = 1;
@@ -468,7 +476,7 @@ static int weight_grad_q8_splits(int64_t tokens, int64_t N, int64_t K) {
   for (int s = 1; s <= 32 && s <= kb; ++s) {
     const int64_t per = (kb + s - 1) / s;
     if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
-    double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (0.4 * static_cast<double>(per) + 2.0);
+    double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (block_us * static_cast<double>(per) + 6.0);
     if (s > 1) us += 3.0 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 6.0e6;
     if (us < best_us) {
       best_us = us;
@@ -486,7 +494,8 @@ static int weight_grad_q8(const void* grad, const void* q, const float* scale, T
   if (!encode_map(&mg, grad, 2, N, tokens, N, kBK) || !encode_map(&mq, q, 1, K, tokens, K, kBK))
     return HLM_ERR_DRIVER;
   GemmParams p;
-  gemm_tiling_pair(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), 256, splits);
+  gemm_tiling(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), 256, splits);
+  p.m_tiles = static_cast<int>((N + kWgBM - 1) / kWgBM);
   p.err = device_error_ptr();
   if (p.err == nullptr) return HLM_ERR_LAUNCH;
   auto kern = weight_grad_q8_kernel<T>;
