@@ -492,7 +492,7 @@ __host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
 }
 
 // Operand kinds of the GEMM kernels.  A K block is one 128-byte swizzle row of
-// either (64 bf16 or 128 int8), read by four MMAs of 32 bytes of K each.
+// either (64 16-bit values or 128 int8), read by four MMAs of 32 bytes of K each.
 struct KindBf16 {
   static constexpr int kBlockK = 64;
   static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
@@ -503,6 +503,11 @@ struct KindBf16 {
   }
   static HLM_DEVICE void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     tc_mma_f16_pair(d, a, b, idesc, acc);
+  }
+};
+struct KindF16 : KindBf16 {  // the same instruction on fp16 operands (A and B format 0)
+  static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
+    return make_idesc_bf16_f32(M, N, a_mn, b_mn) & ~((1u << 7) | (1u << 10));
   }
 };
 struct KindS8 {

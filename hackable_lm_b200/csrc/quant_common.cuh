@@ -70,15 +70,6 @@ HLM_DEVICE void codes_to_float(uint32_t packed, float (&f)[4]) {
   f[3] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7443)) - 8388736.0f;
 }
 
-// The same through a byte dot product: 0x4b400000 (1.5 * 2^23 as a float) plus the
-// signed byte that the one-byte factor selects.  Keeps the work off the integer ALU
-// pipe, where the byte permutes above and the packing of 16-bit results meet.
-HLM_DEVICE void codes_to_float_dp4a(uint32_t packed, float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    f[i] = __int_as_float(__dp4a(static_cast<int>(packed), 1 << (8 * i), 0x4b400000)) - 12582912.0f;
-}
-
 // Largest magnitude among the elements of a 16-byte vector, as fp32 bits.  The
 // 16-bit types compare as packed pairs of 15-bit integers: ordered like the
 // magnitudes, infinities above finite values, NaNs above infinities.
