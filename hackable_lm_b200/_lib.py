@@ -109,6 +109,27 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled binding of the 8-bit operators (csrc/binding.cpp), given the loaded
+    library's entry points."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib = load()
+    try:
+        from . import _hlm_torch
+    except ImportError as e:
+        raise HlmError(f"hackable_lm_b200 binding not usable ({e}); build it with "
+                       "`python -m hackable_lm_b200.build`") from e
+    _hlm_torch.set_entry_points(
+        {name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES}, HlmError)
+    _binding = _hlm_torch
+    return _binding
+
+
 def check(rc: int, what: str) -> None:
     if rc != HLM_OK:
         msg = load().hlm_strerror(rc)

@@ -1,4 +1,5 @@
-"""Build libhlm_b200.so from csrc/ for sm_100a (in-tree, no JIT cache).
+"""Build libhlm_b200.so from csrc/*.cu for sm_100a, and the Python binding
+_hlm_torch.so from csrc/binding.cpp (in-tree, no JIT cache).
 
     python -m hackable_lm_b200.build            # incremental
     python -m hackable_lm_b200.build --force    # rebuild everything
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +25,8 @@ INCLUDE = PKG_DIR.parent / "include"
 BUILD_DIR = PKG_DIR.parent / "_build"
 LIB_NAME = "libhlm_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+BINDING_SRC = CSRC / "binding.cpp"
+BINDING_PATH = PKG_DIR / "_hlm_torch.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -65,8 +69,44 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool) -> tuple[Path, str]
     return obj, proc.stdout + proc.stderr
 
 
+def _build_binding(force: bool) -> None:
+    """Compile and link the binding against the installed torch (its version is noted beside
+    the build, so another torch rebuilds it)."""
+    import torch
+    from torch.utils import cpp_extension
+
+    stamp = BUILD_DIR / "binding.torch"
+    header = INCLUDE / "hlm_b200.h"
+    if (not force and BINDING_PATH.exists() and stamp.exists() and stamp.read_text() == torch.__version__
+            and BINDING_PATH.stat().st_mtime >= max(BINDING_SRC.stat().st_mtime, header.stat().st_mtime)):
+        return
+    cuda_home = Path(_nvcc()).parent.parent
+    includes = [*cpp_extension.include_paths(), str(cuda_home / "include"), sysconfig.get_paths()["include"]]
+    lib_dir = Path(torch.__file__).parent / "lib"
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare", "-DNDEBUG",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(arg for inc in includes for arg in ("-isystem", inc)), str(BINDING_SRC), "-o", str(tmp),
+           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"binding build failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    stamp.write_text(torch.__version__)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every csrc/*.cu for sm_100a and link libhlm_b200.so; return its path."""
+    """Compile every csrc/*.cu for sm_100a and link libhlm_b200.so, and build the Python
+    binding; return the library's path."""
+    with cf.ThreadPoolExecutor(max_workers=1) as pool:
+        BUILD_DIR.mkdir(parents=True, exist_ok=True)
+        binding = pool.submit(_build_binding, force)
+        path = _build_library(force, verbose)
+        binding.result()
+    return path
+
+
+def _build_library(force: bool, verbose: bool) -> Path:
     nvcc = _nvcc()
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     sources = _sources()

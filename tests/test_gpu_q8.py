@@ -21,6 +21,7 @@ import pytest
 import torch
 
 from oracle import quant8
+from test_q8_host import bad_calls
 
 pytestmark = pytest.mark.gpu
 
@@ -618,6 +619,59 @@ def test_gradient_asked_of_an_integer_output_is_refused(cuda_device):
     out, _, _ = kernels.residual_rms_norm_q8(x, x.detach(), 1e-6)
     with pytest.raises(RuntimeError):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("name", sorted(bad_calls("meta")))
+def test_argument_checks(name, cuda_device):
+    from hackable_lm_b200 import _lib
+
+    before = _lib.launch_count()
+    with pytest.raises(RuntimeError):
+        bad_calls(cuda_device)[name]()
+    assert _lib.launch_count() == before
+
+
+def test_unsupported_sizes_raise_the_library_error(cuda_device):
+    """K that is no multiple of 16, or too long; N of the gradient no multiple of 8."""
+    from hackable_lm_b200 import _lib, kernels, ops
+
+    def c(rows, cols):
+        return torch.zeros(rows, cols, dtype=torch.int8, device=cuda_device), torch.ones(rows, device=cuda_device)
+
+    for k in (24, 131072):
+        with pytest.raises(_lib.HlmError, match="unsupported"):
+            kernels.linear_q8(*c(2, k), *c(3, k))
+    g = torch.zeros(5, 12, dtype=torch.bfloat16, device=cuda_device)
+    with pytest.raises(_lib.HlmError, match="unsupported"):
+        ops.weight_grad_q8(g, *c(5, 32))
+    with pytest.raises(_lib.HlmError, match="unsupported"):
+        ops.weight_grad_q8(g[:, :8], *c(5, 24))
+    with pytest.raises(RuntimeError):
+        kernels.linear_ckpt8(g.float().requires_grad_(True), torch.zeros(8, 12, device=cuda_device, requires_grad=True))
+
+
+def test_modes_and_transforms_see_the_operators(cuda_device):
+    """Under a dispatch mode the registered operator runs (and is seen); the result is the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from hackable_lm_b200 import kernels
+
+    seen = []
+
+    class Recorder(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    x = values((5, 64), torch.bfloat16).to(cuda_device)
+    q, scale = kernels.quantize_rows(x)
+    with Recorder():
+        q2, scale2 = kernels.quantize_rows(x)
+    assert any("hackable_lm_b200.quantize_rows" in s for s in seen)
+    assert torch.equal(q, q2) and torch.equal(scale, scale2)
+    neg = torch._neg_view(x)  # a lazily negated view: its storage holds the other sign
+    q3, scale3 = kernels.quantize_rows(neg)
+    assert torch.equal(q3, -q) and torch.equal(scale3, scale)
 
 
 @pytest.mark.parametrize("name", ["quantize_rows", "dequantize_rows", "rms_norm_q8", "residual_rms_norm_q8", "linear_q8",

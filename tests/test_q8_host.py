@@ -58,26 +58,35 @@ def test_cpu_tensors_are_rejected():
             call()
 
 
-def test_argument_checks():
-    x = torch.zeros(4, 32, dtype=torch.bfloat16)
-    q, s = torch.zeros(4, 32, dtype=torch.int8), torch.ones(4)
-    for bad in (lambda: ops._q8._linear_q8(q, s, q[:, :16], s, torch.bfloat16),            # K differs
-                lambda: ops._q8._linear_q8(q, s[:3], q, s, torch.bfloat16),                 # scales of other rows
-                lambda: ops._q8._linear_q8(x, s, q, s, torch.bfloat16),                     # not codes
-                lambda: ops._q8._linear_q8(q, s, q, s, torch.int32),                        # output type
-                lambda: ops._q8._quantize_rows(q),                                          # input type
-                lambda: ops._q8._quantize_rows(torch.zeros(4, 0)),                          # no columns
-                lambda: ops._q8._dequantize_rows(q, s.half(), torch.float32),
-                lambda: ops._q8._residual_rms_norm_q8(x, x[:2], None, 1e-6),
-                lambda: ops._q8._swiglu_ckpt8(torch.zeros(2, 7)),
-                lambda: ops._q8._swiglu_ckpt8_backward(q, torch.ones(4, 4), x[:, :16]),     # scales of another width
-                lambda: ops._q8._weight_grad_q8(x.float(), q, s),
-                lambda: ops._q8._weight_grad_q8(x[:3], q, s)):
-        with pytest.raises(RuntimeError):
-            bad()
-    w = torch.zeros(5, device="meta")
+def bad_calls(device):
+    """Calls whose shapes or types do not fit together."""
+    def t(shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype, device=device)
+
+    x, q, s = t((4, 32)), t((4, 32), torch.int8), t(4, torch.float32)
+    return {
+        "other K": lambda: ops.linear_q8(q, s, q[:, :16], s), "weight of one dimension": lambda: ops.linear_q8(q, s, q[0], s[0]),
+        "scales of other rows": lambda: ops.linear_q8(q, s[:3], q, s), "not codes": lambda: ops.linear_q8(x, s, q, s),
+        "weight scales of other rows": lambda: ops.linear_q8(q, s, q, s[:2]),
+        "output type": lambda: ops.linear_q8(q, s, q, s, torch.int32), "scales in 16 bits": lambda: ops.linear_q8(q, s.half(), q, s),
+        "codes again": lambda: ops.quantize_rows(q), "no columns": lambda: ops.quantize_rows(t((4, 0))),
+        "a number": lambda: ops.quantize_rows(t(())), "read back type": lambda: ops.dequantize_rows(q, s, torch.float64),
+        "read back scales": lambda: ops.dequantize_rows(q, s.half(), torch.float32),
+        "norm rows": lambda: ops.residual_rms_norm_q8(x, x[:2], None, 1e-6),
+        "norm types": lambda: ops.residual_rms_norm_q8(x, x.float(), None, 1e-6),
+        "norm weight": lambda: ops.rms_norm_q8(x, t(5), 1e-6), "norm of doubles": lambda: ops.rms_norm_q8(x.double(), None, 1e-6),
+        "odd width": lambda: ops.swiglu_ckpt8(t((2, 7))), "gate_up type": lambda: ops.swiglu_ckpt8(q),
+        "scales of another width": lambda: ops.swiglu_ckpt8_backward(q, t((4, 4), torch.float32), x[:, :16]),
+        "gradient of another width": lambda: ops.swiglu_ckpt8_backward(q, t((4, 2), torch.float32), x),
+        "gradient in 32 bits": lambda: ops.weight_grad_q8(x.float(), q, s),
+        "gradient of other rows": lambda: ops.weight_grad_q8(x[:3], q, s),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(bad_calls("meta")))
+def test_argument_checks_on_meta_tensors(name):
     with pytest.raises(RuntimeError):
-        ops._q8._norm_weight("rms_norm_q8", torch.zeros(4, 32, device="meta"), w)
+        bad_calls("meta")[name]()
 
 
 def test_shapes_on_meta_tensors():
