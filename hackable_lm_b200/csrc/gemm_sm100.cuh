@@ -64,6 +64,14 @@ template <class E>
 struct epi_relaxed_release<E, std::void_t<decltype(E::kRelaxedRelease)>>
     : std::integral_constant<bool, E::kRelaxedRelease> {};
 
+// Epilogues that read per-row or per-column values from global memory declare a struct
+// `Early` and `load_early`: the pair kernel calls it before it waits for the tile's
+// accumulator, and hands the struct to `run`.
+template <class E, class = void>
+struct epi_early : std::false_type {};
+template <class E>
+struct epi_early<E, std::void_t<typename E::Early>> : std::true_type {};
+
 constexpr int kBM = 128;
 constexpr int kBK = 64;  // 64 bf16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
@@ -566,13 +574,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
       decode_work(w, p, m_pair, n_tile, split);
       const int acc = L::kAccs == 2 ? (it & 1) : 0;
       const uint32_t acc_par = static_cast<uint32_t>(L::kAccs == 2 ? ((it >> 1) & 1) : (it & 1));
-      if (!warp_wait(TFULL_BAR(acc), acc_par, err, kDevErrTimeoutTmemFull, lane)) break;
-      tc_fence_after();
       const uint32_t taddr =
           tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      Epi::template run<BN, kParts>(ep, p, base_ptr + L::kEpiOffset, taddr,
-                                    2 * m_pair + static_cast<int>(rank), n_tile, split, quad, part,
-                                    lane);
+      const int m_tile = 2 * m_pair + static_cast<int>(rank);
+      if constexpr (epi_early<Epi>::value) {
+        typename Epi::Early early;
+        Epi::template load_early<BN, kParts>(ep, p, early, m_tile, n_tile, quad, part, lane);
+        if (!warp_wait(TFULL_BAR(acc), acc_par, err, kDevErrTimeoutTmemFull, lane)) break;
+        tc_fence_after();
+        Epi::template run<BN, kParts>(ep, p, base_ptr + L::kEpiOffset, taddr, m_tile, n_tile, split, quad, part,
+                                      lane, early);
+      } else {
+        if (!warp_wait(TFULL_BAR(acc), acc_par, err, kDevErrTimeoutTmemFull, lane)) break;
+        tc_fence_after();
+        Epi::template run<BN, kParts>(ep, p, base_ptr + L::kEpiOffset, taddr, m_tile, n_tile, split, quad, part,
+                                      lane);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {

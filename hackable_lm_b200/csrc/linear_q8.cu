@@ -113,6 +113,14 @@ struct SplitSmem {
 HLM_DEVICE void st_shared_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+HLM_DEVICE int ld_shared_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// The two halves of a cluster barrier that hands over no memory.
+HLM_DEVICE void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+HLM_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 HLM_DEVICE uint32_t cluster_nctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -164,10 +172,22 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncwarp();
-  cluster_sync_all();  // barriers are set up, and every CTA of the cluster runs (its memory may be written)
+  __syncthreads();
   tc_fence_after();
+  cluster_arrive_relaxed();  // this CTA runs: its memory may be written from now on
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  // What the last step needs from global memory, fetched now.  A warp then takes the owned
+  // columns warp, warp + 6, ...: lane l keeps the token scale of the l-th of them (at most
+  // 128 / 6 = 22), and every lane the scales of its four channels: consecutive ones where
+  // four outputs are one store (vec), else 32 apart (coalesced single stores).
+  constexpr int kWarps = kSplitThreads / 32;
+  const int my_col = rank + (warp + kWarps * lane) * splits;
+  const float my_scale = my_col < tokens ? scale[m0 + my_col] : 0.0f;
+  const int ch0 = vec ? 4 * lane : lane, ch_step = vec ? 1 : 32;
+  float cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = n0 + ch0 + i * ch_step < N ? w_scale[n0 + ch0 + i * ch_step] : 0.0f;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -218,7 +238,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   } else {
     const int quad = warp & 3;
-    if (warp_wait(done_bar, 0, err, kDevErrTimeoutTmemFull, lane)) {
+    const bool ok = warp_wait(done_bar, 0, err, kDevErrTimeoutTmemFull, lane);
+    cluster_wait();  // the owners run
+    if (ok) {
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
       // slot of column c: CTA c % splits, row rank * per + c / splits
@@ -243,40 +265,49 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   }
   __syncwarp();
-  cluster_sync_all();  // every partial of this CTA's columns has arrived
-  {
-    // a warp per owned column, four channels per lane
-    const int n = n0 + 4 * lane;
-    float cs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cs[i] = n + i < N ? w_scale[n + i] : 0.0f;
-    for (int i = warp; rank + i * splits < tokens; i += kSplitThreads / 32) {
-      const int m = m0 + rank + i * splits;
-      int4 sum = make_int4(0, 0, 0, 0);
-      uint32_t addr = base + L::kPartOffset + static_cast<uint32_t>(i * 512 + lane * 16);
-      for (int s = 0; s < splits; ++s, addr += static_cast<uint32_t>(per) * 512u) {
-        const uint4 v = ld_shared_v4(addr);
-        sum.x += static_cast<int>(v.x);
-        sum.y += static_cast<int>(v.y);
-        sum.z += static_cast<int>(v.z);
-        sum.w += static_cast<int>(v.w);
+  if (warp < 2) cluster_wait();  // pairs with the first arrive, like the epilogue warps' above
+  cluster_sync_all();            // every partial of this CTA's columns has arrived
+#pragma unroll 2
+  for (int j = 0; j < (128 + kWarps - 1) / kWarps; ++j) {
+    const int i = warp + kWarps * j;
+    if (rank + i * splits >= tokens) break;
+    const int m = m0 + rank + i * splits;
+    const float rs = __shfl_sync(0xffffffffu, my_scale, j);
+    const uint32_t col = base + L::kPartOffset + static_cast<uint32_t>(i * 512);
+    int sum[4] = {0, 0, 0, 0};
+    if (vec) {
+      for (int s = 0; s < splits; ++s) {
+        const uint4 v = ld_shared_v4(col + static_cast<uint32_t>(s * per * 512 + lane * 16));
+        sum[0] += static_cast<int>(v.x);
+        sum[1] += static_cast<int>(v.y);
+        sum[2] += static_cast<int>(v.z);
+        sum[3] += static_cast<int>(v.w);
       }
-      const float rs = scale[m];
-      alignas(16) const T y[4] = {scaled<T>(sum.x, rs, cs[0]), scaled<T>(sum.y, rs, cs[1]), scaled<T>(sum.z, rs, cs[2]),
-                      scaled<T>(sum.w, rs, cs[3])};
-      T* dst = out + static_cast<int64_t>(m) * N + n;
-      if (vec && n + 4 <= N) {
-        if constexpr (sizeof(T) == 4)
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
-        else
-          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
-      } else {
+    } else {
+      for (int s = 0; s < splits; ++s) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (n + k < N) dst[k] = y[k];
+          sum[k] += ld_shared_s32(col + static_cast<uint32_t>(s * per * 512 + (lane + 32 * k) * 4));
       }
     }
+    alignas(16) T y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = scaled<T>(sum[k], rs, cs[k]);
+    T* dst = out + static_cast<int64_t>(m) * N + n0;
+    if (vec) {
+      if (n0 + ch0 < N) {  // N % 4 == 0: all four or none
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<uint4*>(dst + ch0) = *reinterpret_cast<const uint4*>(y);
+        else
+          *reinterpret_cast<uint2*>(dst + ch0) = *reinterpret_cast<const uint2*>(y);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n0 + lane + 32 * k < N) dst[lane + 32 * k] = y[k];
+    }
   }
+  __syncwarp();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
@@ -311,26 +342,46 @@ struct EpiScaleQ8 {
     return EPI_WARPS * kWarpBytes;
   }
 
+  // This lane's row scale and its column scales of every group the warp takes, loaded
+  // before the wait for the accumulator.
+  struct Early {
+    float rs;
+    float cs[4][2];
+  };
+  template <int BN, int kParts>
+  static HLM_DEVICE void load_early(const Params& ep, const GemmParams& p, Early& e, int m_tile, int n_tile,
+                                    int quad, int part, int lane) {
+    const int row = m_tile * kBM + quad * 32 + lane;
+    e.rs = row < p.M ? ep.row_scale[row] : 0.0f;
+    static_assert(BN / kCols <= 4 * kParts, "groups of a warp");
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const int g = part + k * kParts;
+        const int col = n_tile * BN + g * kCols + 32 * i + lane;
+        e.cs[k][i] = g < BN / kCols && col < p.N ? ep.col_scale[col] : 0.0f;
+      }
+  }
+
   template <int BN, int kParts>
   static HLM_DEVICE void run(const Params& ep, const GemmParams& p, uint8_t* smem, uint32_t taddr,
-                             int m_tile, int n_tile, int, int quad, int part, int lane) {
+                             int m_tile, int n_tile, int, int quad, int part, int lane, const Early& e) {
     uint8_t* box = smem + (part * 4 + quad) * kWarpBytes;
     const uint32_t buf = smem_u32(box);
     float* cs_ptr = reinterpret_cast<float*>(box + kBoxBytes);
     const uint32_t cs_addr = buf + kBoxBytes;
     const int row0 = m_tile * kBM + quad * 32;
-    const int row = row0 + lane;
-    const float rs = row < p.M ? ep.row_scale[row] : 0.0f;
-#pragma unroll 1
-    for (int g = part; g < BN / kCols; g += kParts) {
+    const float rs = e.rs;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int g = part + k * kParts;
+      if (g >= BN / kCols) break;
       const int col0 = n_tile * BN + g * kCols;
       if (col0 >= p.N) break;  // the same for the whole warp
       __syncwarp();            // the box's last group has been read
 #pragma unroll
-      for (int i = 0; i < kCols / 32; ++i) {
-        const int col = col0 + 32 * i + lane;
-        cs_ptr[32 * i + lane] = col < p.N ? ep.col_scale[col] : 0.0f;
-      }
+      for (int i = 0; i < kCols / 32; ++i) cs_ptr[32 * i + lane] = e.cs[k][i];
       __syncwarp();
 #pragma unroll
       for (int hs = 0; hs < kCols / 32; ++hs) {
