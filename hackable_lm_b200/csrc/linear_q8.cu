@@ -6,8 +6,8 @@
 // the same bits), the two scales applied in fp32, one rounding to the output type.
 // Three kernels, by M and the number of output tiles:
 //
-//  - rows kernel, M <= 8: one pass over the weights with dp4a; bound by
-//    reading w (and by launch latency at small sizes).
+//  - rows kernel, one token, or up to 8 and few weights: one pass over the weights with
+//    dp4a; bound by reading w (and by launch latency at small sizes).
 //  - split kernel, fewer 128 x 128 output tiles than SMs: weights as the
 //    128-row MMA operand, tokens as the 16..128-column one, K split over a
 //    thread-block cluster whose CTAs add their int32 partial tiles through
@@ -36,22 +36,26 @@ HLM_DEVICE T scaled(int acc, float row_scale, float col_scale) {
 }
 
 // ---------------------------------------------------------------------------
-// M <= 8: a warp per R output channels, lanes along K.
+// M <= 8: R output channels per KS warps, lanes (and the KS warps) along K.
 // ---------------------------------------------------------------------------
-template <typename T, int MR, int R>
-__global__ void __launch_bounds__(128) linear_q8_rows_kernel(
+constexpr int kRowsWarps = 4;  // warps of a block
+
+template <typename T, int MR, int R, int KS>
+__global__ void __launch_bounds__(32 * kRowsWarps) linear_q8_rows_kernel(
     const int8_t* __restrict__ q, const float* __restrict__ scale, const int8_t* __restrict__ w,
     const float* __restrict__ w_scale, T* __restrict__ out, int M, int N, int K) {
+  static_assert(KS == 1 || KS == kRowsWarps, "a warp's own channels, or a block's");
   const int lane = threadIdx.x & 31;
-  const int64_t n0 = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * R;
-  if (n0 >= N) return;
+  const int warp = threadIdx.x >> 5;
+  const int64_t n0 = (KS == 1 ? static_cast<int64_t>(blockIdx.x) * kRowsWarps + warp : blockIdx.x) * R;
+  if (n0 >= N) return;  // KS > 1: the same for the whole block
   int acc[R][MR];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int m = 0; m < MR; ++m) acc[r][m] = 0;
-#pragma unroll 2
-  for (int k = lane * 16; k < K; k += 512) {
+#pragma unroll 4
+  for (int k = ((KS == 1 ? 0 : warp) * 32 + lane) * 16; k < K; k += 512 * KS) {
     uint4 wv[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -71,20 +75,32 @@ __global__ void __launch_bounds__(128) linear_q8_rows_kernel(
       }
     }
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int m = 0; m < MR; ++m) acc[r][m] = __reduce_add_sync(0xffffffffu, acc[r][m]);
   // lane r * MR + m writes output (m, n0 + r)
+  const int r_out = lane / MR, m_out = lane - r_out * MR;
+  const bool writes = r_out < R && m_out < M && n0 + r_out < N && (KS == 1 || warp == 0);
+  float rs = 0.0f, cs = 0.0f;
+  if (writes) {  // on their way while the lanes' sums are added
+    rs = scale[m_out];
+    cs = w_scale[n0 + r_out];
+  }
   int mine = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int m = 0; m < MR; ++m)
-      if (lane == r * MR + m) mine = acc[r][m];
-  const int r = lane / MR, m = lane - r * MR;
-  if (r < R && m < M && n0 + r < N)
-    out[static_cast<int64_t>(m) * N + n0 + r] = scaled<T>(mine, scale[m], w_scale[n0 + r]);
+    for (int m = 0; m < MR; ++m) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
+      if (lane == r * MR + m) mine = sum;
+    }
+  if constexpr (KS > 1) {
+    __shared__ int part[kRowsWarps][32];
+    part[warp][lane] = mine;
+    __syncthreads();
+    if (warp != 0) return;
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < kRowsWarps; ++i) mine += part[i][lane];
+  }
+  if (writes) out[static_cast<int64_t>(m_out) * N + n0 + r_out] = scaled<T>(mine, rs, cs);
 }
 
 // ---------------------------------------------------------------------------
@@ -500,25 +516,40 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   return launch_status();
 }
 
+// A block's warps share a pair of channels where rows are long and the warps of single
+// pairs few or their tokens one: [1, 4096, 4096] 5.1 us against 6.7 with a warp a pair,
+// [8, 768, 2048] 2.4 against 3.3; but [1, 4096, 1024] 2.8 against 2.6, and
+// [8, 4096, 2048], where the adding of 16 sums weighs, 6.7 against 4.8.
 template <typename T, int MR>
 static int linear_q8_rows(const void* q, const float* scale, const void* w, const float* w_scale, T* out,
                           int64_t M, int64_t N, int64_t K, cudaStream_t s) {
   constexpr int R = 2;
-  constexpr int kWarps = 4;
-  const int64_t blocks = (N + R * kWarps - 1) / (R * kWarps);
+  const int8_t* qp = static_cast<const int8_t*>(q);
+  const int8_t* wp = static_cast<const int8_t*>(w);
   LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
-  linear_q8_rows_kernel<T, MR, R><<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(
-      static_cast<const int8_t*>(q), scale, static_cast<const int8_t*>(w), w_scale, out, static_cast<int>(M),
-      static_cast<int>(N), static_cast<int>(K));
+  if (K >= 2048 && (M == 1 || N <= 2048)) {
+    const int64_t blocks = (N + R - 1) / R;
+    linear_q8_rows_kernel<T, MR, R, kRowsWarps><<<static_cast<unsigned>(blocks), 32 * kRowsWarps, 0, s>>>(
+        qp, scale, wp, w_scale, out, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+  } else {
+    const int64_t blocks = (N + R * kRowsWarps - 1) / (R * kRowsWarps);
+    linear_q8_rows_kernel<T, MR, R, 1><<<static_cast<unsigned>(blocks), 32 * kRowsWarps, 0, s>>>(
+        qp, scale, wp, w_scale, out, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+  }
   return launch_status();
 }
 
 template <typename T>
 static int linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, T* out, int64_t M,
                      int64_t N, int64_t K, cudaStream_t s) {
+  // dp4a for a few tokens of small weights: with M tokens it needs M instructions for four
+  // weights, and falls behind the tensor cores from about 8 M weights on ([8, 4096, 2048]
+  // 4.8 us against 5.6, [8, 4096, 4096] 7.8 against 7.0, [8, 8192, 8192] 25 against 15)
   if (M == 1) return linear_q8_rows<T, 1>(q, scale, w, w_scale, out, M, N, K, s);
-  if (M <= 4) return linear_q8_rows<T, 4>(q, scale, w, w_scale, out, M, N, K, s);
-  if (M <= 8) return linear_q8_rows<T, 8>(q, scale, w, w_scale, out, M, N, K, s);
+  if (M <= 8 && N * K <= (1ll << 23)) {
+    if (M <= 4) return linear_q8_rows<T, 4>(q, scale, w, w_scale, out, M, N, K, s);
+    return linear_q8_rows<T, 8>(q, scale, w, w_scale, out, M, N, K, s);
+  }
   int* err = device_error_ptr();
   if (err == nullptr) return HLM_ERR_LAUNCH;
   const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);

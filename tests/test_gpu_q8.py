@@ -224,7 +224,8 @@ LINEAR_SHAPES = [  # M, N, K
     (1, 1, 16), (1, 4096, 768), (2, 33, 48), (3, 1000, 2048), (4, 768, 16), (5, 129, 8192), (7, 2304, 768), (8, 16, 112),
     (9, 31, 1360), (16, 130, 768), (17, 128, 128), (31, 257, 400), (33, 768, 2048), (64, 512, 64), (65, 100, 4096),
     (127, 96, 144), (128, 128, 128), (129, 1111, 272), (200, 4096, 768), (255, 40, 16), (256, 256, 256), (257, 513, 1040),
-    (777, 1111, 1360), (1000, 24, 528), (1500, 2304, 768)]
+    (777, 1111, 1360), (1000, 24, 528), (1500, 2304, 768), (1, 33, 2064), (1, 5000, 4112), (2, 2049, 4112), (4, 77, 2048),
+    (6, 4096, 4096), (3, 8200, 1040), (1, 2, 131056)]
 
 
 @pytest.mark.parametrize("out_dtype", DTYPES)
