@@ -377,7 +377,8 @@ def bench_d12(args, d: Dist, device) -> dict:
 
     peaks, peak_src = load_peaks()
     window = int(args.attention_window or 0)
-    s = tr.build(device, world=d.world, attention_window=window or None)
+    keep = args.activation_checkpoint
+    s = tr.build(device, world=d.world, attention_window=window or None, activation_checkpoint=keep)
     # fresh data: one distinct micro-batch for every micro-step of the run (warm-up, timed
     # steps and the end-to-end pass), cycling only beyond 1024 micro-batches (268 MB)
     n_micro = min(1024, s.accum * (args.warmup + 2 * args.steps + 1))
@@ -401,7 +402,9 @@ def bench_d12(args, d: Dist, device) -> dict:
     torch.cuda.synchronize()
     # per-kernel timing of the library's own launches during the first timed step
     # capacity: up to two launches per operator call (LM dlogits / grad_hidden run in row halves)
-    timers = {k: _lib.KernelTimer(k, 2 * n * s.accum) for k, n in D12_KERNELS.items()}
+    # (the fused MLP kernels do not run with 8-bit checkpoints, and proj_norm then runs for o_proj alone)
+    timers = {k: _lib.KernelTimer(k, 2 * n * s.accum) for k, n in D12_KERNELS.items()
+              if keep == "none" or k != "proj_norm"}
     clocks = ClockSampler(device.index)
     clocks.start()
     d.barrier()
@@ -540,7 +543,9 @@ def bench_d12(args, d: Dist, device) -> dict:
         "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(ms_per_step, 3),
         "higher_is_better": True, "scaling": "strong", "vs_baseline": None, "dtype": "bf16",
         "data": "synthetic: uniform token ids (seeded per rank), targets = ids shifted by one",
-        "config": d12_config(d.world, s.accum, args.max_grad_norm, window), "roofline": roofline,
+        "config": d12_config(d.world, s.accum, args.max_grad_norm, window)
+        | ({} if keep == "none" else {"activation_checkpoint": keep}), "roofline": roofline,
+        "peak_memory_gb": round(torch.cuda.max_memory_allocated() / 1e9, 2),
         "kernel_breakdown": breakdown,
         "mfu": round(mfu, 4), "mfu_basis": f"{flops_per_token} FLOP/token / measured bf16 burst peak",
         "loss_first_step": first_loss, "loss": float(loss.float().item()),
@@ -650,6 +655,33 @@ def bench_ops(device, iters: int = 20, only: str | None = None) -> dict:
     hbm("rmsnorm_bwd [32768,768]", lambda a, b, c: ops.rms_norm_backward(a, None, b, c, 1e-6), (x, r, gn),
         201_326_592)
     del x, r, gn
+    # 8-bit operators at the d12 shapes (bytes: inputs and outputs once, codes and scales among them)
+    if any(want(n) for n in ("quantize_rows", "residual_rms_norm_q8", "swiglu_ckpt8", "linear_q8", "weight_grad_q8")):
+        xh = torch.randn(32768, 2048, generator=g).to(torch.bfloat16).to(device)
+        hbm("quantize_rows [32768,2048]", lambda a: ops.quantize_rows(a), (xh,), 32768 * (2048 * 3 + 4))
+        q8, s8 = ops.quantize_rows(xh)
+        hbm("dequantize_rows [32768,2048]", lambda a, b: ops.dequantize_rows(a, b), (q8, s8), 32768 * (2048 * 3 + 4))
+        del xh, q8, s8
+        xc = torch.randn(32768, 768, generator=g).to(torch.bfloat16).to(device)
+        rc = torch.randn(32768, 768, generator=g).to(torch.bfloat16).to(device)
+        hbm("residual_rms_norm_q8 [32768,768]", lambda a, b: ops.residual_rms_norm_q8(a, b, None, 1e-6), (rc, xc),
+            32768 * (768 * 7 + 4))
+        q8, s8 = ops.quantize_rows(xc)
+        wq8, ws8 = ops.quantize_rows(torch.randn(4096, 768, generator=g).to(device))
+        tensor("linear_q8 X[32768,768] W[4096,768]", lambda a, b: ops.linear_q8(a, b, wq8, ws8), (q8, s8),
+               2 * 32768 * 768 * 4096)
+        tensor("linear_q8 X[1,768] W[4096,768]", lambda a, b: ops.linear_q8(q8[:1], s8[:1], a, b), (wq8, ws8),
+               2 * 768 * 4096)
+        del xc, rc
+        gu = torch.randn(32768, 4096, generator=g).to(torch.bfloat16).to(device)
+        gh = torch.randn(32768, 2048, generator=g).to(torch.bfloat16).to(device)
+        hbm("swiglu_ckpt8 fwd [32768,4096]", lambda a: ops.swiglu_ckpt8(a), (gu,), 32768 * (2048 * 8 + 128))
+        _, qg8, sg8 = ops.swiglu_ckpt8(gu)
+        hbm("swiglu_ckpt8 bwd [32768,4096]", lambda a, b, c: ops.swiglu_ckpt8_backward(a, b, c), (qg8, sg8, gh),
+            32768 * (2048 * 8 + 128))
+        tensor("weight_grad_q8 dY[32768,4096] X[32768,768]", lambda a, b, c: ops.weight_grad_q8(a, b, c), (gu, q8, s8),
+               2 * 32768 * 768 * 4096)
+        del gu, gh, qg8, sg8, q8, s8, wq8, ws8
     B, T, H, D = 8, 2048, 6, 128
     q = torch.randn(B, T, H, D, generator=g).to(torch.bfloat16).to(device)
     k = torch.randn(B, T, H, D, generator=g).to(torch.bfloat16).to(device)
@@ -832,6 +864,8 @@ def main() -> None:
     ap.add_argument("--attention-window", type=int, default=0,
                     help="d12 variant: sliding window on every layer but each 4th and the last "
                          "(the reference's default pattern); 0 (default, BASELINE config 5) = full causal")
+    ap.add_argument("--activation-checkpoint", choices=("none", "int8"), default="none",
+                    help="d12 variant: what the MLP keeps for its backward pass in 8 bits (default: bf16)")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--ref-tokens", type=int, default=1024, help="tokens per reference-arm step")
     ap.add_argument("--tokens", type=int, default=None,

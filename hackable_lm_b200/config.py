@@ -21,6 +21,10 @@ MODULE_BACKENDS = {"torch", "triton", "b200"}
 # and run on SDPA (sliding-window layers on the tcgen05 kernels), so reference
 # configs and their default "flash_attn_2" select it unchanged.
 ATTENTION_BACKENDS = {"torch", "sdpa", "b200", "flex_attention", "flash_attn_2", "flash_attn_3", "flash_attn_4"}
+# What the MLP keeps of its activations for the backward pass: "none" keeps them whole
+# (bf16), "int8" keeps the projections' inputs and gate_up in 8 bits with scales
+# (kernels.linear_ckpt8, kernels.swiglu_ckpt8).  No counterpart in the reference.
+ACTIVATION_CHECKPOINTS = {"none", "int8"}
 MODULE_BACKEND_FIELDS = (
     "qkv_backend",
     "output_backend",
@@ -56,6 +60,12 @@ def normalize_attention_backend(backend: str) -> str:
     if not isinstance(backend, str) or backend.lower() not in ATTENTION_BACKENDS:
         raise ValueError(f"unknown attention_backend {backend!r}")
     return backend.lower()
+
+
+def normalize_activation_checkpoint(name: str) -> str:
+    if not isinstance(name, str) or name.lower() not in ACTIVATION_CHECKPOINTS:
+        raise ValueError(f"unknown activation_checkpoint {name!r}")
+    return name.lower()
 
 
 def depth_dimensions(depth: int, head_dim: int = DEFAULTS["head_dim"],
@@ -123,6 +133,7 @@ class ModelConfig:
     down_backend: str = "b200"
     lm_head_backend: str = "b200"
     extra: dict[str, Any] = field(default_factory=dict)
+    activation_checkpoint: str = "none"
 
     def to_dict(self) -> dict[str, Any]:
         return asdict(self)
@@ -130,7 +141,8 @@ class ModelConfig:
 
 def model_config_for_depth(depth: int, *, vocab_size: int = 32768, sequence_len: int = 2048,
                            attention_window: int | None = None, backend: str = "b200",
-                           attention_backend: str = "sdpa", **overrides: Any) -> ModelConfig:
+                           attention_backend: str = "sdpa", activation_checkpoint: str = "none",
+                           **overrides: Any) -> ModelConfig:
     """ModelConfig as resolve_config builds it (config.py:433-446)."""
     n_embd, n_head = depth_dimensions(depth)
     backends = {name: normalize_module_backend(name, overrides.pop(name, backend))
@@ -145,6 +157,7 @@ def model_config_for_depth(depth: int, *, vocab_size: int = 32768, sequence_len:
         mlp_hidden=mlp_hidden_dim(n_embd),
         attention_window=attention_window,
         attention_backend=normalize_attention_backend(attention_backend),
+        activation_checkpoint=normalize_activation_checkpoint(activation_checkpoint),
         **backends,
         **overrides,
     )

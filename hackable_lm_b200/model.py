@@ -15,6 +15,8 @@ CPU), ``"b200"`` the hand-written sm_100a kernels:
 * DownProjection.fwd_b200    -> down GEMM with the residual add + RMSNorm in its epilogue
 * MLP (both of the above on b200) -> gate_up_swiglu + swiglu_down_residual_norm:
   the down GEMM's backward computes grad_h and the SwiGLU backward in one kernel
+* MLP with activation_checkpoint "int8" -> linear_ckpt8 + swiglu_ckpt8 + linear_ckpt8:
+  the activations kept for the backward are held in 8 bits
 * LMHeadProjection.fwd_b200  -> fused LM head + cross-entropy
 * input norm                 -> RMSNorm kernel
 
@@ -29,7 +31,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import kernels, ops
-from .config import ModelConfig, layer_attention_window
+from .config import ModelConfig, layer_attention_window, normalize_activation_checkpoint
 
 
 def rms_norm_torch(x: torch.Tensor, weight: torch.Tensor | None, eps: float) -> torch.Tensor:
@@ -246,8 +248,16 @@ class MLP(nn.Module):
         super().__init__()
         self.gate_up = GateUpProjection(config)
         self.down = DownProjection(config)
+        self.keep_int8 = normalize_activation_checkpoint(config.activation_checkpoint) == "int8"
+        if self.keep_int8 and not (self.gate_up.selected_backend() == self.down.selected_backend() == "b200"):
+            raise RuntimeError("activation_checkpoint 'int8' needs the b200 gate_up and down backends")
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor):
+        if self.keep_int8 and torch.is_grad_enabled():
+            # what the backward needs (x, gate_up, h) is kept in 8 bits with scales, half its bytes
+            h = kernels.swiglu_ckpt8(kernels.linear_ckpt8(x, self.gate_up.gate_up_proj.weight))
+            y = kernels.linear_ckpt8(h, self.down.down_proj.weight)
+            return kernels.residual_rms_norm(residual, y, self.down.norm_eps)
         if self.gate_up.selected_backend() == "b200" and self.down.selected_backend() == "b200":
             w_gu = self.gate_up.gate_up_proj.weight
             w_dn = self.down.down_proj.weight
@@ -332,6 +342,13 @@ class LanguageModel(nn.Module):
         for block in self.blocks:
             x, x_norm = block(x, x_norm)
         return self.lm_head(x_norm, targets)
+
+    def quantize_int8(self):
+        """This model with its projections in 8-bit integers, for inference and evaluation
+        (quantized.QuantizedLanguageModel)."""
+        from .quantized import QuantizedLanguageModel
+
+        return QuantizedLanguageModel(self)
 
     def parameter_count(self) -> int:
         return sum(p.numel() for p in self.parameters())

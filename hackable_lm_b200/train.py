@@ -51,11 +51,13 @@ def lr_settings(depth: int) -> dict:
 def build(device: torch.device, *, depth: int = D12["depth"], vocab: int = D12["vocab"],
           seq_len: int = D12["seq_len"], micro_batch: int = D12["micro_batch"],
           global_tokens: int = D12["global_tokens"], world: int = 1, backend: str = "b200",
-          attention_window: int | None = None, seed: int = 0, ddp: bool | None = None) -> StepSetup:
+          attention_window: int | None = None, seed: int = 0, ddp: bool | None = None,
+          activation_checkpoint: str = "none") -> StepSetup:
     torch.manual_seed(seed)
     cfg = model_config_for_depth(depth, vocab_size=vocab, sequence_len=seq_len,
                                  attention_window=attention_window, backend=backend,
-                                 attention_backend="sdpa" if device.type == "cuda" else "torch")
+                                 attention_backend="sdpa" if device.type == "cuda" else "torch",
+                                 activation_checkpoint=activation_checkpoint)
     model = LanguageModel(cfg).to(device)
     kernels.apply_precision_policy(model, "bf16")
     opt = MuonAdamW(model, n_head=cfg.n_head, n_kv_head=cfg.n_kv_head, head_dim=cfg.head_dim,

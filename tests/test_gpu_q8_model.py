@@ -1,0 +1,169 @@
+"""The model on the 8-bit operators: int8 inference and 8-bit activation checkpoints in training."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from hackable_lm_b200.config import model_config_for_depth
+from hackable_lm_b200.model import LanguageModel
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(device, depth=4, **kw):
+    torch.manual_seed(0)
+    cfg = model_config_for_depth(depth, vocab_size=512, sequence_len=256, **kw)
+    return LanguageModel(cfg).to(device).to(torch.bfloat16)
+
+
+def _tokens(device, batch=2, length=256, vocab=512):
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, vocab, (batch, length + 1), generator=g).to(device)
+    return ids[:, :-1].contiguous(), ids[:, 1:].contiguous()
+
+
+def _rel(a, b):
+    a, b = a.double(), b.double()
+    return float((a - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("length", [1, 37, 256])
+@pytest.mark.parametrize("window", [None, 64])
+def test_int8_model_against_bf16_model(length, window, cuda_device):
+    """Rounding a row to 8 bits moves it by a / 127 / sqrt(12) for a magnitude a of about four times
+    its rms: 0.9% of its norm; a projection whose input and weight are both rounded is 1.3% off,
+    and four of them in each of four blocks and the LM head add up to at most sqrt(17) 1.3% = 5.4%
+    of the logits (less: the residual stream carries most).  Held to twice that."""
+    model = _model(cuda_device, attention_window=window)
+    x, y = _tokens(cuda_device, length=length)
+    quantized = model.quantize_int8()
+    with torch.no_grad():
+        logits, none = model(x)
+    got, none8 = quantized(x)
+    assert none is None and none8 is None and got.shape == logits.shape and got.dtype == logits.dtype
+    assert not got.requires_grad
+    assert _rel(got, logits) < 0.11
+    # logits this far apart move the loss by at most their largest difference, on average far less
+    _, loss = quantized(x, y)
+    with torch.no_grad():
+        _, loss16 = model(x, y)
+    assert abs(float(loss) - float(loss16)) <= float((got.float() - logits.float()).abs().max()) + 1e-2
+    y2 = y.clone()
+    y2[0, 0] = -100
+    _, ignored = quantized(x, y2)
+    per = torch.nn.functional.cross_entropy(got.float().reshape(-1, 512), y2.reshape(-1))
+    assert torch.isnan(per) == torch.isnan(ignored) and (torch.isnan(per) or abs(float(per) - float(ignored)) < 1e-2)
+
+
+def test_int8_model_weights_and_state(cuda_device):
+    model = _model(cuda_device, depth=2)
+    quantized = model.quantize_int8()
+    w = quantized.dequantized_weights()
+    assert len(w) == 2 * 4 + 1
+    got, weight = w["blocks.1.gate_up_proj"], model.blocks[1].mlp.gate_up.gate_up_proj.weight
+    step = weight.float().abs().amax(dim=1, keepdim=True) / 127
+    # half a step, and the rounding of the value read back to bf16
+    assert bool(((got.float() - weight.float()).abs() <= 0.5001 * step + weight.float().abs() * 2 ** -8).all())
+    state = quantized.state_dict()
+    assert state["lm_head.weight"].dtype == torch.int8 and state["lm_head.weight_scale"].dtype == torch.float32
+    other = _model(cuda_device, depth=2)
+    with torch.no_grad():
+        for p in other.parameters():
+            p.zero_()
+    other = other.quantize_int8()
+    other.load_state_dict(state)
+    x, _ = _tokens(cuda_device)
+    assert torch.equal(other(x)[0], quantized(x)[0])
+
+
+def test_int8_model_captured_and_replayed(cuda_device):
+    quantized = _model(cuda_device, depth=2).quantize_int8()
+    x, _ = _tokens(cuda_device, batch=1, length=16)
+    quantized(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = quantized(x)
+    x.copy_(x.flip(1))
+    expect, _ = quantized(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, expect)
+
+
+def test_training_with_8_bit_checkpoints(cuda_device):
+    """The forward is that of the bf16 path up to its roundings; each gradient is off by the 8-bit
+    rounding of what was kept: 0.9% of a row's norm for the projections' inputs, 0.7% for gate_up
+    (groups of 128: a is about 2.8 rms), on independent tokens, so below 2% in all, beside the
+    bf16 roundings of two different kernel sequences (below 2% of a gradient, as for the other
+    paths of the model): held to 5%."""
+    x, y = _tokens(cuda_device)
+    plain, kept = _model(cuda_device), _model(cuda_device, activation_checkpoint="int8")
+    kept.load_state_dict(plain.state_dict())
+    _, loss = plain(x, y)
+    _, loss8 = kept(x, y)
+    loss.backward()
+    loss8.backward()
+    loss, loss8 = float(loss.detach()), float(loss8.detach())
+    assert abs(loss - loss8) <= 1e-3 * abs(loss)
+    for (name, p), (_, p8) in zip(plain.named_parameters(), kept.named_parameters()):
+        assert p8.grad is not None and _rel(p8.grad, p.grad) < 0.05, name
+    # the same model in evaluation keeps nothing and runs the usual path
+    with torch.no_grad():
+        assert torch.equal(kept(x)[0], plain(x)[0])
+
+
+def test_8_bit_checkpoints_halve_what_the_mlp_keeps(cuda_device):
+    x = torch.randn(8, 512, 256, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    held = {}
+    for mode in ("none", "int8"):
+        mlp = _model(cuda_device, depth=4, activation_checkpoint=mode).blocks[0].mlp
+        saved = {}
+
+        def keep(t):
+            saved[t.data_ptr()] = t.numel() * t.element_size()
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+            out, norm = mlp(x, x)
+        weights = {p.data_ptr() for p in mlp.parameters()}
+        held[mode] = sum(n for ptr, n in saved.items() if ptr not in weights)
+        (out.float().sum() + norm.float().square().sum()).backward()
+    rows, C, H = 8 * 512, 256, 768
+    assert held["none"] == rows * 2 * (C + 2 * H + H + C)  # x, gate_up, h, and out for the norm
+    assert held["int8"] == rows * (C + 2 * H + H + 4 * (1 + 12 + 1) + 2 * C)
+
+
+def test_train_step_with_8_bit_checkpoints(cuda_device):
+    from hackable_lm_b200 import train
+
+    s = train.build(cuda_device, depth=2, vocab=512, seq_len=256, micro_batch=2, global_tokens=1024,
+                    activation_checkpoint="int8")
+    assert s.config.activation_checkpoint == "int8"
+    batches = train.synthetic_batches(2, 2, 256, 512, 0, cuda_device)
+    loss = train.train_step(s, batches)
+    assert bool(torch.isfinite(loss))
+
+
+def test_compiled_model_with_8_bit_checkpoints(cuda_device):
+    """torch.compile(fullgraph=True) traces the operators.  The compiler's fusions round elsewhere, which
+    moves the gradients of the bf16 model too; the checkpoints, taken of such values, may differ by their
+    own rounding on both sides, sqrt(2) 0.9% of a row's norm: 2% on top of what the bf16 model moves by."""
+    from hackable_lm_b200 import kernels
+    from parity import assert_loss_close
+
+    x, y = _tokens(cuda_device)
+    moved = {}
+    for mode in ("none", "int8"):
+        torch._dynamo.reset()
+        eager = _model(cuda_device, depth=2, activation_checkpoint=mode)
+        twin = _model(cuda_device, depth=2, activation_checkpoint=mode)
+        twin.load_state_dict(eager.state_dict())
+        _, le = eager(x, y)
+        le.backward()
+        _, lc = kernels.compile_training_model(twin, True)(x, y)
+        lc.backward()
+        assert_loss_close(lc.detach(), le.detach(), tol=1e-4, what="compiled loss")
+        moved[mode] = {n: _rel(p.grad, q.grad) for (n, p), (_, q) in zip(twin.named_parameters(), eager.named_parameters())}
+    for n, r in moved["int8"].items():
+        assert r <= moved["none"][n] + 0.02, (n, r, moved["none"][n])

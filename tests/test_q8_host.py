@@ -134,3 +134,39 @@ def test_oracle_swiglu_gradient_against_differences():
     du = (f(gate, up + e) - f(gate, up - e)) / (2 * e)
     tol = 1e-9 * (1 + (d.double() * up).abs().max() + (d.double() * gate).abs().max())
     assert (grad - torch.cat((dg, du), dim=-1)).abs().max() <= tol
+
+
+def test_activation_checkpoint_config():
+    from hackable_lm_b200.config import model_config_for_depth
+    from hackable_lm_b200.model import LanguageModel
+
+    assert model_config_for_depth(2).activation_checkpoint == "none"
+    assert model_config_for_depth(2, activation_checkpoint="INT8").activation_checkpoint == "int8"
+    with pytest.raises(ValueError):
+        model_config_for_depth(2, activation_checkpoint="int4")
+    with pytest.raises(RuntimeError):
+        LanguageModel(model_config_for_depth(2, vocab_size=64, backend="torch", activation_checkpoint="int8"))
+    with pytest.raises(RuntimeError):
+        LanguageModel(model_config_for_depth(2, vocab_size=64)).quantize_int8()
+
+
+def test_models_on_meta_tensors_reach_the_operators():
+    from hackable_lm_b200.config import model_config_for_depth
+    from hackable_lm_b200.model import LanguageModel
+
+    with torch.device("meta"):
+        model = LanguageModel(model_config_for_depth(2, vocab_size=64, sequence_len=128, activation_checkpoint="int8"))
+        model = model.to(torch.bfloat16)
+        idx = torch.zeros(2, 128, dtype=torch.long)
+        kinds = []
+
+        def keep(t):
+            kinds.append(t.dtype)
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+            _, loss = model(idx, idx)
+        loss.backward()
+        assert torch.int8 in kinds and all(p.grad is not None for p in model.parameters())
+        logits, _ = model.quantize_int8()(idx)
+        assert logits.shape == (2, 128, 64) and logits.dtype == torch.bfloat16
