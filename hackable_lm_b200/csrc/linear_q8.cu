@@ -8,12 +8,14 @@
 //
 //  - rows kernel, one token, or up to 8 and few weights: one pass over the weights with
 //    dp4a; bound by reading w (and by launch latency at small sizes).
-//  - split kernel, fewer 128 x 128 output tiles than SMs: weights as the
-//    128-row MMA operand, tokens as the 16..128-column one, K split over a
-//    thread-block cluster whose CTAs add their int32 partial tiles through
-//    distributed shared memory (no workspace, one launch).
-//  - pair kernel, otherwise: the persistent CTA-pair GEMM of gemm_sm100.cuh with
-//    kind::i8 (256 x 256 tiles) and the scales in its epilogue.
+//  - split kernel, few output tiles: weights as the 128-row MMA operand, tokens as
+//    the 16..128-column one, K split over a thread-block cluster whose CTAs add
+//    their int32 partial tiles through distributed shared memory (no workspace,
+//    one launch).
+//  - pair kernel, many: the persistent CTA-pair GEMM of gemm_sm100.cuh with
+//    kind::i8 (256 x 128 or 256 x 256 tiles) and the scales in its epilogue.
+#include <atomic>
+
 #include "gemm_sm100.cuh"
 
 namespace hlm {
@@ -456,7 +458,6 @@ struct EpiScaleQ8 {
   }
 };
 
-constexpr int kQ8Stages = 5;
 constexpr int kQ8EpiWarps = 8;
 
 template <typename T, int BN>
@@ -472,8 +473,49 @@ static int linear_q8_pair(const void* q, const float* scale, const void* w, cons
   GemmParams p;
   gemm_tiling_pair(p, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), BN, 1, KindS8::kBlockK);
   p.err = err;
-  return launch_gemm_pair<BN, kQ8Stages, false, false, EpiScaleQ8<T>, kQ8EpiWarps, KindS8>(
+  return launch_gemm_pair<BN, BN == 256 ? 5 : 7, false, false, EpiScaleQ8<T>, kQ8EpiWarps, KindS8>(
       ma, ma, ma, mb, p, ep, s, HLM_KERNEL_LINEAR_Q8);
+}
+
+// Clusters of `size` CTAs, one to an SM, that the current device holds at once: fewer than
+// SMs / size, since a cluster lies within one GPC (of 148 SMs, 16 clusters of eight).
+// Asked of the runtime once per device and size.
+static int max_clusters(int size) {
+  static std::atomic<int> cache[64][kMaxSplits + 1];
+  int dev = 0;
+  if (size <= 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms_of_current_device();
+  int n = cache[dev][size].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  using L = SplitSmem<64>;
+  auto kern = linear_q8_split_kernel<__nv_bfloat16, 64>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(size), 1, 1);
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 1;
+  }
+  cache[dev][size].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// K blocks of a CTA of the split kernel: the most splits whose clusters run at once.
+static int blocks_per_split(int64_t tiles, int k_blocks) {
+  int64_t splits = num_sms_of_current_device() / tiles;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  if (splits > k_blocks) splits = k_blocks;
+  while (splits > 1 && max_clusters(static_cast<int>(splits)) < tiles) --splits;
+  if (splits < 1) splits = 1;
+  return static_cast<int>((k_blocks + splits - 1) / splits);
 }
 
 template <typename T, int MT>
@@ -484,12 +526,8 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   if (!encode_map(&mw, w, 1, K, N, K, 128) || !encode_map(&mq, q, 1, K, M, K, MT)) return HLM_ERR_DRIVER;
   const int n_tiles = static_cast<int>((N + 127) / 128), m_tiles = static_cast<int>((M + MT - 1) / MT);
   const int k_blocks = static_cast<int>((K + KindS8::kBlockK - 1) / KindS8::kBlockK);
-  int splits = num_sms_of_current_device() / (n_tiles * m_tiles);
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits > k_blocks) splits = k_blocks;
-  if (splits < 1) splits = 1;
-  const int kb_per = (k_blocks + splits - 1) / splits;
-  splits = (k_blocks + kb_per - 1) / kb_per;
+  const int kb_per = blocks_per_split(static_cast<int64_t>(n_tiles) * m_tiles, k_blocks);
+  const int splits = (k_blocks + kb_per - 1) / kb_per;
   auto kern = linear_q8_split_kernel<T, MT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
     return HLM_ERR_LAUNCH;
@@ -539,6 +577,45 @@ static int linear_q8_rows(const void* q, const float* scale, const void* w, cons
   return launch_status();
 }
 
+// The tensor-core kernel that takes least time, in microseconds as measured with K blocks
+// of 128: the split kernel with 16, 32, 64 or 128 tokens a tile (while its tiles fit the
+// SMs at once), or the pair kernel with 256 x 128 (-128) or 256 x 256 (-256) tiles, whose
+// pairs take further tiles in rounds.  Measured either way:
+//   [64, 4096, 768]    32 tokens 4.5 us, 64 tokens 4.9
+//   [128, 768, 2048]   64 tokens 5.2, 128 tokens 6.0;  [128, 8192, 8192] 128 tokens 20, 64 tokens 25
+//   [300, 1000, 4096]  64 tokens 7.7, 256 x 128 14.0;  [512, 2304, 768] 7.3 and 6.5
+//   [1024, 2304, 768]  256 x 128 6.9, 256 x 256 7.7;   [1024, 4096, 768] 9.5 and 8.3
+//   [777, 1111, 1360] to fp32 (rows of 4444 bytes)  64 tokens 8.9, 256 x 128 10.3
+static int choose_tile(int64_t M, int64_t N, int64_t K, bool aligned_rows) {
+  const int64_t sms = num_sms_of_current_device(), pairs = sms / 2 > 0 ? sms / 2 : 1;
+  const int kb = static_cast<int>((K + KindS8::kBlockK - 1) / KindS8::kBlockK);
+  struct {
+    int tokens;
+    double fixed, block;
+  } const split[4] = {{16, 3.4, 0.30}, {32, 3.9, 0.31}, {64, 4.5, 0.34}, {128, 5.5, 0.48}};
+  auto rounds = [&](int64_t bn) {
+    return static_cast<double>((((M + 255) / 256) * ((N + bn - 1) / bn) + pairs - 1) / pairs);
+  };
+  const double r128 = rounds(128), r256 = rounds(256);
+  const double next256 = 0.45 * kb > 3.0 ? 0.45 * kb : 3.0;
+  const double ragged = aligned_rows ? 0.0 : 1.7;  // its epilogue by elements, a round
+  const double pair128 = 4.7 + r128 * (0.29 * kb + ragged) + (r128 - 1.0) * 1.2;
+  const double pair256 = 5.5 + 0.33 * kb + (r256 - 1.0) * next256 + r256 * 2.0 * ragged;
+  int best = pair128 < pair256 ? -128 : -256;
+  double best_us = pair128 < pair256 ? pair128 : pair256;
+  for (const auto& t : split) {
+    const int64_t tiles = ((M + t.tokens - 1) / t.tokens) * ((N + 127) / 128);
+    if (tiles > sms && M > 128) continue;  // (up to 128 tokens a tile is mostly weights: further waves stream on)
+    const double waves = static_cast<double>((tiles + sms - 1) / sms);
+    const double us = t.fixed + waves * t.block * blocks_per_split(tiles, kb);
+    if (us < best_us) {
+      best_us = us;
+      best = t.tokens;
+    }
+  }
+  return best;
+}
+
 template <typename T>
 static int linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, T* out, int64_t M,
                      int64_t N, int64_t K, cudaStream_t s) {
@@ -552,14 +629,20 @@ static int linear_q8(const void* q, const float* scale, const void* w, const flo
   }
   int* err = device_error_ptr();
   if (err == nullptr) return HLM_ERR_LAUNCH;
-  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-  if (M <= 128 || tiles <= num_sms_of_current_device()) {
-    if (M <= 16) return linear_q8_split<T, 16>(q, scale, w, w_scale, out, M, N, K, err, s);
-    if (M <= 32) return linear_q8_split<T, 32>(q, scale, w, w_scale, out, M, N, K, err, s);
-    if (M <= 64) return linear_q8_split<T, 64>(q, scale, w, w_scale, out, M, N, K, err, s);
-    return linear_q8_split<T, 128>(q, scale, w, w_scale, out, M, N, K, err, s);
+  switch (choose_tile(M, N, K, N * static_cast<int64_t>(sizeof(T)) % 16 == 0 && host_aligned16(out))) {
+    case 16:
+      return linear_q8_split<T, 16>(q, scale, w, w_scale, out, M, N, K, err, s);
+    case 32:
+      return linear_q8_split<T, 32>(q, scale, w, w_scale, out, M, N, K, err, s);
+    case 64:
+      return linear_q8_split<T, 64>(q, scale, w, w_scale, out, M, N, K, err, s);
+    case 128:
+      return linear_q8_split<T, 128>(q, scale, w, w_scale, out, M, N, K, err, s);
+    case -128:
+      return linear_q8_pair<T, 128>(q, scale, w, w_scale, out, M, N, K, err, s);
+    default:
+      return linear_q8_pair<T, 256>(q, scale, w, w_scale, out, M, N, K, err, s);
   }
-  return linear_q8_pair<T, 256>(q, scale, w, w_scale, out, M, N, K, err, s);
 }
 
 }  // namespace hlm
