@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_scalar_kernel(
       if (c < hidden) {
         g[i] = to_f32(gate_up[gbase + c]);
         u[i] = to_f32(gate_up[gbase + hidden + c]);
-        h[row * hidden + c] = from_f32<T>(g[i] * sigmoid_fast(g[i]) * u[i]);
+        h[row * hidden + c] = from_f32<T>(g[i] * sigmoidf_(g[i]) * u[i]);
       }
       mg = max(mg, mag_bits(g[i]));
       mu = max(mu, mag_bits(u[i]));

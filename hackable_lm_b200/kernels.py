@@ -298,6 +298,8 @@ def swiglu_ckpt8(gate_up: torch.Tensor) -> torch.Tensor:
     if gate_up.shape[-1] % 2:
         raise RuntimeError(f"SwiGLU input last dimension must be even, got {gate_up.shape[-1]}")
     _cuda_only(gate_up, "swiglu_ckpt8")
+    if not (torch.is_grad_enabled() and gate_up.requires_grad):
+        return ops.swiglu(gate_up)  # no gradient: nothing to keep
     return ops.swiglu_ckpt8(gate_up)[0]
 
 

@@ -110,7 +110,7 @@ uint64_t hlm_launch_count(void);
 #define HLM_KERNEL_LINEAR_Q8 24    /* 8-bit integer projection */
 #define HLM_KERNEL_SWIGLU_CKPT8_FWD 25 /* SwiGLU keeping its input in 8 bits */
 #define HLM_KERNEL_SWIGLU_CKPT8_BWD 26 /* its backward */
-#define HLM_KERNEL_WEIGHT_GRAD_Q8 27   /* weight gradient from an 8-bit input */
+#define HLM_KERNEL_WEIGHT_GRAD_Q8 27   /* weight gradient from an 8-bit input: its GEMM */
 #define HLM_KERNEL_MAX 28
 
 /* Start timing every launch of kernel `kernel_id`: launch i records
@@ -418,10 +418,12 @@ int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const void* grad_h, 
                          int64_t rows, int64_t hidden, int dtype, void* stream);
 
 /* Weight gradient of y = x w^T from x held in 8 bits by rows:
- * grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m]), fp32 sums in a fixed
- * order, rounded to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16
- * (dtype), q int8 [tokens, K], 16-byte aligned; N a multiple of 8, K of 16.
- * tokens == 0 writes zeros.  Workspace bytes from the query, 16-byte aligned. */
+ * grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m]), the values read back
+ * rounded once to dtype, fp32 sums in a fixed order (the same bits every time),
+ * rounded to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16 (dtype), q int8
+ * [tokens, K], 16-byte aligned; N a multiple of 8, K of 16.  tokens == 0 writes
+ * zeros.  Workspace bytes from the query (the values read back, 2 * tokens * K
+ * bytes, and fp32 partial sums where the tokens are split), 16-byte aligned. */
 int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
                        void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N, int64_t K,
                        int dtype, void* stream);

@@ -342,6 +342,18 @@ def test_swiglu_ckpt8_far_and_zero_values(dtype, cuda_device):
     _check_swiglu(gate_up, values((4, 300), dtype, seed=6), cuda_device)
 
 
+@pytest.mark.parametrize("hidden", [64, 100, 129, 2048])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu_ckpt8_output_is_swiglu(hidden, dtype, cuda_device):
+    """The forward's output has the bits of kernels.swiglu_triton, with and without a gradient."""
+    from hackable_lm_b200 import kernels
+
+    gate_up = values((37, 2 * hidden), dtype, seed=hidden).to(cuda_device)
+    plain = kernels.swiglu_triton(gate_up)
+    assert torch.equal(kernels.swiglu_ckpt8(gate_up), plain)
+    assert torch.equal(kernels.swiglu_ckpt8(gate_up.requires_grad_(True)), plain)
+
+
 def test_swiglu_ckpt8_nonfinite_groups_poison_only_themselves(cuda_device):
     from hackable_lm_b200 import ops
 
@@ -608,6 +620,46 @@ def test_backward_captured_while_an_eager_graph_lives(cuda_device):
         again = torch.autograd.grad(live.float().sum(), (x, w))
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(again, expect))
+
+
+def test_first_calls_of_a_process_inside_a_capture(cuda_device, tmp_path):
+    """A process whose first call of each operator is captured: it works, or it is refused with an
+    error; the process goes on and the next, uncaptured call gives the right result."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    script = tmp_path / "first.py"
+    script.write_text(
+        "import sys, torch\n"
+        f"sys.path.insert(0, {str(Path(__file__).resolve().parents[1])!r})\n"
+        "from hackable_lm_b200 import kernels, ops\n"
+        "x = torch.randn(200, 256, device='cuda', dtype=torch.bfloat16)\n"
+        "def run():\n"
+        "    q, s = kernels.quantize_rows(x)\n"
+        "    y = kernels.linear_q8(q, s, q, s)\n"
+        "    one = kernels.linear_q8(q[:1], s[:1], q, s)\n"
+        "    out, nq, ns = kernels.residual_rms_norm_q8(x, x, 1e-6)\n"
+        "    h, cq, cs = ops.swiglu_ckpt8(x)\n"
+        "    return y, one, out, ns, ops.swiglu_ckpt8_backward(cq, cs, h), ops.weight_grad_q8(x, q, s), kernels.dequantize_rows(q, s)\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "try:\n"
+        "    with torch.cuda.graph(g):\n"
+        "        got = run()\n"
+        "    g.replay()\n"
+        "    torch.cuda.synchronize()\n"
+        "    print('captured')\n"
+        "except RuntimeError as e:\n"
+        "    got = None\n"
+        "    print('refused', str(e)[:200])\n"
+        "expect = run()\n"
+        "torch.cuda.synchronize()\n"
+        "assert got is None or all(torch.equal(a, b) for a, b in zip(got, expect))\n"
+        "print('done')\n")
+    out = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("done"), out.stdout + out.stderr
+    print(out.stdout)
 
 
 def test_gradient_asked_of_an_integer_output_is_refused(cuda_device):
