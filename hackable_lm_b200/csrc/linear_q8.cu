@@ -14,6 +14,13 @@
 //    one launch).
 //  - pair kernel, many: the persistent CTA-pair GEMM of gemm_sm100.cuh with
 //    kind::i8 (256 x 128 or 256 x 256 tiles) and the scales in its epilogue.
+//
+// Measured (bf16 out, weights out of L2): one token [4096, 768] 1.9 us, [8192, 8192]
+// 12.6 us (5.3 TB/s of weights); [24, 768, 2048] 3.7 us; [777, 1111, 1360] 8.8 us;
+// [32768, 4096, 768] 94 to 98 us, 2.1 to 2.2 POP/s and 2.9 TB/s of output.  That case
+// takes 78 us without its stores and 92 us without the conversions from int32: the
+// output's stores beside the operands' loads hold it, not the tensor cores, which reach
+// 2.9 POP/s at [8192, 8192, 8192].
 #include <atomic>
 
 #include "gemm_sm100.cuh"
@@ -339,8 +346,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // columns from TMEM (one row per lane), scaled, staged as a 32 x 128-byte box
 // (16-byte chunks swizzled by row) and written out with 16-byte stores, four
 // whole 128-byte row segments per instruction.  Plain stores and not TMA: nothing
-// waits for them, while TMA stores of the two boxes that fit per warp held the
-// epilogue at 3 TB/s.  Outputs whose rows are not 16-byte multiples leave the box
+// waits for them ([32768, 4096, 768] 113 us against 121 with TMA stores of two boxes a
+// warp, and 99 once the accumulator goes back without a release).  Outputs whose rows are not 16-byte multiples leave the box
 // element by element, a row segment per step.
 template <typename T>
 struct EpiScaleQ8 {

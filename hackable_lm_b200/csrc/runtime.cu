@@ -75,7 +75,7 @@ LaunchScope::~LaunchScope() {
 
 using namespace hlm;
 
-extern "C" int hlm_version(void) { return 100; }
+extern "C" int hlm_version(void) { return 200; }
 
 extern "C" const char* hlm_strerror(int code) {
   switch (code) {

@@ -11,7 +11,10 @@
 // (their reads and writes beside the MMA's) held the tensor cores back: 206 us at
 // [32768 tokens, 4096, 768], where the read back costs 13 us once.
 //
-// Bound by the tensor cores (2 * tokens * N * K operations).  Few tiles: the tokens are
+// Bound by the tensor cores (2 * tokens * N * K operations): at [32768, 4096, 768] bf16
+// 175 us back to back, of one call 129 us the GEMM (1.60 PFLOP/s, 96% of the measured
+// burst), 13.5 us the read back and 8.5 us the sum of three partials; small gradients
+// ([1003, 520, 272] 12.7 us) are three launches' latency.  Few tiles: the tokens are
 // split and each split writes an fp32 partial to the workspace; a third kernel adds the
 // partials in the order of the splits (the same bits every time) and rounds.
 #include "gemm_sm100.cuh"
