@@ -24,20 +24,9 @@
 #include <atomic>
 
 #include "gemm_sm100.cuh"
+#include "quant_common.cuh"
 
 namespace hlm {
-
-template <typename T>
-HLM_DEVICE uint32_t pack2(float a, float b);
-template <>
-HLM_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  return pack_bf16x2(a, b);
-}
-template <>
-HLM_DEVICE uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 template <typename T>
 HLM_DEVICE T scaled(int acc, float row_scale, float col_scale) {

@@ -110,6 +110,19 @@ HLM_DEVICE uint32_t unpack_max<__half>(uint32_t m) {
   return mag_bits(__half2float(__ushort_as_half(h)));
 }
 
+// Two floats rounded to a packed pair of 16-bit values, low half first.
+template <typename T>
+HLM_DEVICE uint32_t pack2(float a, float b);
+template <>
+HLM_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  return pack_bf16x2(a, b);
+}
+template <>
+HLM_DEVICE uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 HLM_DEVICE uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 }  // namespace hlm

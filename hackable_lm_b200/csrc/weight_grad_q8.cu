@@ -25,20 +25,8 @@ namespace hlm {
 constexpr int kWgStages = 6;
 constexpr int kWgEpiWarps = 8;
 
-template <typename T>
-HLM_DEVICE uint32_t pack2_16(float a, float b);
-template <>
-HLM_DEVICE uint32_t pack2_16<__nv_bfloat16>(float a, float b) {
-  return pack_bf16x2(a, b);
-}
-template <>
-HLM_DEVICE uint32_t pack2_16<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Write a warp's 32 rows x `kCount` 32-column groups of the accumulator as O (fp32 partial or
-// the 16-bit result): staged in a 32 x 64-byte box (16-byte chunks swizzled by row
+// Write every `parts`-th 32-column group, from `part` on, of a warp's 32 accumulator rows as
+// O (fp32 partial or the 16-bit result): staged in a 32 x 64-byte box (16-byte chunks swizzled by row
 // pairs), out in 16-byte stores, eight 64-byte row segments per instruction.
 template <typename O>
 HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, int cols, uint32_t taddr,
@@ -65,7 +53,7 @@ HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, 
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            w[i] = pack2_16<O>(__uint_as_float(a[8 * c + 2 * i]), __uint_as_float(a[8 * c + 2 * i + 1]));
+            w[i] = pack2<O>(__uint_as_float(a[8 * c + 2 * i]), __uint_as_float(a[8 * c + 2 * i + 1]));
           v = make_uint4(w[0], w[1], w[2], w[3]);
         }
         st_shared_v4(buf + static_cast<uint32_t>(lane * 64) + ((static_cast<uint32_t>(c) ^ sw) << 4), v);
