@@ -565,32 +565,28 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_vec_kernel(
       for (int r = 0; r < R; ++r) {
         uint32_t mg, mu;
         group_maxima<T>(gr[r], ur[r], mg, mu);  // all threads: shuffles
-        if (r0 + r >= rows || cv >= hv) continue;
-        const QuantStep sg = quant_step(mg), su = quant_step(mu);
-        Vec16<T> gv, uv, ov;
-        gv.raw = gr[r];
-        uv.raw = ur[r];
-        float g[VEC], u[VEC], o[VEC];
-        gv.to_float(g);
-        uv.to_float(u);
+        // one division per lane: of a group's threads, 0 and 1 make the gate and up scales (which
+        // they write), 2 and 3 the inverses
+        const float quot = quant_quotient((threadIdx.x & 1) ? mu : mg, threadIdx.x & 2);
+        const float inv_g = __shfl_sync(0xffffffffu, quot, (threadIdx.x & (32 - GT)) + 2);
+        const float inv_u = __shfl_sync(0xffffffffu, quot, (threadIdx.x & (32 - GT)) + 3);
+        if (r0 + r >= rows || cv >= hv_pad) continue;
+        if (cv % GT < 2) scale[(r0 + r) * 2 * groups + (cv & 1) * groups + cv / GT] = quot;
+        if (cv >= hv) continue;
+        F2 g[VEC / 2], u[VEC / 2], o[VEC / 2];
+        f2_load<T>(gr[r], g);
+        f2_load<T>(ur[r], u);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = g[i] * sigmoid_fast(g[i]) * u[i];
-        ov.from_float(o);
-        st_global_v4(h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC, ov.raw);
+        for (int i = 0; i < VEC / 2; ++i) o[i] = g[i] * f2_sigmoid(g[i]) * u[i];
+        st_global_v4(h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC, f2_store<T>(o));
         int8_t* qg = q + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
         if constexpr (VEC == 8) {
-          *reinterpret_cast<uint2*>(qg) =
-              make_uint2(quant_pack4(g[0], g[1], g[2], g[3], sg.inv), quant_pack4(g[4], g[5], g[6], g[7], sg.inv));
+          *reinterpret_cast<uint2*>(qg) = make_uint2(quant_pack4(g[0], g[1], inv_g), quant_pack4(g[2], g[3], inv_g));
           *reinterpret_cast<uint2*>(qg + hidden) =
-              make_uint2(quant_pack4(u[0], u[1], u[2], u[3], su.inv), quant_pack4(u[4], u[5], u[6], u[7], su.inv));
+              make_uint2(quant_pack4(u[0], u[1], inv_u), quant_pack4(u[2], u[3], inv_u));
         } else {
-          *reinterpret_cast<uint32_t*>(qg) = quant_pack4(g[0], g[1], g[2], g[3], sg.inv);
-          *reinterpret_cast<uint32_t*>(qg + hidden) = quant_pack4(u[0], u[1], u[2], u[3], su.inv);
-        }
-        if (cv % GT == 0) {
-          float* sp = scale + (r0 + r) * 2 * groups + cv / GT;
-          sp[0] = sg.scale;
-          sp[groups] = su.scale;
+          *reinterpret_cast<uint32_t*>(qg) = quant_pack4(g[0], g[1], inv_g);
+          *reinterpret_cast<uint32_t*>(qg + hidden) = quant_pack4(u[0], u[1], inv_u);
         }
       }
     }
@@ -634,28 +630,26 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_vec_kernel(
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r0 + r >= rows) continue;
-        Vec16<T> dv, og, ou;
-        dv.raw = dr[r];
-        float d[VEC], rg[VEC], ru[VEC];
-        dv.to_float(d);
+        F2 d[VEC / 2], rg[VEC / 2], ru[VEC / 2];
+        f2_load<T>(dr[r], d);
+        const F2 one = f2(1.0f), minus = f2(-1.0f), sg2 = f2(sg[r]), su2 = f2(su[r]);
 #pragma unroll
         for (int k = 0; k < VEC / 4; ++k) {
-          float g[4], u[4];
-          codes_to_float(qg[r][k], g);
-          codes_to_float(qu[r][k], u);
+          F2 g[2], u[2];
+          codes_to_f2(qg[r][k], g[0], g[1]);
+          codes_to_f2(qu[r][k], u[0], u[1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float gv = g[i] * sg[r], uv = u[i] * su[r], dd = d[4 * k + i];
-            const float s = sigmoid_fast(gv);
-            rg[4 * k + i] = dd * uv * (s * (1.0f + gv * (1.0f - s)));
-            ru[4 * k + i] = dd * (gv * s);
+          for (int i = 0; i < 2; ++i) {
+            const F2 gv = g[i] * sg2, uv = u[i] * su2, dd = d[2 * k + i];
+            const F2 s = f2_sigmoid(gv);
+            // d u s (1 + g (1 - s)) and d (g s)
+            rg[2 * k + i] = dd * uv * (s * f2_fma(gv, f2_fma(s, minus, one), one));
+            ru[2 * k + i] = dd * (gv * s);
           }
         }
-        og.from_float(rg);
-        ou.from_float(ru);
         T* dst = grad_gate_up + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
-        st_global_v4(dst, og.raw);
-        st_global_v4(dst + hidden, ou.raw);
+        st_global_v4(dst, f2_store<T>(rg));
+        st_global_v4(dst + hidden, f2_store<T>(ru));
       }
     }
   }

@@ -42,6 +42,15 @@ HLM_DEVICE QuantStep quant_step(uint32_t max_bits) {
   return s;
 }
 
+// One of the two quotients of quant_step, for threads that share their maximum: each
+// divides once, for the scale or for the inverse, and they pass the values on by shuffle.
+HLM_DEVICE float quant_quotient(uint32_t max_bits, bool is_inv) {
+  const float a = fmaxf(__uint_as_float(max_bits), kQuantFloor);
+  const float d = __fdiv_rn(is_inv ? 127.0f : a, is_inv ? a : 127.0f);
+  if (max_bits >= kInfBits) return is_inv ? 0.0f : __uint_as_float(0x7fc00000u);
+  return d;
+}
+
 // Code of v.  rint through the fp32 magic number 1.5 * 2^23: for |v * inv| <= 127.0001
 // the sum's low mantissa bits are the rounded (half to even) integer in two's
 // complement, so the low byte of the sum is the code.  The product is rounded
@@ -60,14 +69,129 @@ HLM_DEVICE uint32_t quant_pack4(float v0, float v1, float v2, float v3, float in
   return inv == 0.0f ? 0u : __byte_perm(lo, hi, 0x5410);
 }
 
+// Two floats rounded to a packed pair of 16-bit values, low half first.
+template <typename T>
+HLM_DEVICE uint32_t pack2(float a, float b);
+template <>
+HLM_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  return pack_bf16x2(a, b);
+}
+template <>
+HLM_DEVICE uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Pairs of fp32 values in one register pair: sm_100 computes both with one instruction,
+// each rounded as the single operation.  (A packed product that feeds a packed sum
+// is contracted to a fused multiply-add, so products that have to be rounded first
+// are summed one by one.)
+struct F2 {
+  uint64_t v;
+};
+HLM_DEVICE F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+HLM_DEVICE F2 f2(float x) { return f2(x, x); }
+HLM_DEVICE void f2_split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+HLM_DEVICE F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+HLM_DEVICE F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+HLM_DEVICE F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// 1 / (1 + 2^(-x log2 e)) of both values: the bits of sigmoid_fast, whose divide of 1 by a
+// number not below 1 is the approximate reciprocal.
+HLM_DEVICE F2 f2_sigmoid(F2 x) {
+  float a, b;
+  f2_split(x * f2(-1.4426950408889634f), a, b);
+  f2_split(f2(ex2_ftz(a), ex2_ftz(b)) + f2(1.0f), a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return f2(a, b);
+}
+
+// Two packed 16-bit values, or two fp32 ones, as a pair (exact).
+template <typename T>
+HLM_DEVICE F2 f2_unpack(uint32_t w);
+template <>
+HLM_DEVICE F2 f2_unpack<__nv_bfloat16>(uint32_t w) {
+  return f2(bf16_lo(w), bf16_hi(w));
+}
+template <>
+HLM_DEVICE F2 f2_unpack<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2(f.x, f.y);
+}
+// The pairs of a 16-byte vector, and back (rounded to T).
+template <typename T>
+HLM_DEVICE void f2_load(uint4 raw, F2 (&x)[8 / sizeof(T)]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (sizeof(T) == 4) {
+    x[0] = f2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    x[1] = f2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f2_unpack<T>(w[i]);
+  }
+}
+template <typename T>
+HLM_DEVICE uint4 f2_store(const F2 (&x)[8 / sizeof(T)]) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float a, b;
+      f2_split(x[i], a, b);
+      w[2 * i] = __float_as_uint(a);
+      w[2 * i + 1] = __float_as_uint(b);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      f2_split(x[i], a, b);
+      w[i] = pack2<T>(a, b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Four codes of two pairs, packed low byte first.
+HLM_DEVICE uint32_t quant_pack4(F2 x, F2 y, float inv) {
+  float v0, v1, v2, v3;
+  f2_split(x * f2(inv), v0, v1);
+  f2_split(y * f2(inv), v2, v3);
+  const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(v0, 12582912.0f)), __float_as_uint(__fadd_rn(v1, 12582912.0f)), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(v2, 12582912.0f)), __float_as_uint(__fadd_rn(v3, 12582912.0f)), 0x0040);
+  return inv == 0.0f ? 0u : __byte_perm(lo, hi, 0x5410);
+}
+
 // Four codes back as floats: each byte, offset by 128, becomes the low mantissa
 // byte of 2^23, from which 2^23 + 128 is subtracted: exact.
-HLM_DEVICE void codes_to_float(uint32_t packed, float (&f)[4]) {
+HLM_DEVICE void codes_to_f2(uint32_t packed, F2& lo, F2& hi) {
   const uint32_t b = packed ^ 0x80808080u;
-  f[0] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440)) - 8388736.0f;
-  f[1] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7441)) - 8388736.0f;
-  f[2] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7442)) - 8388736.0f;
-  f[3] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7443)) - 8388736.0f;
+  const F2 off = f2(-8388736.0f);
+  lo = f2(__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7441))) + off;
+  hi = f2(__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7443))) + off;
+}
+HLM_DEVICE void codes_to_float(uint32_t packed, float (&f)[4]) {
+  F2 lo, hi;
+  codes_to_f2(packed, lo, hi);
+  f2_split(lo, f[0], f[1]);
+  f2_split(hi, f[2], f[3]);
 }
 
 // Largest magnitude among the elements of a 16-byte vector, as fp32 bits.  The
@@ -108,19 +232,6 @@ template <>
 HLM_DEVICE uint32_t unpack_max<__half>(uint32_t m) {
   const uint16_t h = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
   return mag_bits(__half2float(__ushort_as_half(h)));
-}
-
-// Two floats rounded to a packed pair of 16-bit values, low half first.
-template <typename T>
-HLM_DEVICE uint32_t pack2(float a, float b);
-template <>
-HLM_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  return pack_bf16x2(a, b);
-}
-template <>
-HLM_DEVICE uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 HLM_DEVICE uint32_t warp_max_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }

@@ -354,6 +354,24 @@ def test_swiglu_ckpt8_output_is_swiglu(hidden, dtype, cuda_device):
     assert torch.equal(kernels.swiglu_ckpt8(gate_up.requires_grad_(True)), plain)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu_ckpt8_output_is_swiglu_for_every_16_bit_gate(dtype, cuda_device):
+    """Every 16-bit gate (and 2^20 fp32 ones over the whole range), NaNs and infinities among them."""
+    from hackable_lm_b200 import kernels, ops
+
+    if dtype == torch.float32:
+        g = torch.Generator().manual_seed(3)
+        gate = torch.cat((torch.randn(1 << 19, generator=g) * 30, torch.randint(-2 ** 31, 2 ** 31 - 1, (1 << 19,), generator=g,
+                                                                              dtype=torch.int32).view(torch.float32)))
+    else:
+        gate = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    gate = gate.reshape(-1, 256)
+    gate_up = torch.cat((gate, torch.ones_like(gate)), dim=1).to(cuda_device)
+    plain, h = kernels.swiglu_triton(gate_up), ops.swiglu_ckpt8(gate_up)[0]
+    assert torch.equal(torch.isnan(plain), torch.isnan(h))
+    assert torch.equal(torch.nan_to_num(plain, nan=0.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(h, nan=0.0, posinf=1.0, neginf=-1.0))
+
+
 def test_swiglu_ckpt8_nonfinite_groups_poison_only_themselves(cuda_device):
     from hackable_lm_b200 import ops
 
