@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_scalar_kernel(
       }
       const QuantStep sg = quant_step(warp_max_u32(mg));
       const QuantStep su = quant_step(warp_max_u32(mu));
-      const uint32_t cg = quant_pack4(g[0], g[1], g[2], g[3], sg.inv);
-      const uint32_t cu = quant_pack4(u[0], u[1], u[2], u[3], su.inv);
+      const uint32_t cg = quant_pack4(f2(g[0], g[1]), f2(g[2], g[3]), sg.inv);
+      const uint32_t cu = quant_pack4(f2(u[0], u[1]), f2(u[2], u[3]), su.inv);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = c0 + 32 * i;
@@ -229,6 +229,21 @@ HLM_DEVICE uint32_t row_max(uint32_t v, uint32_t* sh, int t) {
   return v;
 }
 
+// Weights of the VEC columns from c on; columns outside the row (SHIFT) count as zeros.
+template <typename T, bool SHIFT>
+HLM_DEVICE void load_weight(const T* weight, int c, int cols, F2 (&w)[8 / sizeof(T)]) {
+  if constexpr (!SHIFT) {
+    f2_load<T>(ld_global_v4(weight + c), w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(8 / sizeof(T)); ++i) {
+      const int k = c + 2 * i;
+      w[i] = f2(k >= 0 && k < cols ? to_f32(weight[k]) : 0.0f,
+                k + 1 >= 0 && k + 1 < cols ? to_f32(weight[k + 1]) : 0.0f);
+    }
+  }
+}
+
 template <typename T, int TPR, int NV, bool NORM, bool SHIFT>
 __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
     const T* __restrict__ residual, const T* __restrict__ x, const T* __restrict__ weight,
@@ -285,32 +300,27 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
       }
     }
     // the sum, rounded to T once, back in v; squares and magnitudes of it
-    float ss = 0.0f;
+    F2 ss2 = f2(0.0f);
     uint32_t mp = 0;
     uint32_t mw = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (t + TPR * j) * VEC - head;
       if constexpr (NORM) {
-        Vec16<T> a;
-        a.raw = v[j];
-        float f[VEC];
-        a.to_float(f);
+        F2 f[VEC / 2];
+        f2_load<T>(v[j], f);
         if (residual != nullptr) {
-          Vec16<T> b;
-          b.raw = rr[j];
-          float g[VEC];
-          b.to_float(g);
+          F2 g[VEC / 2];
+          f2_load<T>(rr[j], g);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) f[i] += g[i];
-          a.from_float(f);
-          v[j] = a.raw;
-          a.to_float(f);
+          for (int i = 0; i < VEC / 2; ++i) f[i] = f[i] + g[i];
+          v[j] = f2_store<T>(f);
+          f2_load<T>(v[j], f);
           if (row_ok && c < cols) {
             if (!SHIFT || (c >= 0 && c + VEC <= cols)) {
-              st_global_v4(out + base + c, a.raw);
+              st_global_v4(out + base + c, v[j]);
             } else {
-              const T* e = reinterpret_cast<const T*>(&a.raw);
+              const T* e = reinterpret_cast<const T*>(&v[j]);
 #pragma unroll
               for (int i = 0; i < VEC; ++i)
                 if (c + i >= 0 && c + i < cols) out[base + c + i] = e[i];
@@ -318,21 +328,15 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
           }
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) ss += f[i] * f[i];
-        if (weight != nullptr) {
-          if (!SHIFT) {
-            if (c < cols) {
-              Vec16<T> w;
-              w.raw = ld_global_v4(weight + c);
-              float g[VEC];
-              w.to_float(g);
+        for (int i = 0; i < VEC / 2; ++i) ss2 = f2_fma(f[i], f[i], ss2);
+        if (weight != nullptr && row_ok && c < cols) {
+          F2 w[VEC / 2];
+          load_weight<T, SHIFT>(weight, c, cols, w);
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) mw = max(mw, mag_bits(__fmul_rn(f[i], g[i])));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-              if (c + i >= 0 && c + i < cols) mw = max(mw, mag_bits(__fmul_rn(f[i], to_f32(weight[c + i]))));
+          for (int i = 0; i < VEC / 2; ++i) {
+            float a, b;
+            f2_split(f[i] * w[i], a, b);
+            mw = max(mw, max(mag_bits(a), mag_bits(b)));
           }
         }
       }
@@ -342,8 +346,11 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
     if (NORM && weight != nullptr) m = mw;
     m = row_max<TPR>(m, sh_max, t);
     const QuantStep st = quant_step(m);
+    float ss = 0.0f;
     if constexpr (NORM) {
-      ss = warp_sum(ss);
+      float lo, hi;
+      f2_split(ss2, lo, hi);
+      ss = warp_sum(lo + hi);
       if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
         const int w0 = (threadIdx.x / TPR) * W;
@@ -362,30 +369,19 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
     for (int j = 0; j < NV; ++j) {
       const int c = (t + TPR * j) * VEC - head;
       if (!row_ok || c >= cols) continue;
-      Vec16<T> a;
-      a.raw = v[j];
-      float f[VEC];
-      a.to_float(f);
+      F2 f[VEC / 2];
+      f2_load<T>(v[j], f);
       if (NORM && weight != nullptr) {
-        if (!SHIFT) {
-          Vec16<T> w;
-          w.raw = ld_global_v4(weight + c);
-          float g[VEC];
-          w.to_float(g);
+        F2 w[VEC / 2];
+        load_weight<T, SHIFT>(weight, c, cols, w);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) f[i] = __fmul_rn(f[i], g[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (c + i >= 0 && c + i < cols) f[i] = __fmul_rn(f[i], to_f32(weight[c + i]));
-        }
+        for (int i = 0; i < VEC / 2; ++i) f[i] = f[i] * w[i];
       }
       int8_t* dst = SHIFT ? row_stage + c + head : q + base + c;
       if constexpr (VEC == 8)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(quant_pack4(f[0], f[1], f[2], f[3], st.inv),
-                                                    quant_pack4(f[4], f[5], f[6], f[7], st.inv));
+        *reinterpret_cast<uint2*>(dst) = make_uint2(quant_pack4(f[0], f[1], st.inv), quant_pack4(f[2], f[3], st.inv));
       else
-        *reinterpret_cast<uint32_t*>(dst) = quant_pack4(f[0], f[1], f[2], f[3], st.inv);
+        *reinterpret_cast<uint32_t*>(dst) = quant_pack4(f[0], f[1], st.inv);
     }
     if constexpr (SHIFT) {
       row_sync<TPR>();
@@ -491,18 +487,19 @@ __global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* __restr
       const I next = (row + 1) * cols - e;  // codes from here on belong to the next row
       const float s0 = scale[row];
       if (e + VEC <= total) {
-        const float s1 = next < VEC ? scale[row + 1] : s0;
-        float f[VEC];
+        F2 f[VEC / 2];
 #pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) {
-          float c[4];
-          codes_to_float(w[u][k], c);
+        for (int k = 0; k < VEC / 4; ++k) codes_to_f2(w[u][k], f[2 * k], f[2 * k + 1]);
+        if (next >= VEC) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f[4 * k + i] = c[i] * (static_cast<I>(4 * k + i) < next ? s0 : s1);
+          for (int i = 0; i < VEC / 2; ++i) f[i] = f[i] * f2(s0);
+        } else {  // a row ends among these codes
+          const float s1 = scale[row + 1];
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i)
+            f[i] = f[i] * f2(static_cast<I>(2 * i) < next ? s0 : s1, static_cast<I>(2 * i + 1) < next ? s0 : s1);
         }
-        Vec16<T> o;
-        o.from_float(f);
-        st_global_v4(out + e, o.raw);
+        st_global_v4(out + e, f2_store<T>(f));
       } else {
         for (I i = 0; e + i < total; ++i)
           out[e + i] = from_f32<T>(static_cast<float>(q[e + i]) * (i < next ? s0 : scale[row + 1]));

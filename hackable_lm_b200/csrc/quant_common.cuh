@@ -62,13 +62,6 @@ HLM_DEVICE uint32_t quant_bits(float v, float inv) {
 HLM_DEVICE int8_t quant_code(float v, const QuantStep& s) {
   return s.inv == 0.0f ? static_cast<int8_t>(0) : static_cast<int8_t>(quant_bits(v, s.inv) & 0xffu);
 }
-// Four codes packed low byte first.
-HLM_DEVICE uint32_t quant_pack4(float v0, float v1, float v2, float v3, float inv) {
-  const uint32_t lo = __byte_perm(quant_bits(v0, inv), quant_bits(v1, inv), 0x0040);
-  const uint32_t hi = __byte_perm(quant_bits(v2, inv), quant_bits(v3, inv), 0x0040);
-  return inv == 0.0f ? 0u : __byte_perm(lo, hi, 0x5410);
-}
-
 // Two floats rounded to a packed pair of 16-bit values, low half first.
 template <typename T>
 HLM_DEVICE uint32_t pack2(float a, float b);
@@ -186,12 +179,6 @@ HLM_DEVICE void codes_to_f2(uint32_t packed, F2& lo, F2& hi) {
   const F2 off = f2(-8388736.0f);
   lo = f2(__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7441))) + off;
   hi = f2(__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7443))) + off;
-}
-HLM_DEVICE void codes_to_float(uint32_t packed, float (&f)[4]) {
-  F2 lo, hi;
-  codes_to_f2(packed, lo, hi);
-  f2_split(lo, f[0], f[1]);
-  f2_split(hi, f[2], f[3]);
 }
 
 // Largest magnitude among the elements of a 16-byte vector, as fp32 bits.  The
