@@ -64,6 +64,14 @@ template <class E>
 struct epi_relaxed_release<E, std::void_t<decltype(E::kRelaxedRelease)>>
     : std::integral_constant<bool, E::kRelaxedRelease> {};
 
+// Epilogues that declare `static constexpr bool kDependentLaunch = true` run as dependents
+// of the kernel before them in the stream (pair kernel): set-up overlaps its end.
+template <class E, class = void>
+struct epi_dependent : std::false_type {};
+template <class E>
+struct epi_dependent<E, std::void_t<decltype(E::kDependentLaunch)>>
+    : std::integral_constant<bool, E::kDependentLaunch> {};
+
 // Epilogues that read per-row or per-column values from global memory declare a struct
 // `Early` and `load_early`: the pair kernel calls it before it waits for the tile's
 // accumulator, and hands the struct to `run`.
@@ -424,6 +432,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
   __syncwarp();
   cluster_sync_all();  // both CTAs' barriers initialised before any cross-CTA signal
   tc_fence_after();
+  if constexpr (epi_dependent<Epi>::value) {
+    grid_launch_next();
+    grid_wait();
+  }
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int total = p.m_tiles * p.n_tiles * p.splits;  // m_tiles counts 256-row pair tiles
   const int w_first = static_cast<int>(cluster_id_x());
@@ -721,7 +733,13 @@ int launch_gemm_pair(const CUtensorMap& a0, const CUtensorMap& a1, const CUtenso
   if (pairs < 1) pairs = 1;
   {
     LaunchScope scope(kernel_id, stream);
-    kern<<<2 * pairs, gemm_threads<EPI_WARPS>(), smem, stream>>>(a0, a1, a2, b, p, ep);
+    if constexpr (epi_dependent<Epi>::value) {
+      if (launch_dependent(kern, dim3(2 * pairs), dim3(gemm_threads<EPI_WARPS>()), smem, stream, 1, a0, a1, a2, b, p,
+                           ep) != cudaSuccess)
+        return HLM_ERR_LAUNCH;
+    } else {
+      kern<<<2 * pairs, gemm_threads<EPI_WARPS>(), smem, stream>>>(a0, a1, a2, b, p, ep);
+    }
   }
   return launch_status();
 }

@@ -568,6 +568,17 @@ HLM_DEVICE uint4 ld_global_nc_v4(const void* p) {
                : "l"(p));
   return v;
 }
+// The same through the coherent path, for kernels that run as dependents of the kernel that
+// writes the data (launch_dependent): the read-only path asks that nobody writes it while
+// the kernel runs, its set-up included.
+HLM_DEVICE uint4 ld_global_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
 HLM_DEVICE uint4 ld_global_v4(const void* p) {
   uint4 v;
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -626,6 +637,40 @@ HLM_DEVICE float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// ---------------------------------------------------------------------------
+// Programmatic dependent launch.  A kernel launched with launch_dependent() may be set up
+// on the SMs while the kernel before it in the stream finishes: it touches global
+// memory only after grid_wait(), which returns when that kernel (and, since every
+// kernel here waits, all before it) has completed and its writes are visible;
+// grid_launch_next() allows the same to the kernel after it.  Its loads take the
+// coherent path: no __restrict__, no __ldg, no ld.global.nc.  Launched without the
+// attribute, both do nothing.
+// ---------------------------------------------------------------------------
+HLM_DEVICE void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+HLM_DEVICE void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launch on `stream` as a dependent of the kernel before it, in clusters of `cluster` CTAs
+// along x (1: as the kernel declares).
+template <class... Params, class... Args>
+inline cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                    int cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
 }
 
 // Host helper: 16-byte alignment of a device pointer.

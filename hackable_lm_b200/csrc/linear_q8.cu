@@ -15,12 +15,14 @@
 //  - pair kernel, many: the persistent CTA-pair GEMM of gemm_sm100.cuh with
 //    kind::i8 (256 x 128 or 256 x 256 tiles) and the scales in its epilogue.
 //
-// Measured (bf16 out, weights out of L2): one token [4096, 768] 1.9 us, [8192, 8192]
-// 12.6 us (5.3 TB/s of weights); [24, 768, 2048] 3.7 us; [777, 1111, 1360] 8.8 us;
-// [32768, 4096, 768] 94 to 98 us, 2.1 to 2.2 POP/s and 2.9 TB/s of output.  That case
-// takes 78 us without its stores and 92 us without the conversions from int32: the
-// output's stores beside the operands' loads hold it, not the tensor cores, which reach
-// 2.9 POP/s at [8192, 8192, 8192].
+// Measured (bf16 out, weights out of L2): one token [4096, 768] 2.0 us, [8192, 8192]
+// 12.7 us (5.3 TB/s of weights); [24, 768, 2048] 3.0 us; [777, 1111, 1360] 7.9 us;
+// [32768, 4096, 768] 94 us, 2.2 POP/s and 2.9 TB/s of output (110 us once the power cap
+// holds the clock at 1.4 GHz).  That case takes 78 us without its stores and 92 us without
+// the conversions from int32: the output's stores beside the operands' loads hold it,
+// not the tensor cores, which reach 2.9 POP/s at [8192, 8192, 8192].  Launched as
+// dependents of the kernel before: [24, 768, 2048] 3.7 -> 3.0 us, [1024, 4096, 768]
+// 8.1 -> 7.0.
 #include <atomic>
 
 #include "gemm_sm100.cuh"
@@ -40,9 +42,11 @@ constexpr int kRowsWarps = 4;  // warps of a block
 
 template <typename T, int MR, int R, int KS>
 __global__ void __launch_bounds__(32 * kRowsWarps) linear_q8_rows_kernel(
-    const int8_t* __restrict__ q, const float* __restrict__ scale, const int8_t* __restrict__ w,
-    const float* __restrict__ w_scale, T* __restrict__ out, int M, int N, int K) {
+    const int8_t* q, const float* scale, const int8_t* w,
+    const float* w_scale, T* out, int M, int N, int K) {
   static_assert(KS == 1 || KS == kRowsWarps, "a warp's own channels, or a block's");
+  grid_launch_next();
+  grid_wait();
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   const int64_t n0 = (KS == 1 ? static_cast<int64_t>(blockIdx.x) * kRowsWarps + warp : blockIdx.x) * R;
@@ -58,12 +62,12 @@ __global__ void __launch_bounds__(32 * kRowsWarps) linear_q8_rows_kernel(
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t n = n0 + r < N ? n0 + r : N - 1;  // the last warp's spare rows repeat a row
-      wv[r] = ld_global_nc_v4(w + n * K + k);
+      wv[r] = ld_global_stream_v4(w + n * K + k);
     }
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
       const int mm = m < M ? m : M - 1;
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + static_cast<int64_t>(mm) * K + k));
+      const uint4 x = ld_global_v4(q + static_cast<int64_t>(mm) * K + k);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         acc[r][m] = __dp4a(static_cast<int>(wv[r].x), static_cast<int>(x.x), acc[r][m]);
@@ -150,8 +154,8 @@ HLM_DEVICE uint32_t cluster_nctarank() {
 template <typename T, int MT>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     linear_q8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_q,
-                           const float* __restrict__ scale, const float* __restrict__ w_scale,
-                           T* __restrict__ out, int M, int N, int k_blocks, int kb_per, int vec, int* err) {
+                           const float* scale, const float* w_scale,
+                           T* out, int M, int N, int k_blocks, int kb_per, int vec, int* err) {
   using L = SplitSmem<MT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -189,6 +193,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncthreads();
   tc_fence_after();
   cluster_arrive_relaxed();  // this CTA runs: its memory may be written from now on
+  grid_launch_next();
+  grid_wait();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   // What the last step needs from global memory, fetched now.  A warp then takes the owned
@@ -347,6 +353,7 @@ struct EpiScaleQ8 {
     int vec;  // rows of the output are 16-byte aligned
   };
   static constexpr bool kRelaxedRelease = true;
+  static constexpr bool kDependentLaunch = true;
   static constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a group
   static constexpr int kPerChunk = 16 / static_cast<int>(sizeof(T));
   static constexpr int kBoxBytes = 32 * 128;
@@ -527,24 +534,13 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   auto kern = linear_q8_split_kernel<T, MT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
     return HLM_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
   // four outputs of a lane as one store
   const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
-  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles), 1);
-  cfg.blockDim = dim3(kSplitThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   {
     LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
-    if (cudaLaunchKernelEx(&cfg, kern, mw, mq, scale, w_scale, out, static_cast<int>(M), static_cast<int>(N),
-                           k_blocks, kb_per, vec, err) != cudaSuccess)
+    if (launch_dependent(kern, dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles)),
+                         dim3(kSplitThreads), L::kBytes, s, splits, mw, mq, scale, w_scale, out, static_cast<int>(M),
+                         static_cast<int>(N), k_blocks, kb_per, vec, err) != cudaSuccess)
       return HLM_ERR_LAUNCH;
   }
   return launch_status();
@@ -561,15 +557,12 @@ static int linear_q8_rows(const void* q, const float* scale, const void* w, cons
   const int8_t* qp = static_cast<const int8_t*>(q);
   const int8_t* wp = static_cast<const int8_t*>(w);
   LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
-  if (K >= 2048 && (M == 1 || N <= 2048)) {
-    const int64_t blocks = (N + R - 1) / R;
-    linear_q8_rows_kernel<T, MR, R, kRowsWarps><<<static_cast<unsigned>(blocks), 32 * kRowsWarps, 0, s>>>(
-        qp, scale, wp, w_scale, out, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
-  } else {
-    const int64_t blocks = (N + R * kRowsWarps - 1) / (R * kRowsWarps);
-    linear_q8_rows_kernel<T, MR, R, 1><<<static_cast<unsigned>(blocks), 32 * kRowsWarps, 0, s>>>(
-        qp, scale, wp, w_scale, out, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
-  }
+  const bool shared = K >= 2048 && (M == 1 || N <= 2048);
+  const int64_t blocks = shared ? (N + R - 1) / R : (N + R * kRowsWarps - 1) / (R * kRowsWarps);
+  if (launch_dependent(shared ? linear_q8_rows_kernel<T, MR, R, kRowsWarps> : linear_q8_rows_kernel<T, MR, R, 1>,
+                       dim3(static_cast<unsigned>(blocks)), dim3(32 * kRowsWarps), 0, s, 1, qp, scale, wp, w_scale, out,
+                       static_cast<int>(M), static_cast<int>(N), static_cast<int>(K)) != cudaSuccess)
+    return HLM_ERR_LAUNCH;
   return launch_status();
 }
 

@@ -5,11 +5,14 @@
 // All bound by HBM: each reads its inputs once (16-byte vectors, kept in registers
 // between the maximum and the codes) and writes its outputs once.  Measured with the
 // inputs out of L2, share of the measured copy rate (6.55 TB/s):
-//   quantise   [32768, 2048] bf16 33.8 us (91%), fp32 51 us (100%)
-//   read back  [32768, 2048] bf16 32.8 us (94%), fp32 53 us (96%)
-//   norm       [32768, 768] bf16 29.3 us (92%), fp32 51 us (98%)
-//   SwiGLU     [32768, 2 x 2048] bf16 84 us forward (98%), 85.5 us backward (96%)
-// A few rows: 1.5 to 2.5 us, a launch.
+//   quantise   [32768, 2048] bf16 32.1 us (96%), fp32 50.6 us (101%)
+//   read back  [32768, 2048] bf16 31.5 us (97%), fp32 52.4 us (98%)
+//   norm       [32768, 768] bf16 27.0 us (100%), [32768, 2048] 73 us (98%)
+//   SwiGLU     [32768, 2 x 2048] bf16 82 us forward and backward (100%)
+// A few rows: 1.4 to 2 us, a launch.  Arithmetic on packed fp32 pairs: under the power cap
+// the clock falls to 1.4 GHz and the SwiGLU kernels come near their issue rate (0.78
+// instructions a cycle at full clock before).  Launched as dependents of the kernel before:
+// quantise and read back, one after the other, 69.6 -> 65.6 us.
 #include "quant_common.cuh"
 
 namespace hlm {
@@ -45,6 +48,12 @@ static inline int quant_grid(int64_t items, int per_block) {
   return static_cast<int>(blocks);
 }
 
+// Launch as a dependent of the kernel before (a failure shows in launch_status()).
+template <class... Params, class... Args>
+static inline void launch_quant(void (*kern)(Params...), int grid, int block, cudaStream_t s, Args... args) {
+  (void)launch_dependent(kern, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(block)), 0, s, 1, args...);
+}
+
 // Rows wider than 16,384 16-bit or 8,192 fp32 columns, and tensors that are aligned
 // differently: one warp per row, two passes over it (the second one hits L1/L2).
 // NORM: v = round(residual + branch) [* weight], written to `out` when there is
@@ -52,9 +61,11 @@ static inline int quant_grid(int64_t items, int per_block) {
 // to the row, so it cancels from the codes and scales the step alone.
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(256) quant_rows_scalar_kernel(
-    const T* __restrict__ residual, const T* __restrict__ x, const T* __restrict__ weight,
-    T* __restrict__ out, int8_t* __restrict__ q, float* __restrict__ scale, int64_t rows, int cols,
+    const T* residual, const T* x, const T* weight,
+    T* out, int8_t* q, float* scale, int64_t rows, int cols,
     float eps) {
+  grid_launch_next();
+  grid_wait();
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * wpb + (threadIdx.x >> 5); row < rows;
@@ -94,10 +105,12 @@ __global__ void __launch_bounds__(256) quant_rows_scalar_kernel(
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dequant_rows_scalar_kernel(const int8_t* __restrict__ q,
-                                                                 const float* __restrict__ scale,
-                                                                 T* __restrict__ out, int64_t rows,
+__global__ void __launch_bounds__(256) dequant_rows_scalar_kernel(const int8_t* q,
+                                                                 const float* scale,
+                                                                 T* out, int64_t rows,
                                                                  int cols) {
+  grid_launch_next();
+  grid_wait();
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * wpb + (threadIdx.x >> 5); row < rows;
@@ -114,8 +127,10 @@ __global__ void __launch_bounds__(256) dequant_rows_scalar_kernel(const int8_t* 
 // elements one by one); two and four rows a warp at once measured slower (fewer warps fit).
 template <typename T>
 __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_scalar_kernel(
-    const T* __restrict__ gate_up, T* __restrict__ h, int8_t* __restrict__ q,
-    float* __restrict__ scale, int64_t rows, int hidden, int groups) {
+    const T* gate_up, T* h, int8_t* q,
+    float* scale, int64_t rows, int hidden, int groups) {
+  grid_launch_next();
+  grid_wait();
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -163,8 +178,10 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_scalar_kernel(
 
 template <typename T>
 __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
-    const int8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ grad_h,
-    T* __restrict__ grad_gate_up, int64_t rows, int hidden, int groups) {
+    const int8_t* q, const float* scale, const T* grad_h,
+    T* grad_gate_up, int64_t rows, int hidden, int groups) {
+  grid_launch_next();
+  grid_wait();
   const int lane = threadIdx.x & 31;
   const int wpb = blockDim.x >> 5;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -195,7 +212,7 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
 // kept in registers between the maximum (and the sum of squares) and the codes.
 //
 // A row starts anywhere in its 16-byte vector when cols is not a multiple of the
-// vector (SHIFT; [16384, 2047] bf16 27 us, 57% of the copy rate): threads then load the aligned vectors that cover the row, elements
+// vector (SHIFT; [16384, 2047] bf16 26 us, 60% of the copy rate): threads then load the aligned vectors that cover the row, elements
 // outside the row count as zeros, and the codes go through shared memory so that
 // they too leave in 16-byte stores.  Only the row's first and last vectors, whose
 // other elements belong to the neighbouring rows, are read and written by elements.
@@ -246,9 +263,11 @@ HLM_DEVICE void load_weight(const T* weight, int c, int cols, F2 (&w)[8 / sizeof
 
 template <typename T, int TPR, int NV, bool NORM, bool SHIFT>
 __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
-    const T* __restrict__ residual, const T* __restrict__ x, const T* __restrict__ weight,
-    T* __restrict__ out, int8_t* __restrict__ q, float* __restrict__ scale, int64_t rows, int cols,
+    const T* residual, const T* x, const T* weight,
+    T* out, int8_t* q, float* scale, int64_t rows, int cols,
     float eps) {
+  grid_launch_next();
+  grid_wait();
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
   constexpr int RPB = kRowThreads / TPR;
   constexpr int kStage = SHIFT ? TPR * NV * VEC + 16 : 16;  // bytes of one row's codes
@@ -271,8 +290,8 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_vec_kernel(
       const int c = (t + TPR * j) * VEC - head;  // column of the vector's first element
       if (!row_ok || c >= cols) continue;
       if (!SHIFT || (base + c >= 0 && base + c + VEC <= total)) {
-        v[j] = ld_global_nc_v4(x + base + c);
-        if (NORM && residual != nullptr) rr[j] = ld_global_nc_v4(residual + base + c);
+        v[j] = ld_global_stream_v4(x + base + c);
+        if (NORM && residual != nullptr) rr[j] = ld_global_stream_v4(residual + base + c);
       } else {  // the tensor's own first or last vector
         T* e = reinterpret_cast<T*>(&v[j]);
         T* f = reinterpret_cast<T*>(&rr[NORM ? j : 0]);
@@ -427,8 +446,8 @@ static bool launch_quant_rows_vec(const T* residual, const T* x, const T* weight
   const int64_t nv = aligned ? cols / VEC : (cols + VEC - 1) / VEC + 1;
 #define HLM_ROWS_LAUNCH(TPR, NV, SHIFT)                                                                     \
   do {                                                                                                      \
-    quant_rows_vec_kernel<T, TPR, NV, NORM, SHIFT><<<quant_grid(rows, kRowThreads / TPR), kRowThreads, 0, s>>>( \
-        residual, x, weight, out, q, scale, rows, cols, eps);                                               \
+    launch_quant(quant_rows_vec_kernel<T, TPR, NV, NORM, SHIFT>, quant_grid(rows, kRowThreads / TPR), kRowThreads, s, \
+                 residual, x, weight, out, q, scale, rows, cols, eps);                                       \
     return true;                                                                                            \
   } while (0)
   if (aligned) {
@@ -457,9 +476,11 @@ static bool launch_quant_rows_vec(const T* residual, const T* x, const T* weight
 // store) whatever the row length, since so few lie in at most two rows of 16 or more
 // columns; one division finds the row.  Four such steps of a block in flight.
 template <typename T, typename I>
-__global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* __restrict__ q,
-                                                          const float* __restrict__ scale,
-                                                          T* __restrict__ out, I total, I cols) {
+__global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* q,
+                                                          const float* scale,
+                                                          T* out, I total, I cols) {
+  grid_launch_next();
+  grid_wait();
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
   constexpr int U = 4;
   constexpr I kSpan = 256 * VEC;  // codes of one step of the block
@@ -471,11 +492,11 @@ __global__ void __launch_bounds__(256) dequant_flat_kernel(const int8_t* __restr
       const I e = e0 + u * kSpan;
       if (e + VEC <= total) {
         if constexpr (VEC == 8) {
-          const uint2 a = __ldg(reinterpret_cast<const uint2*>(q + e));
+          const uint2 a = *reinterpret_cast<const uint2*>(q + e);
           w[u][0] = a.x;
           w[u][1] = a.y;
         } else {
-          w[u][0] = __ldg(reinterpret_cast<const uint32_t*>(q + e));
+          w[u][0] = *reinterpret_cast<const uint32_t*>(q + e);
         }
       }
     }
@@ -538,8 +559,10 @@ static inline int row_block(int64_t n) {
 
 template <typename T, int R>
 __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_vec_kernel(
-    const T* __restrict__ gate_up, T* __restrict__ h, int8_t* __restrict__ q,
-    float* __restrict__ scale, int64_t rows, int hv, int groups) {
+    const T* gate_up, T* h, int8_t* q,
+    float* scale, int64_t rows, int hv, int groups) {
+  grid_launch_next();
+  grid_wait();
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
   constexpr int GT = kCkptGroup / VEC;  // threads of a group
   const int64_t hidden = static_cast<int64_t>(hv) * VEC;
@@ -554,8 +577,8 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_vec_kernel(
         gr[r] = ur[r] = make_uint4(0, 0, 0, 0);
         if (r0 + r < rows && cv < hv) {
           const T* src = gate_up + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
-          gr[r] = ld_global_nc_v4(src);
-          ur[r] = ld_global_nc_v4(src + hidden);
+          gr[r] = ld_global_stream_v4(src);
+          ur[r] = ld_global_stream_v4(src + hidden);
         }
       }
 #pragma unroll
@@ -592,8 +615,10 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_fwd_vec_kernel(
 
 template <typename T, int R>
 __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_vec_kernel(
-    const int8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ grad_h,
-    T* __restrict__ grad_gate_up, int64_t rows, int hv, int groups) {
+    const int8_t* q, const float* scale, const T* grad_h,
+    T* grad_gate_up, int64_t rows, int hv, int groups) {
+  grid_launch_next();
+  grid_wait();
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
   constexpr int GT = kCkptGroup / VEC;
   const int64_t hidden = static_cast<int64_t>(hv) * VEC;
@@ -608,20 +633,20 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_vec_kernel(
         if (r0 + r < rows) {
           const int8_t* src = q + (r0 + r) * 2 * hidden + static_cast<int64_t>(cv) * VEC;
           if constexpr (VEC == 8) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(src));
-            const uint2 b = __ldg(reinterpret_cast<const uint2*>(src + hidden));
+            const uint2 a = *reinterpret_cast<const uint2*>(src);
+            const uint2 b = *reinterpret_cast<const uint2*>(src + hidden);
             qg[r][0] = a.x;
             qg[r][1] = a.y;
             qu[r][0] = b.x;
             qu[r][1] = b.y;
           } else {
-            qg[r][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
-            qu[r][0] = __ldg(reinterpret_cast<const uint32_t*>(src + hidden));
+            qg[r][0] = *reinterpret_cast<const uint32_t*>(src);
+            qu[r][0] = *reinterpret_cast<const uint32_t*>(src + hidden);
           }
-          dr[r] = ld_global_nc_v4(grad_h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC);
+          dr[r] = ld_global_stream_v4(grad_h + (r0 + r) * hidden + static_cast<int64_t>(cv) * VEC);
           const float* sp = scale + (r0 + r) * 2 * groups + cv / GT;
-          sg[r] = __ldg(sp);
-          su[r] = __ldg(sp + groups);
+          sg[r] = sp[0];
+          su[r] = sp[groups];
         }
       }
 #pragma unroll
@@ -666,7 +691,7 @@ extern "C" int hlm_quantize_rows(const void* x, void* q, float* scale, int64_t r
     LaunchScope scope(HLM_KERNEL_QUANT_ROWS, s);
     if (!launch_quant_rows_vec<T, false>(nullptr, static_cast<const T*>(x), nullptr, nullptr,
                                          static_cast<int8_t*>(q), scale, rows, static_cast<int>(cols), 0.0f, s))
-      quant_rows_scalar_kernel<T, false><<<quant_grid(rows, 8), 256, 0, s>>>(
+      launch_quant(quant_rows_scalar_kernel<T, false>, quant_grid(rows, 8), 256, s, 
         nullptr, static_cast<const T*>(x), nullptr, nullptr, static_cast<int8_t*>(q), scale, rows,
         static_cast<int>(cols), 0.0f);
   });
@@ -685,15 +710,15 @@ extern "C" int hlm_dequantize_rows(const void* q, const float* scale, void* out,
     const int grid = quant_grid((total + 16 / sizeof(T) - 1) / (16 / sizeof(T)), 4 * 256);
     if (cols >= 16 && host_aligned16(q) && host_aligned16(out)) {
       if (total < (1ll << 31))  // 32-bit division; a step past the end stays below 2^32
-        dequant_flat_kernel<T, uint32_t><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(q), scale,
+        launch_quant(dequant_flat_kernel<T, uint32_t>, grid, 256, s, static_cast<const int8_t*>(q), scale,
                                                               static_cast<T*>(out), static_cast<uint32_t>(total),
                                                               static_cast<uint32_t>(cols));
       else
-        dequant_flat_kernel<T, uint64_t><<<grid, 256, 0, s>>>(static_cast<const int8_t*>(q), scale,
+        launch_quant(dequant_flat_kernel<T, uint64_t>, grid, 256, s, static_cast<const int8_t*>(q), scale,
                                                               static_cast<T*>(out), static_cast<uint64_t>(total),
                                                               static_cast<uint64_t>(cols));
     } else
-      dequant_rows_scalar_kernel<T><<<quant_grid(rows, 8), 256, 0, s>>>(
+      launch_quant(dequant_rows_scalar_kernel<T>, quant_grid(rows, 8), 256, s, 
         static_cast<const int8_t*>(q), scale, static_cast<T*>(out), rows, static_cast<int>(cols));
   });
   return launch_status();
@@ -712,7 +737,7 @@ extern "C" int hlm_residual_rms_norm_q8(const void* residual, const void* branch
     if (!launch_quant_rows_vec<T, true>(static_cast<const T*>(residual), static_cast<const T*>(branch),
                                         static_cast<const T*>(weight), static_cast<T*>(out),
                                         static_cast<int8_t*>(q), scale, rows, static_cast<int>(cols), eps, s))
-      quant_rows_scalar_kernel<T, true><<<quant_grid(rows, 8), 256, 0, s>>>(
+      launch_quant(quant_rows_scalar_kernel<T, true>, quant_grid(rows, 8), 256, s, 
         static_cast<const T*>(residual), static_cast<const T*>(branch),
         static_cast<const T*>(weight), static_cast<T*>(out), static_cast<int8_t*>(q), scale, rows,
         static_cast<int>(cols), eps);
@@ -733,11 +758,11 @@ extern "C" int hlm_swiglu_ckpt8_fwd(const void* gate_up, void* h, void* q, float
     constexpr int VEC = 16 / sizeof(T);
     if (hidden % VEC == 0 && host_aligned16(gate_up) && host_aligned16(h) && host_aligned16(q)) {
       constexpr int R = 2;
-      swiglu_ckpt8_fwd_vec_kernel<T, R><<<quant_grid(rows, R), row_block(hidden / VEC), 0, s>>>(
+      launch_quant(swiglu_ckpt8_fwd_vec_kernel<T, R>, quant_grid(rows, R), row_block(hidden / VEC), s, 
           static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
           static_cast<int>(hidden / VEC), groups);
     } else
-      swiglu_ckpt8_fwd_scalar_kernel<T><<<quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), 0, s>>>(
+      launch_quant(swiglu_ckpt8_fwd_scalar_kernel<T>, quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), s, 
         static_cast<const T*>(gate_up), static_cast<T*>(h), static_cast<int8_t*>(q), scale, rows,
         static_cast<int>(hidden), groups);
   });
@@ -758,11 +783,11 @@ extern "C" int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const voi
     constexpr int VEC = 16 / sizeof(T);
     if (hidden % VEC == 0 && host_aligned16(grad_h) && host_aligned16(grad_gate_up) && host_aligned16(q)) {
       constexpr int R = 2;
-      swiglu_ckpt8_bwd_vec_kernel<T, R><<<quant_grid(rows, R), row_block(hidden / VEC), 0, s>>>(
+      launch_quant(swiglu_ckpt8_bwd_vec_kernel<T, R>, quant_grid(rows, R), row_block(hidden / VEC), s, 
           static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
           static_cast<T*>(grad_gate_up), rows, static_cast<int>(hidden / VEC), groups);
     } else
-      swiglu_ckpt8_bwd_scalar_kernel<T><<<quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), 0, s>>>(
+      launch_quant(swiglu_ckpt8_bwd_scalar_kernel<T>, quant_grid(rows, 1), row_block(32 * static_cast<int64_t>(groups)), s, 
         static_cast<const int8_t*>(q), scale, static_cast<const T*>(grad_h),
         static_cast<T*>(grad_gate_up), rows, static_cast<int>(hidden), groups);
   });

@@ -12,9 +12,9 @@
 // [32768 tokens, 4096, 768], where the read back costs 13 us once.
 //
 // Bound by the tensor cores (2 * tokens * N * K operations): at [32768, 4096, 768] bf16
-// 175 us back to back, of one call 129 us the GEMM (1.60 PFLOP/s, 96% of the measured
+// 165 us back to back, of one call 129 us the GEMM (1.60 PFLOP/s, 96% of the measured
 // burst), 13.5 us the read back and 8.5 us the sum of three partials; small gradients
-// ([1003, 520, 272] 12.7 us) are three launches' latency.  Few tiles: the tokens are
+// ([1003, 520, 272] 11.8 us) are three launches' latency.  Few tiles: the tokens are
 // split and each split writes an fp32 partial to the workspace; a third kernel adds the
 // partials in the order of the splits (the same bits every time) and rounds.
 #include "gemm_sm100.cuh"
@@ -78,6 +78,7 @@ struct EpiWeightGrad {
     int fp16;
   };
   static constexpr bool kRelaxedRelease = true;
+  static constexpr bool kDependentLaunch = true;
   template <int EPI_WARPS>
   static constexpr int smem_bytes() {
     return EPI_WARPS * 2048;
@@ -101,8 +102,10 @@ struct EpiWeightGrad {
 
 // Sum of the splits' partials in their order, rounded to T; eight elements per thread.
 template <typename T>
-__global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float* __restrict__ partial,
-                                                                   T* __restrict__ grad_w, int64_t n, int splits) {
+__global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float* partial,
+                                                                   T* grad_w, int64_t n, int splits) {
+  grid_launch_next();
+  grid_wait();
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x * 8) {
     float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -175,8 +178,9 @@ template <typename T>
 static int weight_grad_q8_reduce(const float* partial, void* grad_w, int64_t n, int splits, cudaStream_t s) {
   const int64_t blocks = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms_of_current_device()) * 16;
   LaunchScope scope(0, s);
-  weight_grad_q8_reduce_kernel<T><<<static_cast<int>(blocks < cap ? blocks : cap), 256, 0, s>>>(
-      partial, static_cast<T*>(grad_w), n, splits);
+  if (launch_dependent(weight_grad_q8_reduce_kernel<T>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)),
+                       dim3(256), 0, s, 1, partial, static_cast<T*>(grad_w), n, splits) != cudaSuccess)
+    return HLM_ERR_LAUNCH;
   return launch_status();
 }
 

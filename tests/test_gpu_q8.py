@@ -606,6 +606,61 @@ def test_captured_and_replayed_with_other_inputs(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(ob, expect_b))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_neighbours_of_other_kinds_in_the_stream(captured, cuda_device):
+    """The kernels are set up while the work before them in the stream still runs.  Whatever that is
+    (a copy, a fill, a torch kernel, a join of another stream) is waited for, and what follows waits
+    for them; run many times over the same buffers, eagerly and captured."""
+    from hackable_lm_b200 import kernels, ops
+
+    rows, cols = 3000, 768
+    src = [values((rows, cols), torch.bfloat16, seed=i).to(cuda_device) for i in range(4)]
+    w, ws = kernels.quantize_rows(values((384, cols), torch.bfloat16, seed=9).to(cuda_device))
+    x, r = torch.empty_like(src[0]), torch.empty_like(src[0])
+    side = torch.cuda.Stream()
+
+    def run(i):
+        main = torch.cuda.current_stream()
+        x.copy_(src[i % 4])                       # a device copy, then a kernel that reads it
+        r.fill_(0.5)                              # a fill
+        out, q, s = kernels.residual_rms_norm_q8(r, x, 1e-6)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y = kernels.linear_q8(q, s, w, ws)    # on another stream
+        main.wait_stream(side)
+        h, cq, cs = ops.swiglu_ckpt8(y)           # after the join
+        g = h.mul(2.0)                            # a torch kernel between two of the library's
+        x.zero_()                                 # overwrites what the first kernel read
+        grad = ops.swiglu_ckpt8_backward(cq, cs, g)
+        gw = ops.weight_grad_q8(grad, q, s)
+        few = kernels.linear_q8(q[:7], s[:7], w, ws, torch.float32)
+        back = kernels.dequantize_rows(q, s)
+        return [t.clone() for t in (out, y, h, grad, gw, few, back)]
+
+    torch.cuda.synchronize()
+    expect = []
+    for i in range(4):
+        expect.append(run(i))
+        torch.cuda.synchronize()
+    runs = []
+    if captured:
+        for i in range(4):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = run(i)
+            runs.append((graph, got))
+    for _ in range(20):
+        for i in range(4):
+            if captured:
+                runs[i][0].replay()
+                got = runs[i][1]
+            else:
+                got = run(i)
+            checks = [torch.equal(a, b) for a, b in zip(got, expect[i])] if _ % 5 == 4 else []
+            assert all(checks), (i, checks)
+    torch.cuda.synchronize()
+
+
 def test_backward_captured_while_an_eager_graph_lives(cuda_device):
     """The checkpoint operators' backward, captured with its forward on a side stream, beside an
     eager graph of the same leaves made on that stream.  (One made on the default stream keeps the
