@@ -6,13 +6,14 @@
 //
 // Every function returns None, and does nothing, when its tensors are not plain ones that
 // may go straight to the library: not on CUDA, a tensor subclass, wrapped by a transform,
-// under a dispatch mode, or with a gradient asked for.  The caller then goes through the
+// under a dispatch mode or torch.jit.trace, or with a gradient asked for.  The caller then goes through the
 // registered operator.  The entry points of libhlm_b200 are handed over by address
 // (set_entry_points), so that the one library that ctypes loaded is used.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -51,10 +52,14 @@ const at::Tensor* plain(PyObject* o) {
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.key_set().has_any(kWrapped)) return nullptr;
   if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+  // no operator here has a forward-mode derivative, and the registered ones would drop the tangent
+  TORCH_CHECK(!t._fw_grad(0).defined(), "hackable_lm_b200: the 8-bit operators have no forward-mode derivatives");
   return &t;
 }
 
-bool modes_active() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+bool modes_active() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::tracer::impl::is_dispatch_enabled();
+}
 
 int dtype_code(at::ScalarType t) {
   switch (t) {

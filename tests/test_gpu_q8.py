@@ -800,6 +800,35 @@ def test_modes_and_transforms_see_the_operators(cuda_device):
     assert torch.equal(q3, -q) and torch.equal(scale3, scale)
 
 
+def test_traced_operators_are_recorded(cuda_device):
+    """torch.jit.trace records the operators, not the values of the traced call."""
+    from hackable_lm_b200 import kernels
+
+    x, y = values((5, 64), torch.bfloat16, seed=1).to(cuda_device), values((5, 64), torch.bfloat16, seed=2).to(cuda_device)
+    traced = torch.jit.trace(lambda t: kernels.dequantize_rows(*kernels.quantize_rows(t)), x, check_trace=False)
+    assert torch.equal(traced(y), kernels.dequantize_rows(*kernels.quantize_rows(y)))
+
+
+def test_forward_mode_derivatives_are_refused(cuda_device):
+    """A tangent is never dropped in silence."""
+    import torch.autograd.forward_ad as fw
+
+    from hackable_lm_b200 import kernels, ops
+
+    x = values((4, 64), torch.bfloat16, seed=1).to(cuda_device)
+    w = values((16, 64), torch.bfloat16, seed=2).to(cuda_device)
+    q, scale = kernels.quantize_rows(x)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        ds = fw.make_dual(scale, torch.ones_like(scale))
+        for call in (lambda: kernels.quantize_rows(d), lambda: kernels.rms_norm_q8(d, None, 1e-6),
+                     lambda: kernels.residual_rms_norm_q8(x, d, 1e-6), lambda: kernels.dequantize_rows(q, ds),
+                     lambda: kernels.linear_q8(q, ds, q, scale), lambda: ops.swiglu_ckpt8(d),
+                     lambda: kernels.linear_ckpt8(d, w.requires_grad_(True))):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+
+
 @pytest.mark.parametrize("name", ["quantize_rows", "dequantize_rows", "rms_norm_q8", "residual_rms_norm_q8", "linear_q8",
                                   "swiglu_ckpt8", "swiglu_ckpt8_backward", "weight_grad_q8", "linear_ckpt8"])
 def test_opcheck(name, cuda_device):
