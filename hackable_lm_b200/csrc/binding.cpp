@@ -114,14 +114,25 @@ void check_rc(int rc, const char* name) {
     throw LibraryError{std::string(name) + " failed: " + p_strerror(rc) + " (code " + std::to_string(rc) + ")"};
 }
 
-// The current stream of t's device, which is made current for the scope.
+// The current stream of t's device, which is made current for the scope, with the
+// interpreter lock released: a launch waits while the stream's queue is full, and what it
+// waits for may be another Python thread's.  done() takes the lock again before a result
+// is made; an exception takes it on its way out.
 struct On {
   c10::cuda::OptionalCUDAGuard guard;
   void* stream;
+  PyThreadState* thread;
   explicit On(const at::Tensor& t) {
     if (c10::cuda::current_device() != t.get_device()) guard.set_device(t.device());
     stream = c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+    thread = PyEval_SaveThread();
   }
+  On(const On&) = delete;
+  void done() {
+    if (thread != nullptr) PyEval_RestoreThread(thread);
+    thread = nullptr;
+  }
+  ~On() { done(); }
 };
 
 template <class F>
@@ -175,6 +186,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_rc(p_quantize_rows(x.const_data_ptr(), q.data_ptr(), scale.data_ptr<float>(), scale.numel(), x.size(-1),
                              dtype_code(x.scalar_type()), on.stream),
              "hlm_quantize_rows");
+    on.done();
     return pack({q, scale});
   });
 }
@@ -194,6 +206,7 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
       check_rc(p_dequantize_rows(q.const_data_ptr(), scale.const_data_ptr<float>(), out.data_ptr(), scale.numel(),
                                  q.size(-1), code, on.stream),
                "hlm_dequantize_rows");
+    on.done();
     return THPVariable_Wrap(out);
   });
 }
@@ -227,6 +240,7 @@ PyObject* residual_rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                     q.data_ptr(), scale.data_ptr<float>(), scale.numel(), x.size(-1),
                                     static_cast<float>(eps), dtype_code(x.scalar_type()), on.stream),
              "hlm_residual_rms_norm_q8");
+    on.done();
     return has_r ? pack({out, q, scale}) : pack({q, scale});
   });
 }
@@ -249,6 +263,7 @@ PyObject* linear_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_rc(p_linear_q8(q.const_data_ptr(), scale.const_data_ptr<float>(), w.const_data_ptr(),
                          w_scale.const_data_ptr<float>(), out.data_ptr(), scale.numel(), N, K, code, on.stream),
              "hlm_linear_q8");
+    on.done();
     return THPVariable_Wrap(out);
   });
 }
@@ -276,6 +291,7 @@ PyObject* swiglu_ckpt8(PyObject*, PyObject* const* a, Py_ssize_t n) {
       check_rc(p_swiglu_ckpt8_fwd(x.const_data_ptr(), h.data_ptr(), q.data_ptr(), scale.data_ptr<float>(),
                                   h.numel() / hidden, hidden, code, on.stream),
                "hlm_swiglu_ckpt8_fwd");
+    on.done();
     return pack({h, q, scale});
   });
 }
@@ -300,6 +316,7 @@ PyObject* swiglu_ckpt8_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       check_rc(p_swiglu_ckpt8_bwd(q.const_data_ptr(), scale.const_data_ptr<float>(), g.const_data_ptr(),
                                   grad.data_ptr(), g.numel() / hidden, hidden, code, on.stream),
                "hlm_swiglu_ckpt8_bwd");
+    on.done();
     return THPVariable_Wrap(grad);
   });
 }
@@ -325,6 +342,7 @@ PyObject* weight_grad_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_rc(p_weight_grad_q8(g.const_data_ptr(), q.const_data_ptr(), scale.const_data_ptr<float>(), out.data_ptr(),
                               ws.data_ptr(), bytes, tokens, N, K, dtype_code(g.scalar_type()), on.stream),
              "hlm_weight_grad_q8");
+    on.done();
     return THPVariable_Wrap(out);
   });
 }

@@ -576,6 +576,30 @@ def test_side_stream_and_two_streams_at_once(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(ea, ga)) and all(torch.equal(p, q) for p, q in zip(eb, gb))
 
 
+def test_two_threads_at_once(cuda_device):
+    """The calls release the interpreter lock: threads with a stream each get their own results."""
+    import threading
+
+    runs = [_all_operators(cuda_device, seed)[0] for seed in (0, 50)]
+    expected = [run() for run in runs]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = runs[i]()
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for e, g in zip(expected, got):
+        assert g is not None and all(torch.equal(p, q) for p, q in zip(e, g))
+
+
 def test_captured_and_replayed_with_other_inputs(cuda_device):
     a, (x, r) = _all_operators(cuda_device, 0)
     b, _ = _all_operators(cuda_device, 50)
