@@ -308,7 +308,7 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     weight gradient in 8 bits by rows; the output and the gradient of x are those of F.linear."""
     _cuda_only(x, "linear_ckpt8")
     if not (torch.is_grad_enabled() and weight.requires_grad):
-        return F.linear(x, weight)  # no weight gradient: nothing of x to keep
+        return ops.linear_in_own_type(x, weight)  # no weight gradient: nothing of x to keep
     return ops.linear_ckpt8(x, weight)[0]
 
 

@@ -916,6 +916,6 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn_major: bool = False, b_mn_maj
 # ---------------------------------------------------------------------------
 from . import ops_q8 as _q8  # noqa: E402
 from .ops_q8 import (  # noqa: E402
-    dequantize_rows, linear_ckpt8, linear_ckpt8_supported, linear_q8, quantize_rows, residual_rms_norm_q8,
-    rms_norm_q8, swiglu_ckpt8, swiglu_ckpt8_backward, weight_grad_q8,
+    dequantize_rows, linear_ckpt8, linear_ckpt8_supported, linear_in_own_type, linear_q8, quantize_rows,
+    residual_rms_norm_q8, rms_norm_q8, swiglu_ckpt8, swiglu_ckpt8_backward, weight_grad_q8,
 )

@@ -274,6 +274,14 @@ def linear_ckpt8_supported(x: torch.Tensor, weight: torch.Tensor) -> bool:
             and weight.shape[1] % 16 == 0 and weight.numel() > 0)
 
 
+def linear_in_own_type(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """F.linear whose result has x's type, as the gradients do, whatever autocast's type is."""
+    if torch.is_autocast_enabled("cuda"):
+        with torch.autocast("cuda", enabled=False):
+            return torch.nn.functional.linear(x, weight)
+    return torch.nn.functional.linear(x, weight)
+
+
 @torch.library.custom_op("hackable_lm_b200::linear_ckpt8", mutates_args=())
 def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, q, scale): y = x @ weight^T, and x in 8 bits by rows, kept for the weight gradient
@@ -284,7 +292,7 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor) -> tuple[torch.Tensor, t
                            f"multiple of 8 and K of 16, got {x.dtype} {tuple(x.shape)}, {weight.dtype} "
                            f"{tuple(weight.shape)}")
     q, scale = _run("quantize_rows", x)
-    return torch.nn.functional.linear(x, weight), q, scale
+    return linear_in_own_type(x, weight), q, scale
 
 
 @linear_ckpt8.register_fake

@@ -800,6 +800,21 @@ def test_unsupported_sizes_raise_the_library_error(cuda_device):
         kernels.linear_ckpt8(g.float().requires_grad_(True), torch.zeros(8, 12, device=cuda_device, requires_grad=True))
 
 
+def test_linear_ckpt8_keeps_its_type_under_autocast(cuda_device):
+    from hackable_lm_b200 import kernels
+
+    x = values((20, 48), torch.bfloat16, seed=1).to(cuda_device).requires_grad_(True)
+    w = values((24, 48), torch.bfloat16, seed=2, scale=0.1).to(cuda_device).requires_grad_(True)
+    y = kernels.linear_ckpt8(x, w)
+    grads = torch.autograd.grad(y.sum(), (x, w))
+    with torch.autocast("cuda", dtype=torch.float16):
+        y2 = kernels.linear_ckpt8(x, w)
+        with torch.no_grad():
+            assert torch.equal(y, kernels.linear_ckpt8(x, w))
+    assert y2.dtype == torch.bfloat16 and torch.equal(y, y2)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(y2.sum(), (x, w))))
+
+
 def test_modes_and_transforms_see_the_operators(cuda_device):
     """Under a dispatch mode the registered operator runs (and is seen); the result is the same."""
     from torch.utils._python_dispatch import TorchDispatchMode
