@@ -13,6 +13,8 @@ model runs in bf16 only.
 """
 from __future__ import annotations
 
+import copy
+
 import torch
 import torch.nn.functional as F
 from torch import nn
@@ -43,8 +45,8 @@ class QuantizedBlock(nn.Module):
         qkv = block.attn.qkv
         self.n_head, self.n_kv_head, self.head_dim = qkv.n_head, qkv.n_kv_head, qkv.head_dim
         self.eps = block.mlp.down.norm_eps
-        self.rope = qkv.rope
-        self.attention = block.attn.attention
+        self.rope = copy.deepcopy(qkv.rope)
+        self.attention = copy.deepcopy(block.attn.attention)
         self.qkv_proj = Int8Linear(qkv.qkv_proj.weight)
         self.o_proj = Int8Linear(block.attn.out.o_proj.weight)
         self.gate_up_proj = Int8Linear(block.mlp.gate_up.gate_up_proj.weight)
@@ -68,15 +70,16 @@ class QuantizedBlock(nn.Module):
 class QuantizedLanguageModel(nn.Module):
     """``model.LanguageModel`` on 8-bit integer projections.  ``forward(idx, targets)`` returns
     what the model returns: (logits, None) without targets, else (None, mean loss over the
-    targets that are not ignore_index -100).  No gradients."""
+    targets that are not ignore_index -100).  No gradients.  It holds copies: training the model
+    further, or moving it, changes nothing here."""
 
     def __init__(self, model: nn.Module) -> None:
         super().__init__()
         for p in model.parameters():
             if not (p.is_cuda or p.is_meta):
                 raise RuntimeError("quantize_int8: the 8-bit operators run only on CUDA (sm_100a) tensors")
-        self.config = model.config
-        self.tok_emb = nn.Embedding.from_pretrained(model.tok_emb.weight.detach(), freeze=True)
+        self.config = copy.deepcopy(model.config)
+        self.tok_emb = nn.Embedding.from_pretrained(model.tok_emb.weight.detach().clone(), freeze=True)
         self.blocks = nn.ModuleList([QuantizedBlock(b) for b in model.blocks])
         self.lm_head = Int8Linear(model.lm_head.lm_head.weight)
         self.loss_rows = model.lm_head.chunk_size or 4096

@@ -76,6 +76,30 @@ def test_int8_model_weights_and_state(cuda_device):
     assert torch.equal(other(x)[0], quantized(x)[0])
 
 
+def test_int8_model_is_a_snapshot(cuda_device):
+    """What happens to the model afterwards does not reach the 8-bit one."""
+    model = _model(cuda_device, depth=2)
+    quantized = model.quantize_int8()
+    x, _ = _tokens(cuda_device)
+    before = quantized(x)[0]
+    with torch.no_grad():
+        for p in model.parameters():
+            p.mul_(0.5)
+    model.to("cpu")
+    assert torch.equal(quantized(x)[0], before)
+
+
+def test_int8_model_compiled(cuda_device):
+    """torch.compile of the 8-bit model runs the registered operators: the same bits where the
+    surrounding operations are the same kernels."""
+    quantized = _model(cuda_device, depth=2).quantize_int8()
+    x, _ = _tokens(cuda_device)
+    eager = quantized(x)[0]
+    compiled = torch.compile(quantized, fullgraph=True, dynamic=False)(x)[0]
+    assert compiled.shape == eager.shape and compiled.dtype == eager.dtype
+    assert torch.equal(compiled, eager)
+
+
 def test_int8_model_captured_and_replayed(cuda_device):
     quantized = _model(cuda_device, depth=2).quantize_int8()
     x, _ = _tokens(cuda_device, batch=1, length=16)
