@@ -652,7 +652,8 @@ HLM_DEVICE void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory");
 HLM_DEVICE void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Launch on `stream` as a dependent of the kernel before it, in clusters of `cluster` CTAs
-// along x (1: as the kernel declares).
+// along x (1: as the kernel declares).  A failure is the runtime's last error too, which
+// launch_status() returns and clears.
 template <class... Params, class... Args>
 inline cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                     int cluster, Args... args) {

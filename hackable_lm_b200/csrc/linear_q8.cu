@@ -533,15 +533,14 @@ static int linear_q8_split(const void* q, const float* scale, const void* w, con
   const int splits = (k_blocks + kb_per - 1) / kb_per;
   auto kern = linear_q8_split_kernel<T, MT>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
-    return HLM_ERR_LAUNCH;
+    return launch_status();
   // four outputs of a lane as one store
   const int vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
   {
     LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
-    if (launch_dependent(kern, dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles)),
-                         dim3(kSplitThreads), L::kBytes, s, splits, mw, mq, scale, w_scale, out, static_cast<int>(M),
-                         static_cast<int>(N), k_blocks, kb_per, vec, err) != cudaSuccess)
-      return HLM_ERR_LAUNCH;
+    (void)launch_dependent(kern, dim3(static_cast<unsigned>(n_tiles * splits), static_cast<unsigned>(m_tiles)),
+                           dim3(kSplitThreads), L::kBytes, s, splits, mw, mq, scale, w_scale, out, static_cast<int>(M),
+                           static_cast<int>(N), k_blocks, kb_per, vec, err);
   }
   return launch_status();
 }
@@ -559,10 +558,9 @@ static int linear_q8_rows(const void* q, const float* scale, const void* w, cons
   LaunchScope scope(HLM_KERNEL_LINEAR_Q8, s);
   const bool shared = K >= 2048 && (M == 1 || N <= 2048);
   const int64_t blocks = shared ? (N + R - 1) / R : (N + R * kRowsWarps - 1) / (R * kRowsWarps);
-  if (launch_dependent(shared ? linear_q8_rows_kernel<T, MR, R, kRowsWarps> : linear_q8_rows_kernel<T, MR, R, 1>,
-                       dim3(static_cast<unsigned>(blocks)), dim3(32 * kRowsWarps), 0, s, 1, qp, scale, wp, w_scale, out,
-                       static_cast<int>(M), static_cast<int>(N), static_cast<int>(K)) != cudaSuccess)
-    return HLM_ERR_LAUNCH;
+  (void)launch_dependent(shared ? linear_q8_rows_kernel<T, MR, R, kRowsWarps> : linear_q8_rows_kernel<T, MR, R, 1>,
+                         dim3(static_cast<unsigned>(blocks)), dim3(32 * kRowsWarps), 0, s, 1, qp, scale, wp, w_scale, out,
+                         static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
   return launch_status();
 }
 

@@ -178,9 +178,8 @@ template <typename T>
 static int weight_grad_q8_reduce(const float* partial, void* grad_w, int64_t n, int splits, cudaStream_t s) {
   const int64_t blocks = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms_of_current_device()) * 16;
   LaunchScope scope(0, s);
-  if (launch_dependent(weight_grad_q8_reduce_kernel<T>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)),
-                       dim3(256), 0, s, 1, partial, static_cast<T*>(grad_w), n, splits) != cudaSuccess)
-    return HLM_ERR_LAUNCH;
+  (void)launch_dependent(weight_grad_q8_reduce_kernel<T>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)),
+                         dim3(256), 0, s, 1, partial, static_cast<T*>(grad_w), n, splits);
   return launch_status();
 }
 
