@@ -4,7 +4,7 @@
 //
 // Two passes: the codes are read back once to the gradient's type (q * scale in fp32,
 // rounded once: the tensor cores take one 16-bit type for both operands) into the
-// workspace, and a CTA-pair tcgen05 GEMM (256 x 256 tiles of grad_w, both operands
+// workspace, and a CTA-pair tcgen05 GEMM (256 x 256 or 256 x 128 tiles of grad_w, both operands
 // MN-major, tokens as the reduction) multiplies.  Making the operand inside the GEMM,
 // by converter warps from codes in shared memory, was built and measured first: every
 // row of tiles then converts the codes again, and the converters' shared-memory traffic
@@ -14,7 +14,7 @@
 // Bound by the tensor cores (2 * tokens * N * K operations): at [32768, 4096, 768] bf16
 // 165 us back to back, of one call 129 us the GEMM (1.60 PFLOP/s, 96% of the measured
 // burst), 13.5 us the read back and 8.5 us the sum of three partials; small gradients
-// ([1003, 520, 272] 11.8 us) are three launches' latency.  Few tiles: the tokens are
+// ([1003, 520, 272] 10.6 us) are two or three launches' latency.  Few tiles: the tokens are
 // split and each split writes an fp32 partial to the workspace; a third kernel adds the
 // partials in the order of the splits (the same bits every time) and rounds.
 #include "gemm_sm100.cuh"
@@ -28,7 +28,7 @@ constexpr int kWgEpiWarps = 8;
 // Write every `parts`-th 32-column group, from `part` on, of a warp's 32 accumulator rows as
 // O (fp32 partial or the 16-bit result): staged in a 32 x 64-byte box (16-byte chunks swizzled by row
 // pairs), out in 16-byte stores, eight 64-byte row segments per instruction.
-template <typename O>
+template <typename O, int GROUPS>
 HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, int cols, uint32_t taddr,
                               uint32_t buf, int lane, int part, int parts) {
   constexpr int kCols = 64 / static_cast<int>(sizeof(O));  // columns of a box: 16 fp32 or 32 16-bit
@@ -36,7 +36,7 @@ HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, 
   if (row0 >= rows) return;
   const uint32_t sw = static_cast<uint32_t>(lane >> 1) & 3u;
 #pragma unroll 1
-  for (int g = part; g < 8; g += parts) {
+  for (int g = part; g < GROUPS; g += parts) {
     if (col0 + 32 * g >= cols) break;
     uint32_t a[32];
     tmem_ld_32x32b_x32(taddr + static_cast<uint32_t>(g * 32), a);
@@ -86,17 +86,18 @@ struct EpiWeightGrad {
   template <int BN, int kParts>
   static HLM_DEVICE void run(const Params& ep, const GemmParams& p, uint8_t* smem, uint32_t taddr, int m_tile,
                              int n_tile, int split, int quad, int part, int lane) {
-    static_assert(BN == 256, "eight 32-column groups");
+    constexpr int kGroups = BN / 32;
     const uint32_t buf = smem_u32(smem) + static_cast<uint32_t>(part * 4 + quad) * 2048u;
     const int row0 = m_tile * kBM + quad * 32;
     if (ep.partial != nullptr)
-      wg_store_tile(ep.partial + static_cast<int64_t>(split) * p.M * p.N, p.N, row0, p.M, n_tile * BN, p.N, taddr,
-                    buf, lane, part, kParts);
+      wg_store_tile<float, kGroups>(ep.partial + static_cast<int64_t>(split) * p.M * p.N, p.N, row0, p.M, n_tile * BN,
+                                    p.N, taddr, buf, lane, part, kParts);
     else if (ep.fp16)
-      wg_store_tile(static_cast<__half*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N, taddr, buf, lane, part, kParts);
+      wg_store_tile<__half, kGroups>(static_cast<__half*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N, taddr, buf, lane,
+                                     part, kParts);
     else
-      wg_store_tile(static_cast<__nv_bfloat16*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N, taddr, buf, lane, part,
-                    kParts);
+      wg_store_tile<__nv_bfloat16, kGroups>(static_cast<__nv_bfloat16*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N,
+                                            taddr, buf, lane, part, kParts);
   }
 };
 
@@ -128,24 +129,34 @@ __global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float*
   }
 }
 
-// Splits of the tokens: the number that the cost in microseconds is least for, of
-// rounds of pair tiles at 0.42 us per 64 tokens (the measured rate) and 1.5 us to fill
-// and drain, and, with partials, a second launch (2.5 us) and 8 bytes per partial
-// element at 7 TB/s (most of it L2).
-static int weight_grad_q8_splits(int64_t tokens, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + 255) / 256) * ((K + 255) / 256);
+// Tile width and splits of the tokens: the pair that the cost in microseconds is least for,
+// of rounds of pair tiles at 0.28 us (256 x 128) or 0.33 us (256 x 256) per 64 tokens and 1 us to fill
+// and drain, and, with partials, another launch (2.5 us, 3.5 of the host's time) and 8 bytes per partial element at
+// 7 TB/s (most of it L2).  Within 6% of the best of all pairs at sixteen sizes measured, and
+// for all but three the best: [1003, 520, 272] 128 columns x 1 split 10.6 us, 128 x 4 9.9, 256 x 8 11.8;
+// [4096, 768, 768] 128 x 4 15.9, 256 x 8 17.5; [8192, 2304, 768] 256 x 2 36.7, 128 x 4 44.9;
+// [2048, 2304, 768] 128 x 1 18.4, 128 x 2 22.5.
+struct WgPlan {
+  int bn;  // 256 x bn tiles
+  int splits;
+};
+static WgPlan weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K) {
   const int64_t pairs = num_sms_of_current_device() / 2;
   const int64_t kb = (tokens + kBK - 1) / kBK;
-  int best = 1;
+  WgPlan best = {256, 1};
   double best_us = 1e30;
-  for (int s = 1; s <= 32 && s <= kb; ++s) {
-    const int64_t per = (kb + s - 1) / s;
-    if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
-    double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (0.42 * static_cast<double>(per) + 1.5);
-    if (s > 1) us += 2.5 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
-    if (us < best_us) {
-      best_us = us;
-      best = s;
+  for (int bn = 128; bn <= 256; bn += 128) {
+    const int64_t tiles = ((N + 255) / 256) * ((K + bn - 1) / bn);
+    const double block = bn == 256 ? 0.33 : 0.28;
+    for (int s = 1; s <= 32 && s <= kb; ++s) {
+      const int64_t per = (kb + s - 1) / s;
+      if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
+      double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (block * static_cast<double>(per) + 1.0);
+      if (s > 1) us += 3.5 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
+      if (us < best_us) {
+        best_us = us;
+        best = {bn, s};
+      }
     }
   }
   return best;
@@ -156,13 +167,13 @@ static size_t weight_grad_q8_back_bytes(int64_t tokens, int64_t K) {
   return (static_cast<size_t>(tokens) * static_cast<size_t>(K) * 2 + 255) / 256 * 256;
 }
 
-template <class Kind>
+template <class Kind, int BN>
 static int weight_grad_q8_gemm(const void* grad, const void* back, void* grad_w, float* partial, int fp16,
                                int64_t tokens, int64_t N, int64_t K, int splits, cudaStream_t s) {
   CUtensorMap ma, mb;  // both [tokens][features]: boxes of 64 features x 64 tokens
   if (!encode_map(&ma, grad, 2, N, tokens, N, 64) || !encode_map(&mb, back, 2, K, tokens, K, 64)) return HLM_ERR_DRIVER;
   GemmParams p;
-  gemm_tiling_pair(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), 256, splits);
+  gemm_tiling_pair(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), BN, splits);
   if (static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits > (1ll << 30)) return HLM_ERR_UNSUPPORTED;
   p.err = device_error_ptr();
   if (p.err == nullptr) return HLM_ERR_LAUNCH;
@@ -170,7 +181,7 @@ static int weight_grad_q8_gemm(const void* grad, const void* back, void* grad_w,
   ep.out = grad_w;
   ep.partial = p.splits > 1 ? partial : nullptr;
   ep.fp16 = fp16;
-  return launch_gemm_pair<256, kWgStages, true, true, EpiWeightGrad, kWgEpiWarps, Kind>(
+  return launch_gemm_pair<BN, kWgStages, true, true, EpiWeightGrad, kWgEpiWarps, Kind>(
       ma, ma, ma, mb, p, ep, s, HLM_KERNEL_WEIGHT_GRAD_Q8);
 }
 
@@ -189,7 +200,7 @@ using namespace hlm;
 
 extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, int64_t K) {
   if (tokens <= 0 || N <= 0 || K <= 0) return 0;
-  const int splits = weight_grad_q8_splits(tokens, N, K);
+  const int splits = weight_grad_q8_plan(tokens, N, K).splits;
   const size_t part = splits > 1 ? static_cast<size_t>(splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4 : 0;
   return weight_grad_q8_back_bytes(tokens, K) + part;
 }
@@ -215,13 +226,15 @@ extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* 
   const size_t need = hlm_weight_grad_q8_workspace_bytes(tokens, N, K);
   if (workspace == nullptr || workspace_bytes < need) return HLM_ERR_WORKSPACE;
   if (!host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
-  const int splits = weight_grad_q8_splits(tokens, N, K);
+  const WgPlan plan = weight_grad_q8_plan(tokens, N, K);
+  const int splits = plan.splits;
   float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + weight_grad_q8_back_bytes(tokens, K));
   const int fp16 = dtype == HLM_F16;
   int rc = hlm_dequantize_rows(q, scale, workspace, tokens, K, dtype, stream);
   if (rc != HLM_OK) return rc;
-  rc = fp16 ? weight_grad_q8_gemm<KindF16>(grad, workspace, grad_w, partial, fp16, tokens, N, K, splits, s)
-            : weight_grad_q8_gemm<KindBf16>(grad, workspace, grad_w, partial, fp16, tokens, N, K, splits, s);
+  auto gemm = plan.bn == 128 ? (fp16 ? weight_grad_q8_gemm<KindF16, 128> : weight_grad_q8_gemm<KindBf16, 128>)
+                             : (fp16 ? weight_grad_q8_gemm<KindF16, 256> : weight_grad_q8_gemm<KindBf16, 256>);
+  rc = gemm(grad, workspace, grad_w, partial, fp16, tokens, N, K, splits, s);
   if (rc != HLM_OK || splits == 1) return rc;
   return fp16 ? weight_grad_q8_reduce<__half>(partial, grad_w, N * K, splits, s)
               : weight_grad_q8_reduce<__nv_bfloat16>(partial, grad_w, N * K, splits, s);

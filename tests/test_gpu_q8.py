@@ -449,6 +449,14 @@ def test_weight_grad_q8(tokens, N, K, dtype, cuda_device):
     _check_wgrad(values((tokens, N), dtype, seed=N, scale=0.1), q, scale, cuda_device)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,N,K", [(1000, 2048, 2064), (4090, 2304, 768), (130, 8, 4096)])
+def test_weight_grad_q8_wide_tiles_and_splits(tokens, N, K, dtype, cuda_device):
+    """Sizes of the 256 x 256 tiles, whole and with the tokens split, and of a row of narrow ones."""
+    q, scale = codes((tokens, K), seed=tokens)
+    _check_wgrad(values((tokens, N), dtype, seed=N, scale=0.1), q, scale, cuda_device)
+
+
 def test_weight_grad_q8_same_bits_every_time(cuda_device):
     from hackable_lm_b200 import ops
 
