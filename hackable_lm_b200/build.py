@@ -87,7 +87,7 @@ def _build_binding(force: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare", "-DNDEBUG",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(arg for inc in includes for arg in ("-isystem", inc)), str(BINDING_SRC), "-o", str(tmp),
-           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+           f"-L{lib_dir}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"binding build failed:\n{proc.stdout}\n{proc.stderr}")

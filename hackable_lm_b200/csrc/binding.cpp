@@ -2,7 +2,7 @@
 // checks, output allocation and the C ABI call of one operator in one C call.
 //
 // The kernels of a few tokens run for 2 us; the same steps in Python with ctypes cost
-// 10 to 18 us a call, here about 3 beside the launch itself.
+// 10 to 18 us a call, here 0.6 to 2 beside the launch itself (2.5).
 //
 // Every function returns None, and does nothing, when its tensors are not plain ones that
 // may go straight to the library: not on CUDA, a tensor subclass, wrapped by a transform,
@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -87,6 +88,11 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> o
 at::Tensor packed(const at::Tensor& t) {
   at::Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+// An uninitialised tensor on t's device (at::empty less its way through the dispatcher, 0.3 us of each).
+at::Tensor fresh(const at::Tensor& t, c10::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
 }
 
 std::vector<int64_t> with_last(const at::Tensor& t, int64_t last) {
@@ -181,8 +187,8 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_cols("quantize_rows", *x0);
     On on(*x0);
     const at::Tensor x = x0->contiguous();
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    at::Tensor q = fresh(x, x.sizes(), at::kChar);
+    at::Tensor scale = fresh(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
     check_rc(p_quantize_rows(x.const_data_ptr(), q.data_ptr(), scale.data_ptr<float>(), scale.numel(), x.size(-1),
                              dtype_code(x.scalar_type()), on.stream),
              "hlm_quantize_rows");
@@ -201,7 +207,7 @@ PyObject* dequantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     same_device(*q0, {s0});
     On on(*q0);
     const at::Tensor q = q0->contiguous(), scale = s0->contiguous();
-    at::Tensor out = at::empty(q.sizes(), q.options().dtype(dtype_of(code)));
+    at::Tensor out = fresh(q, q.sizes(), dtype_of(code));
     if (q.numel() > 0)
       check_rc(p_dequantize_rows(q.const_data_ptr(), scale.const_data_ptr<float>(), out.data_ptr(), scale.numel(),
                                  q.size(-1), code, on.stream),
@@ -232,9 +238,9 @@ PyObject* residual_rms_norm_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor x = x0->contiguous();
     const at::Tensor r = has_r ? r0->contiguous() : at::Tensor();
     const at::Tensor w = has_w ? w0->to(x.scalar_type()).contiguous() : at::Tensor();
-    at::Tensor out = has_r ? at::empty(x.sizes(), x.options()) : at::Tensor();
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    at::Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    at::Tensor out = has_r ? fresh(x, x.sizes(), x.scalar_type()) : at::Tensor();
+    at::Tensor q = fresh(x, x.sizes(), at::kChar);
+    at::Tensor scale = fresh(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
     check_rc(p_residual_rms_norm_q8(has_r ? r.const_data_ptr() : nullptr, x.const_data_ptr(),
                                     has_w ? w.const_data_ptr() : nullptr, has_r ? out.data_ptr() : nullptr,
                                     q.data_ptr(), scale.data_ptr<float>(), scale.numel(), x.size(-1),
@@ -259,7 +265,7 @@ PyObject* linear_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     On on(*q0);
     const at::Tensor q = packed(*q0), w = packed(*w0), scale = s0->contiguous(), w_scale = t0->contiguous();
     const int64_t N = w.size(0), K = w.size(1);
-    at::Tensor out = at::empty(with_last(q, N), q.options().dtype(dtype_of(code)));
+    at::Tensor out = fresh(q, with_last(q, N), dtype_of(code));
     check_rc(p_linear_q8(q.const_data_ptr(), scale.const_data_ptr<float>(), w.const_data_ptr(),
                          w_scale.const_data_ptr<float>(), out.data_ptr(), scale.numel(), N, K, code, on.stream),
              "hlm_linear_q8");
@@ -284,9 +290,9 @@ PyObject* swiglu_ckpt8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t hidden = check_gate_up("swiglu_ckpt8", *x0);
     On on(*x0);
     const at::Tensor x = x0->contiguous();
-    at::Tensor h = at::empty(with_last(x, hidden), x.options());
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    at::Tensor scale = at::empty(with_last(x, scale_cols(hidden)), x.options().dtype(at::kFloat));
+    at::Tensor h = fresh(x, with_last(x, hidden), x.scalar_type());
+    at::Tensor q = fresh(x, x.sizes(), at::kChar);
+    at::Tensor scale = fresh(x, with_last(x, scale_cols(hidden)), at::kFloat);
     if (hidden > 0)
       check_rc(p_swiglu_ckpt8_fwd(x.const_data_ptr(), h.data_ptr(), q.data_ptr(), scale.data_ptr<float>(),
                                   h.numel() / hidden, hidden, code, on.stream),
@@ -311,7 +317,7 @@ PyObject* swiglu_ckpt8_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     same_device(*q0, {s0, g0});
     On on(*q0);
     const at::Tensor q = q0->contiguous(), scale = s0->contiguous(), g = g0->contiguous();
-    at::Tensor grad = at::empty(q.sizes(), g.options());
+    at::Tensor grad = fresh(g, q.sizes(), g.scalar_type());
     if (hidden > 0)
       check_rc(p_swiglu_ckpt8_bwd(q.const_data_ptr(), scale.const_data_ptr<float>(), g.const_data_ptr(),
                                   grad.data_ptr(), g.numel() / hidden, hidden, code, on.stream),
@@ -336,9 +342,9 @@ PyObject* weight_grad_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     On on(*g0);
     const at::Tensor g = packed(*g0), q = packed(*q0), scale = s0->contiguous();
     const int64_t tokens = scale.numel(), N = g.size(-1), K = q.size(-1);
-    at::Tensor out = at::empty({N, K}, g.options());
+    at::Tensor out = fresh(g, {N, K}, g.scalar_type());
     const size_t bytes = p_weight_grad_q8_workspace_bytes(tokens, N, K);
-    at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, g.options().dtype(at::kByte));
+    at::Tensor ws = fresh(g, {static_cast<int64_t>(bytes)}, at::kByte);
     check_rc(p_weight_grad_q8(g.const_data_ptr(), q.const_data_ptr(), scale.const_data_ptr<float>(), out.data_ptr(),
                               ws.data_ptr(), bytes, tokens, N, K, dtype_code(g.scalar_type()), on.stream),
              "hlm_weight_grad_q8");
