@@ -18,9 +18,9 @@
 // Measured (bf16 out, weights out of L2): one token [4096, 768] 2.0 us, [8192, 8192]
 // 12.7 us (5.3 TB/s of weights); [24, 768, 2048] 3.0 us; [777, 1111, 1360] 7.9 us;
 // [32768, 4096, 768] 94 us, 2.2 POP/s and 2.9 TB/s of output (110 us once the power cap
-// holds the clock at 1.4 GHz).  That case takes 78 us without its stores and 92 us without
-// the conversions from int32: the output's stores beside the operands' loads hold it,
-// not the tensor cores, which reach 2.9 POP/s at [8192, 8192, 8192].  Launched as
+// holds the clock at 1.4 GHz).  That case takes 66 us without its epilogue (3.1 POP/s), 79
+// with it but for the stores, 94 to 96 whole: the output's way out holds it, not the tensor
+// cores, which reach 2.9 POP/s at [8192, 8192, 8192].  Launched as
 // dependents of the kernel before: [24, 768, 2048] 3.7 -> 3.0 us, [1024, 4096, 768]
 // 8.1 -> 7.0.
 #include <atomic>
