@@ -72,6 +72,15 @@ template <class E>
 struct epi_dependent<E, std::void_t<decltype(E::kDependentLaunch)>>
     : std::integral_constant<bool, E::kDependentLaunch> {};
 
+// Epilogues of GEMMs whose B operand is the sum of two tensors, hi + lo, of A's type declare
+// `static constexpr bool kSplitB = true` (pair kernel, both operands MN-major, BN <= 256): a
+// stage holds a block of A and those of hi (the B map) and lo (the A1 map, which has no
+// segment to serve then), and each step of K multiplies A by both.
+template <class E, class = void>
+struct epi_split_b : std::false_type {};
+template <class E>
+struct epi_split_b<E, std::void_t<decltype(E::kSplitB)>> : std::integral_constant<bool, E::kSplitB> {};
+
 // Epilogues that read per-row or per-column values from global memory declare a struct
 // `Early` and `load_early`: the pair kernel calls it before it waits for the tile's
 // accumulator, and hands the struct to `run`.
@@ -362,11 +371,11 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
 // drains its own 128 accumulator rows from its own TMEM.  Per SM this halves
 // the B traffic into shared memory for the same MMA rate.
 // ---------------------------------------------------------------------------
-template <int BN, int STAGES>
+template <int BN, int STAGES, bool SPLIT_B = false>
 struct PairSmem {
   static constexpr int kABytes = kBM * kBK * 2;       // this CTA's 128 A rows
   static constexpr int kBBytes = (BN / 2) * kBK * 2;  // this CTA's half of B
-  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStageBytes = kABytes + (SPLIT_B ? 2 : 1) * kBBytes;
   static constexpr int kBarOffset = STAGES * kStageBytes;
   static constexpr int kNumBars = 2 * STAGES + 4;
   static constexpr int kTmemSlotOffset = kBarOffset + kNumBars * 8;
@@ -387,7 +396,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
                      const __grid_constant__ CUtensorMap tmA2,
                      const __grid_constant__ CUtensorMap tmB, const GemmParams p,
                      const __grid_constant__ typename Epi::Params ep) {
-  using L = PairSmem<BN, STAGES>;
+  constexpr bool kSplitB = epi_split_b<Epi>::value;
+  static_assert(!kSplitB || (A_MN && B_MN && BN <= 256), "a split B");
+  using L = PairSmem<BN, STAGES, kSplitB>;
   static_assert(EPI_WARPS == 4 || EPI_WARPS == 8, "4 or 8 epilogue warps");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -418,10 +429,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
     if constexpr (epi_has_init<Epi>::value) Epi::init(base_ptr + L::kEpiOffset);
     fence_mbar_init();
     prefetch_tensormap(&tmA0);
-    if (p.a_seg1 > 0) {
-      prefetch_tensormap(&tmA1);
-      prefetch_tensormap(&tmA2);
-    }
+    if (kSplitB || p.a_seg1 > 0) prefetch_tensormap(&tmA1);
+    if (p.a_seg1 > 0) prefetch_tensormap(&tmA2);
     prefetch_tensormap(&tmB);
   }
   if (warp == 1) {
@@ -494,6 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
               tma_load_2d_pair(sb + i * 8192u, &tmB, k0, nb0 + 64 * i, full);
             else
               tma_load_2d_pair(sb + i * 8192u, &tmB, nb0 + 64 * i, k0, full);
+            if constexpr (kSplitB) tma_load_2d_pair(sb + L::kBBytes + i * 8192u, &tmA1, nb0 + 64 * i, k0, full);
           }
           if constexpr (L::kN1 > 0) {
             const int nb1 = n_tile * BN + L::kN0 + static_cast<int>(rank) * (L::kN1 / 2);
@@ -555,6 +565,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
                                         : make_sw128_desc(sb + kk * 32u, 16u, 1024u);
             const uint32_t accum = (kb > kb0 || kk > 0) ? 1u : 0u;
             Kind::mma_pair(d_tmem, adesc, bdesc, idesc0, accum);
+            if constexpr (kSplitB)
+              Kind::mma_pair(d_tmem, adesc, make_sw128_desc(sb + L::kBBytes + kk * 2048u, 8192u, 1024u), idesc0, 1u);
             if constexpr (L::kN1 > 0) {
               // second MMA: columns [256, BN); its B half starts after the first's
               constexpr uint32_t off = static_cast<uint32_t>(L::kN0 / 2) * 128u;
@@ -719,7 +731,7 @@ template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4
 int launch_gemm_pair(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                      const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                      cudaStream_t stream, int kernel_id) {
-  using L = PairSmem<BN, STAGES>;
+  using L = PairSmem<BN, STAGES, epi_split_b<Epi>::value>;
   auto kern = gemm_pair_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,

@@ -2,27 +2,29 @@
 //
 //   grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m])
 //
-// Two passes: the codes are read back once to the gradient's type (q * scale in fp32,
-// rounded once: the tensor cores take one 16-bit type for both operands) into the
-// workspace, and a CTA-pair tcgen05 GEMM (256 x 256 or 256 x 128 tiles of grad_w, both operands
-// MN-major, tokens as the reduction) multiplies.  Making the operand inside the GEMM,
-// by converter warps from codes in shared memory, was built and measured first: every
-// row of tiles then converts the codes again, and the converters' shared-memory traffic
-// (their reads and writes beside the MMA's) held the tensor cores back: 206 us at
-// [32768 tokens, 4096, 768], where the read back costs 13 us once.
+// Two passes: the codes are read back once to the workspace, as two values of the gradient's
+// type (the tensor cores take one 16-bit type for both operands): x = q * scale in fp32 is cut
+// into hi, its leading 8 or 11 bits, and lo, the rest rounded, so that hi + lo is x to within
+// 2^-15 (bf16) or 2^-21 (fp16) of it.  A CTA-pair tcgen05 GEMM (256 x 256 or 256 x 128 tiles of
+// grad_w, both operands MN-major, tokens as the reduction) multiplies each block of the gradient
+// by both.  One rounded value in place of the two halves the products, but rounds as coarsely
+// as the result itself: the error against 64 bits is then 1.4 times that of the exact result
+// rounded once, with the two it is that.
+// Making the operand inside the GEMM, by converter warps from codes in shared memory, was built
+// first (with one value: 206 us at [32768 tokens, 4096, 768] against 165): every row of tiles
+// then converts the codes again, and the converters' shared-memory traffic (their reads and
+// writes beside the MMA's) holds the tensor cores back.
 //
-// Bound by the tensor cores (2 * tokens * N * K operations): at [32768, 4096, 768] bf16
-// 165 us back to back, of one call 129 us the GEMM (1.60 PFLOP/s, 96% of the measured
-// burst), 13.5 us the read back and 8.5 us the sum of three partials; small gradients
-// ([1003, 520, 272] 10.6 us) are two or three launches' latency.  Few tiles: the tokens are
-// split and each split writes an fp32 partial to the workspace; a third kernel adds the
-// partials in the order of the splits (the same bits every time) and rounds.
+// Bound by the tensor cores (4 * tokens * N * K operations): [32768, 4096, 768] bf16 277 us a call
+// at full clock (1.49 PFLOP/s over the whole call), 333 at the power cap; small gradients
+// ([1003, 520, 272] 11.2 us, [64, 1024, 1024] 8.6) are their launches' latency.  Few tiles: the
+// tokens are split and each split writes an fp32 partial to the workspace; a third kernel adds
+// the partials in the order of the splits (the same bits every time) and rounds.
 #include "gemm_sm100.cuh"
 #include "quant_common.cuh"
 
 namespace hlm {
 
-constexpr int kWgStages = 6;
 constexpr int kWgEpiWarps = 8;
 
 // Write every `parts`-th 32-column group, from `part` on, of a warp's 32 accumulator rows as
@@ -71,6 +73,70 @@ HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, 
   }
 }
 
+// x as two values of type T: hi, x cut towards zero, and lo, the rest.  The rest is exact in
+// fp32 and rounded to T.  Both have the sign of x, and lo is not zero unless x is (a rest of
+// zero becomes 2^-24 of x, or fp16's smallest value), so that an infinite gradient times
+// either is the same infinity.
+template <typename T>
+HLM_DEVICE void split_value(float x, float& hi, float& lo);
+template <>
+HLM_DEVICE void split_value<__nv_bfloat16>(float x, float& hi, float& lo) {
+  hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  lo = x - hi;
+  if (lo == 0.0f) lo = x * 5.9604644775390625e-8f;
+  if (!isfinite(x)) hi = lo = x;
+}
+template <>
+HLM_DEVICE void split_value<__half>(float x, float& hi, float& lo) {
+  hi = __half2float(__float2half_rz(x));
+  lo = __half2float(__float2half_rn(x - hi));
+  if (lo == 0.0f && x != 0.0f) lo = copysignf(5.9604644775390625e-8f, x);
+  if (!isfinite(x)) hi = lo = x;
+}
+
+// The codes read back as hi and lo; a thread takes eight consecutive codes (of one row: K is
+// a multiple of 16), four such steps of a block in flight.
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) weight_grad_q8_split_kernel(const int8_t* q, const float* scale, T* hi, T* lo,
+                                                                  I total, I cols) {
+  grid_launch_next();
+  grid_wait();
+  constexpr int U = 4;
+  constexpr I kSpan = 256 * 8;
+  for (I e0 = static_cast<I>(blockIdx.x) * (U * kSpan) + threadIdx.x * 8; e0 < total;
+       e0 += static_cast<I>(gridDim.x) * (U * kSpan)) {
+    uint2 w[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const I e = e0 + u * kSpan;
+      if (e < total) {
+        w[u] = *reinterpret_cast<const uint2*>(q + e);
+        s[u] = scale[e / cols];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const I e = e0 + u * kSpan;
+      if (e >= total) break;
+      F2 f[4], a[4], b[4];
+      codes_to_f2(w[u].x, f[0], f[1]);
+      codes_to_f2(w[u].y, f[2], f[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x0, x1, h0, h1, l0, l1;
+        f2_split(f[i] * f2(s[u]), x0, x1);
+        split_value<T>(x0, h0, l0);
+        split_value<T>(x1, h1, l1);
+        a[i] = f2(h0, h1);
+        b[i] = f2(l0, l1);
+      }
+      st_global_v4(hi + e, f2_store<T>(a));
+      st_global_v4(lo + e, f2_store<T>(b));
+    }
+  }
+}
+
 struct EpiWeightGrad {
   struct Params {
     void* out;       // grad_w [N][K], 16-bit
@@ -79,6 +145,7 @@ struct EpiWeightGrad {
   };
   static constexpr bool kRelaxedRelease = true;
   static constexpr bool kDependentLaunch = true;
+  static constexpr bool kSplitB = true;
   template <int EPI_WARPS>
   static constexpr int smem_bytes() {
     return EPI_WARPS * 2048;
@@ -130,12 +197,12 @@ __global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float*
 }
 
 // Tile width and splits of the tokens: the pair that the cost in microseconds is least for,
-// of rounds of pair tiles at 0.28 us (256 x 128) or 0.33 us (256 x 256) per 64 tokens and 1 us to fill
-// and drain, and, with partials, another launch (2.5 us, 3.5 of the host's time) and 8 bytes per partial element at
-// 7 TB/s (most of it L2).  Within 6% of the best of all pairs at sixteen sizes measured, and
-// for all but three the best: [1003, 520, 272] 128 columns x 1 split 10.6 us, 128 x 4 9.9, 256 x 8 11.8;
-// [4096, 768, 768] 128 x 4 15.9, 256 x 8 17.5; [8192, 2304, 768] 256 x 2 36.7, 128 x 4 44.9;
-// [2048, 2304, 768] 128 x 1 18.4, 128 x 2 22.5.
+// of rounds of pair tiles at 0.47 us (256 x 128) or 0.70 us (256 x 256) per 64 tokens and 1 us to fill
+// and drain, and, with partials, 2 us of another launch (less than its 3.5 us alone, since it
+// overlaps) and 8 bytes per partial element at 7 TB/s (most of it L2).  Within 6% of the best of
+// all pairs at fifteen sizes measured, [1003, 520, 272] apart (128 columns x 8 splits 11.5 to
+// 14 us, x 4 11.2, x 1 16.4): [4096, 768, 768] 128 x 4 20.7, 256 x 8 21.7; [8192, 2304, 768] 256 x 5 52.4,
+// 128 x 4 60.5; [2048, 2304, 768] 128 x 1 22.3, 128 x 4 27.9.
 struct WgPlan {
   int bn;  // 256 x bn tiles
   int splits;
@@ -147,12 +214,12 @@ static WgPlan weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K) {
   double best_us = 1e30;
   for (int bn = 128; bn <= 256; bn += 128) {
     const int64_t tiles = ((N + 255) / 256) * ((K + bn - 1) / bn);
-    const double block = bn == 256 ? 0.33 : 0.28;
+    const double block = bn == 256 ? 0.70 : 0.47;
     for (int s = 1; s <= 32 && s <= kb; ++s) {
       const int64_t per = (kb + s - 1) / s;
       if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
       double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (block * static_cast<double>(per) + 1.0);
-      if (s > 1) us += 3.5 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
+      if (s > 1) us += 2.0 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
       if (us < best_us) {
         best_us = us;
         best = {bn, s};
@@ -162,16 +229,18 @@ static WgPlan weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K) {
   return best;
 }
 
-// Workspace: the input read back, then the partials.
+// Workspace: the input read back, hi and lo (each of this many bytes), then the partials.
 static size_t weight_grad_q8_back_bytes(int64_t tokens, int64_t K) {
   return (static_cast<size_t>(tokens) * static_cast<size_t>(K) * 2 + 255) / 256 * 256;
 }
 
 template <class Kind, int BN>
-static int weight_grad_q8_gemm(const void* grad, const void* back, void* grad_w, float* partial, int fp16,
+static int weight_grad_q8_gemm(const void* grad, const void* hi, const void* lo, void* grad_w, float* partial, int fp16,
                                int64_t tokens, int64_t N, int64_t K, int splits, cudaStream_t s) {
-  CUtensorMap ma, mb;  // both [tokens][features]: boxes of 64 features x 64 tokens
-  if (!encode_map(&ma, grad, 2, N, tokens, N, 64) || !encode_map(&mb, back, 2, K, tokens, K, 64)) return HLM_ERR_DRIVER;
+  CUtensorMap ma, mh, ml;  // all [tokens][features]: boxes of 64 features x 64 tokens
+  if (!encode_map(&ma, grad, 2, N, tokens, N, 64) || !encode_map(&mh, hi, 2, K, tokens, K, 64) ||
+      !encode_map(&ml, lo, 2, K, tokens, K, 64))
+    return HLM_ERR_DRIVER;
   GemmParams p;
   gemm_tiling_pair(p, static_cast<int>(N), static_cast<int>(K), static_cast<int>(tokens), BN, splits);
   if (static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits > (1ll << 30)) return HLM_ERR_UNSUPPORTED;
@@ -181,8 +250,28 @@ static int weight_grad_q8_gemm(const void* grad, const void* back, void* grad_w,
   ep.out = grad_w;
   ep.partial = p.splits > 1 ? partial : nullptr;
   ep.fp16 = fp16;
-  return launch_gemm_pair<BN, kWgStages, true, true, EpiWeightGrad, kWgEpiWarps, Kind>(
-      ma, ma, ma, mb, p, ep, s, HLM_KERNEL_WEIGHT_GRAD_Q8);
+  constexpr int kStages = BN == 256 ? 4 : 6;  // of 48 and 32 KB
+  return launch_gemm_pair<BN, kStages, true, true, EpiWeightGrad, kWgEpiWarps, Kind>(
+      ma, ml, ma, mh, p, ep, s, HLM_KERNEL_WEIGHT_GRAD_Q8);
+}
+
+template <typename T>
+static int weight_grad_q8_split(const void* q, const float* scale, void* hi, void* lo, int64_t tokens, int64_t K,
+                                cudaStream_t s) {
+  const int64_t total = tokens * K;
+  const int64_t blocks = (total + 4 * 2048 - 1) / (4 * 2048);
+  const int64_t cap = static_cast<int64_t>(num_sms_of_current_device()) * 64;
+  const dim3 grid(static_cast<unsigned>(blocks < cap ? blocks : cap));
+  const int8_t* qp = static_cast<const int8_t*>(q);
+  T *hp = static_cast<T*>(hi), *lp = static_cast<T*>(lo);
+  LaunchScope scope(HLM_KERNEL_DEQUANT_ROWS, s);
+  if (total < (1ll << 31))  // 32-bit division; a step past the end stays below 2^32
+    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint32_t>, grid, dim3(256), 0, s, 1, qp, scale, hp, lp,
+                           static_cast<uint32_t>(total), static_cast<uint32_t>(K));
+  else
+    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint64_t>, grid, dim3(256), 0, s, 1, qp, scale, hp, lp,
+                           static_cast<uint64_t>(total), static_cast<uint64_t>(K));
+  return launch_status();
 }
 
 template <typename T>
@@ -202,7 +291,7 @@ extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, 
   if (tokens <= 0 || N <= 0 || K <= 0) return 0;
   const int splits = weight_grad_q8_plan(tokens, N, K).splits;
   const size_t part = splits > 1 ? static_cast<size_t>(splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4 : 0;
-  return weight_grad_q8_back_bytes(tokens, K) + part;
+  return 2 * weight_grad_q8_back_bytes(tokens, K) + part;
 }
 
 extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
@@ -228,13 +317,16 @@ extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* 
   if (!host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
   const WgPlan plan = weight_grad_q8_plan(tokens, N, K);
   const int splits = plan.splits;
-  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + weight_grad_q8_back_bytes(tokens, K));
+  uint8_t* hi = static_cast<uint8_t*>(workspace);
+  uint8_t* lo = hi + weight_grad_q8_back_bytes(tokens, K);
+  float* partial = reinterpret_cast<float*>(lo + weight_grad_q8_back_bytes(tokens, K));
   const int fp16 = dtype == HLM_F16;
-  int rc = hlm_dequantize_rows(q, scale, workspace, tokens, K, dtype, stream);
+  int rc = fp16 ? weight_grad_q8_split<__half>(q, scale, hi, lo, tokens, K, s)
+                : weight_grad_q8_split<__nv_bfloat16>(q, scale, hi, lo, tokens, K, s);
   if (rc != HLM_OK) return rc;
   auto gemm = plan.bn == 128 ? (fp16 ? weight_grad_q8_gemm<KindF16, 128> : weight_grad_q8_gemm<KindBf16, 128>)
                              : (fp16 ? weight_grad_q8_gemm<KindF16, 256> : weight_grad_q8_gemm<KindBf16, 256>);
-  rc = gemm(grad, workspace, grad_w, partial, fp16, tokens, N, K, splits, s);
+  rc = gemm(grad, hi, lo, grad_w, partial, fp16, tokens, N, K, splits, s);
   if (rc != HLM_OK || splits == 1) return rc;
   return fp16 ? weight_grad_q8_reduce<__half>(partial, grad_w, N * K, splits, s)
               : weight_grad_q8_reduce<__nv_bfloat16>(partial, grad_w, N * K, splits, s);

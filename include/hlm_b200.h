@@ -419,10 +419,10 @@ int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const void* grad_h, 
 
 /* Weight gradient of y = x w^T from x held in 8 bits by rows:
  * grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m]), the values read back
- * rounded once to dtype, fp32 sums in a fixed order (the same bits every time),
- * rounded to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16 (dtype), q int8
+ * held in two values of dtype (to 2^-15 of each in bf16, 2^-21 in fp16), fp32 sums
+ * in a fixed order (the same bits every time), rounded once to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16 (dtype), q int8
  * [tokens, K], 16-byte aligned; N a multiple of 8, K of 16.  tokens == 0 writes
- * zeros.  Workspace bytes from the query (the values read back, 2 * tokens * K
+ * zeros.  Workspace bytes from the query (the values read back, 4 * tokens * K
  * bytes, and fp32 partial sums where the tokens are split), 16-byte aligned. */
 int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
                        void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N, int64_t K,

@@ -457,6 +457,59 @@ def test_weight_grad_q8_wide_tiles_and_splits(tokens, N, K, dtype, cuda_device):
     _check_wgrad(values((tokens, N), dtype, seed=N, scale=0.1), q, scale, cuda_device)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,N,K", [(1, 24, 48), (2, 264, 272), (63, 24, 16), (65, 520, 2064), (130, 2048, 2304)])
+def test_weight_grad_q8_keeps_the_bits_of_what_it_reads_back(tokens, N, K, dtype, cuda_device):
+    """The values read back are not rounded to the gradient's type: they are held in two of its
+    values, the first cut (within eps of it), the rest rounded, which leaves eps * E of it, and
+    in fp16 at most its smallest value.  Their product with fp32 (U), the sum of 2 m terms, the
+    result's rounding."""
+    from hackable_lm_b200 import ops
+
+    q, scale = codes((tokens, K), seed=tokens)
+    grad = values((tokens, N), dtype, seed=N, scale=0.1)
+    y = ops.weight_grad_q8(grad.to(cuda_device), q.to(cuda_device), scale.to(cuda_device))
+    e = quant8.weight_grad_q8(grad, q, scale)
+    size = grad.double().abs().t() @ quant8.read_back(q, scale).abs()
+    E = half_step(dtype)
+    sub = grad.double().abs().sum(dim=0).unsqueeze(1) * 2 * half_subnormal(dtype)
+    bound = size * (2 * E * E + (2 * tokens + 4) * U) + sub
+    assert_within(y, e, bound + (e.abs() + bound) * E + half_subnormal(dtype), "grad_w")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,N,K", [(1003, 520, 272), (4096, 256, 128), (4090, 768, 2048)])
+def test_weight_grad_q8_is_as_exact_as_its_result_can_be(tokens, N, K, dtype, cuda_device):
+    """Over all elements, the error against 64 bits is that of the exact result rounded once: what the
+    operands and the sum add is 2^-7 of a half step of the result and less (5% is allowed for)."""
+    from hackable_lm_b200 import ops
+
+    q, scale = codes((tokens, K), seed=tokens)
+    grad = values((tokens, N), dtype, seed=N, scale=0.1)
+    e = quant8.weight_grad_q8(grad, q, scale)
+    y = ops.weight_grad_q8(grad.to(cuda_device), q.to(cuda_device), scale.to(cuda_device)).cpu().double()
+    assert float((y - e).norm()) <= 1.05 * float((e.to(dtype).double() - e).norm())
+
+
+def test_weight_grad_q8_infinite_gradients(cuda_device):
+    """An infinity in the gradient gives infinities of the products' signs, not NaN, and NaN where
+    the value read back is zero; with scales whose values one 16-bit number holds, too."""
+    from hackable_lm_b200 import ops
+
+    for dtype in (torch.bfloat16, torch.float16):
+        q, scale = codes((40, 32), seed=1)
+        scale[3:5] = 0.25
+        grad = values((40, 16), dtype, seed=2)
+        grad[3, 5], grad[4, 6] = float("inf"), float("-inf")
+        q[3, 7] = 0
+        q[4, :8] = 1
+        y = ops.weight_grad_q8(grad.to(cuda_device), q.to(cuda_device), scale.to(cuda_device)).cpu()
+        e = quant8.weight_grad_q8(grad, q, scale).to(dtype)
+        assert torch.equal(torch.isnan(y), torch.isnan(e)) and torch.equal(torch.isinf(y), torch.isinf(e))
+        bad = torch.isinf(e)
+        assert torch.equal(y[bad], e[bad])
+
+
 def test_weight_grad_q8_same_bits_every_time(cuda_device):
     from hackable_lm_b200 import ops
 
