@@ -28,11 +28,11 @@ namespace hlm {
 constexpr int kWgEpiWarps = 8;
 
 // Write every `parts`-th 32-column group, from `part` on, of a warp's 32 accumulator rows as
-// O (fp32 partial or the 16-bit result): staged in a 32 x 64-byte box (16-byte chunks swizzled by row
+// O (fp32 partial, or the 16-bit result, times `up`): staged in a 32 x 64-byte box (16-byte chunks swizzled by row
 // pairs), out in 16-byte stores, eight 64-byte row segments per instruction.
 template <typename O, int GROUPS>
 HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, int cols, uint32_t taddr,
-                              uint32_t buf, int lane, int part, int parts) {
+                              uint32_t buf, int lane, int part, int parts, float up) {
   constexpr int kCols = 64 / static_cast<int>(sizeof(O));  // columns of a box: 16 fp32 or 32 16-bit
   constexpr int kPerChunk = 16 / static_cast<int>(sizeof(O));
   if (row0 >= rows) return;
@@ -55,7 +55,7 @@ HLM_DEVICE void wg_store_tile(O* dst, int64_t ld, int row0, int rows, int col0, 
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            w[i] = pack2<O>(__uint_as_float(a[8 * c + 2 * i]), __uint_as_float(a[8 * c + 2 * i + 1]));
+            w[i] = pack2<O>(__uint_as_float(a[8 * c + 2 * i]) * up, __uint_as_float(a[8 * c + 2 * i + 1]) * up);
           v = make_uint4(w[0], w[1], w[2], w[3]);
         }
         st_shared_v4(buf + static_cast<uint32_t>(lane * 64) + ((static_cast<uint32_t>(c) ^ sw) << 4), v);
@@ -94,13 +94,55 @@ HLM_DEVICE void split_value<__half>(float x, float& hi, float& lo) {
   if (!isfinite(x)) hi = lo = x;
 }
 
-// The codes read back as hi and lo; a thread takes eight consecutive codes (of one row: K is
-// a multiple of 16), four such steps of a block in flight.
-template <typename T, typename I>
-__global__ void __launch_bounds__(256) weight_grad_q8_split_kernel(const int8_t* q, const float* scale, T* hi, T* lo,
-                                                                  I total, I cols) {
+// fp16 holds less than the scales' range (the codes may be those of wider values: fp32 rows,
+// whole tensors of tiny ones).  Its values read back are therefore held times a power of two
+// that puts the largest scale into [2^7, 2^8), their largest magnitude below 2^15, and the
+// sums are multiplied by its inverse in fp32.  What is off by its subnormal steps is then off
+// by at most 2^-39 of the largest value that the scales allow.
+
+// The largest finite magnitude among n floats, by the block's 256 threads.
+HLM_DEVICE float block_max_finite(const float* v, int64_t n) {
+  __shared__ uint32_t sh[8];
+  uint32_t m = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 256) {
+    const uint32_t b = mag_bits(v[i]);
+    if (b < kInfBits) m = max(m, b);
+  }
+  m = warp_max_u32(m);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, sh[i]);
+  return __uint_as_float(m);
+}
+constexpr int kScalePart = 1024;  // scales that every block of the next kernel may read itself
+constexpr int kScaleBlocks = 128;
+
+// Partial maxima of more of them.
+__global__ void __launch_bounds__(256) weight_grad_q8_scale_max_kernel(const float* scale, int64_t tokens, int64_t per,
+                                                                      float* maxima) {
   grid_launch_next();
   grid_wait();
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * per;
+  const float m = block_max_finite(scale + i0, min(per, tokens - i0));
+  if (threadIdx.x == 0) maxima[blockIdx.x] = m;
+}
+
+// The codes read back as hi and lo; a thread takes eight consecutive codes (of one row: K is
+// a multiple of 16), four such steps of a block in flight.  fp16: `maxima` holds the scales or
+// maxima of them, and *up gets the factor of the sums.
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) weight_grad_q8_split_kernel(const int8_t* q, const float* scale,
+                                                                  const float* maxima, int n_maxima, float* up, T* hi,
+                                                                  T* lo, I total, I cols) {
+  grid_launch_next();
+  grid_wait();
+  float down = 1.0f;
+  if constexpr (std::is_same_v<T, __half>) {
+    const uint32_t e = max(__float_as_uint(block_max_finite(maxima, n_maxima)) >> 23, 8u);  // biased exponent
+    down = __uint_as_float((127u + 7u + 127u - e) << 23);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *up = __uint_as_float((e - 7u) << 23);
+  }
   constexpr int U = 4;
   constexpr I kSpan = 256 * 8;
   for (I e0 = static_cast<I>(blockIdx.x) * (U * kSpan) + threadIdx.x * 8; e0 < total;
@@ -112,7 +154,7 @@ __global__ void __launch_bounds__(256) weight_grad_q8_split_kernel(const int8_t*
       const I e = e0 + u * kSpan;
       if (e < total) {
         w[u] = *reinterpret_cast<const uint2*>(q + e);
-        s[u] = scale[e / cols];
+        s[u] = scale[e / cols] * down;
       }
     }
 #pragma unroll
@@ -141,6 +183,7 @@ struct EpiWeightGrad {
   struct Params {
     void* out;       // grad_w [N][K], 16-bit
     float* partial;  // or fp32 partials [splits][N][K]
+    const float* up;  // the sums' factor (fp16)
     int fp16;
   };
   static constexpr bool kRelaxedRelease = true;
@@ -158,22 +201,24 @@ struct EpiWeightGrad {
     const int row0 = m_tile * kBM + quad * 32;
     if (ep.partial != nullptr)
       wg_store_tile<float, kGroups>(ep.partial + static_cast<int64_t>(split) * p.M * p.N, p.N, row0, p.M, n_tile * BN,
-                                    p.N, taddr, buf, lane, part, kParts);
+                                    p.N, taddr, buf, lane, part, kParts, 1.0f);
     else if (ep.fp16)
       wg_store_tile<__half, kGroups>(static_cast<__half*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N, taddr, buf, lane,
-                                     part, kParts);
+                                     part, kParts, *ep.up);
     else
       wg_store_tile<__nv_bfloat16, kGroups>(static_cast<__nv_bfloat16*>(ep.out), p.N, row0, p.M, n_tile * BN, p.N,
-                                            taddr, buf, lane, part, kParts);
+                                            taddr, buf, lane, part, kParts, 1.0f);
   }
 };
 
-// Sum of the splits' partials in their order, rounded to T; eight elements per thread.
+// Sum of the splits' partials in their order, times *up (fp16), rounded to T; eight elements per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float* partial,
-                                                                   T* grad_w, int64_t n, int splits) {
+                                                                   T* grad_w, int64_t n, int splits,
+                                                                   const float* up) {
   grid_launch_next();
   grid_wait();
+  const float factor = std::is_same_v<T, __half> ? *up : 1.0f;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x * 8) {
     float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -190,6 +235,8 @@ __global__ void __launch_bounds__(256) weight_grad_q8_reduce_kernel(const float*
       f[6] += b.z;
       f[7] += b.w;
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] *= factor;
     Vec16<T> o;
     o.from_float(f);
     st_global_v4(grad_w + i, o.raw);
@@ -229,13 +276,17 @@ static WgPlan weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K) {
   return best;
 }
 
-// Workspace: the input read back, hi and lo (each of this many bytes), then the partials.
+// Workspace: the sums' factor and the scales' maxima, the input read back, hi and lo (each of
+// this many bytes), then the partials.
+constexpr size_t kWgHeadBytes = (1 + kScaleBlocks) * sizeof(float) + 252;
+static_assert(kWgHeadBytes % 256 == 0, "what follows stays aligned");
 static size_t weight_grad_q8_back_bytes(int64_t tokens, int64_t K) {
   return (static_cast<size_t>(tokens) * static_cast<size_t>(K) * 2 + 255) / 256 * 256;
 }
 
 template <class Kind, int BN>
-static int weight_grad_q8_gemm(const void* grad, const void* hi, const void* lo, void* grad_w, float* partial, int fp16,
+static int weight_grad_q8_gemm(const void* grad, const void* hi, const void* lo, void* grad_w, float* partial,
+                               const float* up, int fp16,
                                int64_t tokens, int64_t N, int64_t K, int splits, cudaStream_t s) {
   CUtensorMap ma, mh, ml;  // all [tokens][features]: boxes of 64 features x 64 tokens
   if (!encode_map(&ma, grad, 2, N, tokens, N, 64) || !encode_map(&mh, hi, 2, K, tokens, K, 64) ||
@@ -249,6 +300,7 @@ static int weight_grad_q8_gemm(const void* grad, const void* hi, const void* lo,
   EpiWeightGrad::Params ep;
   ep.out = grad_w;
   ep.partial = p.splits > 1 ? partial : nullptr;
+  ep.up = up;
   ep.fp16 = fp16;
   constexpr int kStages = BN == 256 ? 4 : 6;  // of 48 and 32 KB
   return launch_gemm_pair<BN, kStages, true, true, EpiWeightGrad, kWgEpiWarps, Kind>(
@@ -256,8 +308,18 @@ static int weight_grad_q8_gemm(const void* grad, const void* hi, const void* lo,
 }
 
 template <typename T>
-static int weight_grad_q8_split(const void* q, const float* scale, void* hi, void* lo, int64_t tokens, int64_t K,
-                                cudaStream_t s) {
+static int weight_grad_q8_split(const void* q, const float* scale, float* head, void* hi, void* lo, int64_t tokens,
+                                int64_t K, cudaStream_t s) {
+  const float* maxima = scale;
+  int64_t n_maxima = tokens;
+  if (std::is_same_v<T, __half> && tokens > kScalePart) {
+    const int64_t least = (tokens + kScaleBlocks - 1) / kScaleBlocks, per = least > kScalePart ? least : kScalePart;
+    n_maxima = (tokens + per - 1) / per;
+    LaunchScope scope(0, s);
+    (void)launch_dependent(weight_grad_q8_scale_max_kernel, dim3(static_cast<unsigned>(n_maxima)), dim3(256), 0, s, 1,
+                           scale, tokens, per, head + 1);
+    maxima = head + 1;
+  }
   const int64_t total = tokens * K;
   const int64_t blocks = (total + 4 * 2048 - 1) / (4 * 2048);
   const int64_t cap = static_cast<int64_t>(num_sms_of_current_device()) * 64;
@@ -266,20 +328,23 @@ static int weight_grad_q8_split(const void* q, const float* scale, void* hi, voi
   T *hp = static_cast<T*>(hi), *lp = static_cast<T*>(lo);
   LaunchScope scope(HLM_KERNEL_DEQUANT_ROWS, s);
   if (total < (1ll << 31))  // 32-bit division; a step past the end stays below 2^32
-    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint32_t>, grid, dim3(256), 0, s, 1, qp, scale, hp, lp,
+    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint32_t>, grid, dim3(256), 0, s, 1, qp, scale,
+                           maxima, static_cast<int>(n_maxima), head, hp, lp,
                            static_cast<uint32_t>(total), static_cast<uint32_t>(K));
   else
-    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint64_t>, grid, dim3(256), 0, s, 1, qp, scale, hp, lp,
+    (void)launch_dependent(weight_grad_q8_split_kernel<T, uint64_t>, grid, dim3(256), 0, s, 1, qp, scale,
+                           maxima, static_cast<int>(n_maxima), head, hp, lp,
                            static_cast<uint64_t>(total), static_cast<uint64_t>(K));
   return launch_status();
 }
 
 template <typename T>
-static int weight_grad_q8_reduce(const float* partial, void* grad_w, int64_t n, int splits, cudaStream_t s) {
+static int weight_grad_q8_reduce(const float* partial, void* grad_w, int64_t n, int splits, const float* up,
+                                 cudaStream_t s) {
   const int64_t blocks = (n / 8 + 255) / 256, cap = static_cast<int64_t>(num_sms_of_current_device()) * 16;
   LaunchScope scope(0, s);
   (void)launch_dependent(weight_grad_q8_reduce_kernel<T>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)),
-                         dim3(256), 0, s, 1, partial, static_cast<T*>(grad_w), n, splits);
+                         dim3(256), 0, s, 1, partial, static_cast<T*>(grad_w), n, splits, up);
   return launch_status();
 }
 
@@ -291,7 +356,7 @@ extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, 
   if (tokens <= 0 || N <= 0 || K <= 0) return 0;
   const int splits = weight_grad_q8_plan(tokens, N, K).splits;
   const size_t part = splits > 1 ? static_cast<size_t>(splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4 : 0;
-  return 2 * weight_grad_q8_back_bytes(tokens, K) + part;
+  return kWgHeadBytes + 2 * weight_grad_q8_back_bytes(tokens, K) + part;
 }
 
 extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
@@ -317,17 +382,18 @@ extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* 
   if (!host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
   const WgPlan plan = weight_grad_q8_plan(tokens, N, K);
   const int splits = plan.splits;
-  uint8_t* hi = static_cast<uint8_t*>(workspace);
+  float* head = static_cast<float*>(workspace);
+  uint8_t* hi = static_cast<uint8_t*>(workspace) + kWgHeadBytes;
   uint8_t* lo = hi + weight_grad_q8_back_bytes(tokens, K);
   float* partial = reinterpret_cast<float*>(lo + weight_grad_q8_back_bytes(tokens, K));
   const int fp16 = dtype == HLM_F16;
-  int rc = fp16 ? weight_grad_q8_split<__half>(q, scale, hi, lo, tokens, K, s)
-                : weight_grad_q8_split<__nv_bfloat16>(q, scale, hi, lo, tokens, K, s);
+  int rc = fp16 ? weight_grad_q8_split<__half>(q, scale, head, hi, lo, tokens, K, s)
+                : weight_grad_q8_split<__nv_bfloat16>(q, scale, head, hi, lo, tokens, K, s);
   if (rc != HLM_OK) return rc;
   auto gemm = plan.bn == 128 ? (fp16 ? weight_grad_q8_gemm<KindF16, 128> : weight_grad_q8_gemm<KindBf16, 128>)
                              : (fp16 ? weight_grad_q8_gemm<KindF16, 256> : weight_grad_q8_gemm<KindBf16, 256>);
-  rc = gemm(grad, hi, lo, grad_w, partial, fp16, tokens, N, K, splits, s);
+  rc = gemm(grad, hi, lo, grad_w, partial, head, fp16, tokens, N, K, splits, s);
   if (rc != HLM_OK || splits == 1) return rc;
-  return fp16 ? weight_grad_q8_reduce<__half>(partial, grad_w, N * K, splits, s)
-              : weight_grad_q8_reduce<__nv_bfloat16>(partial, grad_w, N * K, splits, s);
+  return fp16 ? weight_grad_q8_reduce<__half>(partial, grad_w, N * K, splits, head, s)
+              : weight_grad_q8_reduce<__nv_bfloat16>(partial, grad_w, N * K, splits, head, s);
 }

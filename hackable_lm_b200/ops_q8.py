@@ -263,7 +263,7 @@ def weight_grad_q8(grad: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> 
     """grad^T @ (q * scale) [N, K]: the weight gradient of a projection from its input in 8 bits
     (grad [..., N] bf16 or fp16, q int8 [..., K] with a scale for each row; N a multiple of 8, K of 16).
     The values read back are held in two values of grad's type (to 2^-15 of each in bf16, 2^-21 in
-    fp16), the sums in fp32; the result is rounded once.  Takes 4 bytes of workspace for each code."""
+    fp16, whatever the scales' size, or 2^-39 of the largest value), the sums in fp32; the result is rounded once.  Takes 4 bytes of workspace for each code."""
     out = None if _compiling() else _lib.binding().weight_grad_q8(grad, q, scale)
     return _weight_grad_q8_op(grad, q, scale) if out is None else out
 

@@ -419,8 +419,10 @@ int hlm_swiglu_ckpt8_bwd(const void* q, const float* scale, const void* grad_h, 
 
 /* Weight gradient of y = x w^T from x held in 8 bits by rows:
  * grad_w[n, k] = sum_m grad[m, n] * (q[m, k] * scale[m]), the values read back
- * held in two values of dtype (to 2^-15 of each in bf16, 2^-21 in fp16), fp32 sums
- * in a fixed order (the same bits every time), rounded once to dtype.  grad [tokens, N], grad_w [N, K] bf16 or fp16 (dtype), q int8
+ * held in two values of dtype (to 2^-15 of each in bf16, 2^-21 in fp16, or 2^-39 of
+ * the largest), fp32 sums in a fixed order (the same bits every time), rounded once
+ * to dtype.  Scales of any size: fp16 values are held times a power of two that
+ * brings the largest finite scale into its range.  grad [tokens, N], grad_w [N, K] bf16 or fp16 (dtype), q int8
  * [tokens, K], 16-byte aligned; N a multiple of 8, K of 16.  tokens == 0 writes
  * zeros.  Workspace bytes from the query (the values read back, 4 * tokens * K
  * bytes, and fp32 partial sums where the tokens are split), 16-byte aligned. */

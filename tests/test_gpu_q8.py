@@ -491,6 +491,39 @@ def test_weight_grad_q8_is_as_exact_as_its_result_can_be(tokens, N, K, dtype, cu
     assert float((y - e).norm()) <= 1.05 * float((e.to(dtype).double() - e).norm())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [50, 3000, 200000])
+@pytest.mark.parametrize("least,most,reach", [(2.0 ** 4, 2.0 ** 11, 2.0 ** -12), (2.0 ** -40, 2.0 ** -30, 2.0 ** 13),
+                                              (2.0 ** -20, 2.0 ** 5, 2.0 ** -4), (2.0 ** -117, 2.0 ** -110, 2.0 ** 15),
+                                              (2.0 ** 105, 2.0 ** 120, 2.0 ** -14)])
+def test_weight_grad_q8_scales_outside_the_gradients_type(least, most, reach, tokens, dtype, cuda_device):
+    """Codes may stand for values that the gradient's type cannot hold (fp16: over 65504, or below
+    2^-24).  Their product with the gradient counts all the same: each value is off as it is
+    elsewhere, and in fp16 by at most 2^-24 of a unit that is 2^-7 of the largest scale's power
+    of two.  Results beyond the type are infinities there, as for any rounding."""
+    from hackable_lm_b200 import ops
+
+    g = torch.Generator().manual_seed(tokens)
+    q, _ = codes((tokens, 16), seed=tokens)
+    scale = least * (most / least) ** torch.rand(tokens, generator=g, dtype=torch.float64)
+    scale = scale.clamp(max=most).float()
+    scale[tokens // 2] = most
+    grad = (torch.randn(tokens, 8, generator=g) * reach / tokens ** 0.5).to(dtype)
+    y = ops.weight_grad_q8(grad.to(cuda_device), q.to(cuda_device), scale.to(cuda_device)).cpu().double()
+    e = quant8.weight_grad_q8(grad, q, scale)
+    size = grad.double().abs().t() @ quant8.read_back(q, scale).abs()
+    E = half_step(dtype)
+    unit = most * 2.0 ** -7 if dtype == torch.float16 else 0.0
+    bound = size * (2 * E * E + (2 * tokens + 4) * U) + grad.double().abs().sum(dim=0).unsqueeze(1) * unit * 2.0 ** -24
+    most_out = torch.finfo(dtype).max
+    inside = e.abs() + bound <= most_out
+    beyond = e.abs() - bound >= most_out * (1 + E)
+    err = (y - e).abs()
+    assert bool((err <= bound + (e.abs() + bound) * E + half_subnormal(dtype))[inside].all()), float((err - bound)[inside].max())
+    assert torch.equal(y[beyond], e[beyond].sign() * float("inf"))
+    assert bool((inside | beyond).any())
+
+
 def test_weight_grad_q8_infinite_gradients(cuda_device):
     """An infinity in the gradient gives infinities of the products' signs, not NaN, and NaN where
     the value read back is zero; with scales whose values one 16-bit number holds, too."""
