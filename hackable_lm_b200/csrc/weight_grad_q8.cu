@@ -256,17 +256,19 @@ struct WgPlan {
 };
 static WgPlan weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K) {
   const int64_t pairs = num_sms_of_current_device() / 2;
-  const int64_t kb = (tokens + kBK - 1) / kBK;
+  const int kb = static_cast<int>((tokens + kBK - 1) / kBK);
+  const double part_us = static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
   WgPlan best = {256, 1};
   double best_us = 1e30;
   for (int bn = 128; bn <= 256; bn += 128) {
     const int64_t tiles = ((N + 255) / 256) * ((K + bn - 1) / bn);
     const double block = bn == 256 ? 0.70 : 0.47;
     for (int s = 1; s <= 32 && s <= kb; ++s) {
-      const int64_t per = (kb + s - 1) / s;
+      const double extra = s > 1 ? 2.0 + s * part_us : 0.0;
+      if (extra >= best_us) break;
+      const int per = (kb + s - 1) / s;
       if ((kb + per - 1) / per != s) continue;  // the same blocks with fewer splits
-      double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (block * static_cast<double>(per) + 1.0);
-      if (s > 1) us += 2.0 + static_cast<double>(s) * static_cast<double>(N) * static_cast<double>(K) * 8.0 / 7.0e6;
+      const double us = static_cast<double>((tiles * s + pairs - 1) / pairs) * (block * per + 1.0) + extra;
       if (us < best_us) {
         best_us = us;
         best = {bn, s};
@@ -352,11 +354,15 @@ static int weight_grad_q8_reduce(const float* partial, void* grad_w, int64_t n, 
 
 using namespace hlm;
 
+static size_t weight_grad_q8_bytes(const WgPlan& plan, int64_t tokens, int64_t N, int64_t K) {
+  const size_t part =
+      plan.splits > 1 ? static_cast<size_t>(plan.splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4 : 0;
+  return kWgHeadBytes + 2 * weight_grad_q8_back_bytes(tokens, K) + part;
+}
+
 extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, int64_t K) {
   if (tokens <= 0 || N <= 0 || K <= 0) return 0;
-  const int splits = weight_grad_q8_plan(tokens, N, K).splits;
-  const size_t part = splits > 1 ? static_cast<size_t>(splits) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4 : 0;
-  return kWgHeadBytes + 2 * weight_grad_q8_back_bytes(tokens, K) + part;
+  return weight_grad_q8_bytes(weight_grad_q8_plan(tokens, N, K), tokens, N, K);
 }
 
 extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
@@ -377,10 +383,9 @@ extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* 
   }
   if (grad == nullptr || q == nullptr || scale == nullptr) return HLM_ERR_INVALID_ARG;
   if (!host_aligned16(grad) || !host_aligned16(q)) return HLM_ERR_UNSUPPORTED;
-  const size_t need = hlm_weight_grad_q8_workspace_bytes(tokens, N, K);
-  if (workspace == nullptr || workspace_bytes < need) return HLM_ERR_WORKSPACE;
-  if (!host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
   const WgPlan plan = weight_grad_q8_plan(tokens, N, K);
+  if (workspace == nullptr || workspace_bytes < weight_grad_q8_bytes(plan, tokens, N, K)) return HLM_ERR_WORKSPACE;
+  if (!host_aligned16(workspace)) return HLM_ERR_UNSUPPORTED;
   const int splits = plan.splits;
   float* head = static_cast<float*>(workspace);
   uint8_t* hi = static_cast<uint8_t*>(workspace) + kWgHeadBytes;
