@@ -67,10 +67,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "hlm_dequantize_rows": ([_P, _P, _P, _I64, _I64, c_int, _P], c_int),
     "hlm_residual_rms_norm_q8": ([_P, _P, _P, _P, _P, _P, _I64, _I64, c_float, c_int, _P], c_int),
     "hlm_linear_q8": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, c_int, _P], c_int),
+    "hlm_linear_q8_plan": ([_I64, _I64, _I64, c_int, POINTER(c_int)], c_int),
     "hlm_swiglu_ckpt8_fwd": ([_P, _P, _P, _P, _I64, _I64, c_int, _P], c_int),
     "hlm_swiglu_ckpt8_bwd": ([_P, _P, _P, _P, _I64, _I64, c_int, _P], c_int),
     "hlm_weight_grad_q8": ([_P, _P, _P, _P, _P, c_size_t, _I64, _I64, _I64, c_int, _P], c_int),
     "hlm_weight_grad_q8_workspace_bytes": ([_I64, _I64, _I64], c_size_t),
+    "hlm_weight_grad_q8_plan": ([_I64, _I64, _I64, POINTER(c_int), POINTER(c_int)], c_int),
     "hlm_gemm_bf16": (
         [_P, _P, _P, _I64, _I64, _I64, c_int, c_int, _I64, _I64, _I64, c_int, c_int, _P], c_int),
 }

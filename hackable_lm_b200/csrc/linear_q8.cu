@@ -603,14 +603,16 @@ static int choose_tile(int64_t M, int64_t N, int64_t K, bool aligned_rows) {
   return best;
 }
 
+// dp4a for a few tokens of small weights: with M tokens it needs M instructions for four
+// weights, and falls behind the tensor cores from about 8 M weights on ([8, 4096, 2048]
+// 4.8 us against 5.6, [8, 4096, 4096] 7.8 against 7.0, [8, 8192, 8192] 25 against 15)
+static bool rows_kernel(int64_t M, int64_t N, int64_t K) { return M == 1 || (M <= 8 && N * K <= (1ll << 23)); }
+
 template <typename T>
 static int linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, T* out, int64_t M,
                      int64_t N, int64_t K, cudaStream_t s) {
-  // dp4a for a few tokens of small weights: with M tokens it needs M instructions for four
-  // weights, and falls behind the tensor cores from about 8 M weights on ([8, 4096, 2048]
-  // 4.8 us against 5.6, [8, 4096, 4096] 7.8 against 7.0, [8, 8192, 8192] 25 against 15)
-  if (M == 1) return linear_q8_rows<T, 1>(q, scale, w, w_scale, out, M, N, K, s);
-  if (M <= 8 && N * K <= (1ll << 23)) {
+  if (rows_kernel(M, N, K)) {
+    if (M == 1) return linear_q8_rows<T, 1>(q, scale, w, w_scale, out, M, N, K, s);
     if (M <= 4) return linear_q8_rows<T, 4>(q, scale, w, w_scale, out, M, N, K, s);
     return linear_q8_rows<T, 8>(q, scale, w, w_scale, out, M, N, K, s);
   }
@@ -636,6 +638,19 @@ static int linear_q8(const void* q, const float* scale, const void* w, const flo
 
 using namespace hlm;
 
+static bool linear_q8_supported(int64_t M, int64_t N, int64_t K) {
+  // 128 * 128 * K stays within int32 up to K = 131056; TMA rows are 16-byte multiples
+  return K > 0 && K % 16 == 0 && K <= HLM_LINEAR_Q8_MAX_K && M <= (1ll << 31) - 512 && N <= (1ll << 31) - 512;
+}
+
+extern "C" int hlm_linear_q8_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int* tile) {
+  if (M <= 0 || N <= 0 || K < 0 || tile == nullptr) return HLM_ERR_INVALID_ARG;
+  if (out_dtype != HLM_F32 && out_dtype != HLM_BF16 && out_dtype != HLM_F16) return HLM_ERR_UNSUPPORTED;
+  if (!linear_q8_supported(M, N, K)) return HLM_ERR_UNSUPPORTED;
+  *tile = rows_kernel(M, N, K) ? 0 : choose_tile(M, N, K, N * (out_dtype == HLM_F32 ? 4 : 2) % 16 == 0);
+  return HLM_OK;
+}
+
 extern "C" int hlm_linear_q8(const void* q, const float* scale, const void* w, const float* w_scale,
                              void* out, int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
   if (M < 0 || N < 0 || K < 0) return HLM_ERR_INVALID_ARG;
@@ -644,9 +659,7 @@ extern "C" int hlm_linear_q8(const void* q, const float* scale, const void* w, c
   if (M == 0 || N == 0) return HLM_OK;
   if (q == nullptr || scale == nullptr || w == nullptr || w_scale == nullptr || out == nullptr)
     return HLM_ERR_INVALID_ARG;
-  // 128 * 128 * K stays within int32 up to K = 131056; TMA rows are 16-byte multiples
-  if (K == 0 || K % 16 != 0 || K > HLM_LINEAR_Q8_MAX_K) return HLM_ERR_UNSUPPORTED;
-  if (M > (1ll << 31) - 512 || N > (1ll << 31) - 512) return HLM_ERR_UNSUPPORTED;
+  if (!linear_q8_supported(M, N, K)) return HLM_ERR_UNSUPPORTED;
   if (!host_aligned16(q) || !host_aligned16(w)) return HLM_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (out_dtype) {

@@ -365,6 +365,14 @@ extern "C" size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, 
   return weight_grad_q8_bytes(weight_grad_q8_plan(tokens, N, K), tokens, N, K);
 }
 
+extern "C" int hlm_weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K, int* columns, int* splits) {
+  if (tokens <= 0 || N <= 0 || K <= 0 || columns == nullptr || splits == nullptr) return HLM_ERR_INVALID_ARG;
+  const WgPlan plan = weight_grad_q8_plan(tokens, N, K);
+  *columns = plan.bn;
+  *splits = plan.splits;
+  return HLM_OK;
+}
+
 extern "C" int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void* grad_w,
                                   void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N,
                                   int64_t K, int dtype, void* stream) {

@@ -404,6 +404,11 @@ int hlm_residual_rms_norm_q8(const void* residual, const void* branch, const voi
 #define HLM_LINEAR_Q8_MAX_K 131056
 int hlm_linear_q8(const void* q, const float* scale, const void* w, const float* w_scale, void* out,
                   int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
+/* Which kernel hlm_linear_q8 runs at these sizes on the current device (out 16-byte
+ * aligned), for tests and profiles: *tile = 0 the dp4a pass over the weights; 16, 32, 64
+ * or 128 the cluster kernel with so many tokens a tile; -128 or -256 the CTA-pair GEMM
+ * with 256 x 128 or 256 x 256 tiles.  The same refusals as the operator's. */
+int hlm_linear_q8_plan(int64_t M, int64_t N, int64_t K, int out_dtype, int* tile);
 
 /* SwiGLU that keeps its input in 8 bits for the backward pass.  Forward:
  * h = silu(gate) * up (as hlm_swiglu_fwd) and the codes of gate_up, in groups of
@@ -430,6 +435,9 @@ int hlm_weight_grad_q8(const void* grad, const void* q, const float* scale, void
                        void* workspace, size_t workspace_bytes, int64_t tokens, int64_t N, int64_t K,
                        int dtype, void* stream);
 size_t hlm_weight_grad_q8_workspace_bytes(int64_t tokens, int64_t N, int64_t K);
+/* How hlm_weight_grad_q8 divides these sizes on the current device, for tests and profiles:
+ * 256 x *columns tiles of grad_w (128 or 256), the tokens in *splits parts. */
+int hlm_weight_grad_q8_plan(int64_t tokens, int64_t N, int64_t K, int* columns, int* splits);
 
 /* ------------------------------------------------------------------------
  * Plain tcgen05 GEMM (building block; also used by tests)

@@ -236,6 +236,46 @@ def test_linear_q8(M, N, K, out_dtype, cuda_device):
     _check_linear(q, scale * (1e-2 if out_dtype == torch.float16 else 1.0), w, w_scale, out_dtype, cuda_device)
 
 
+def _linear_tile(M, N, K, out_dtype):
+    import ctypes
+
+    from hackable_lm_b200 import _lib, ops
+
+    tile = ctypes.c_int()
+    _lib.check(_lib.load().hlm_linear_q8_plan(M, N, K, ops._code(out_dtype), ctypes.byref(tile)), "hlm_linear_q8_plan")
+    return tile.value
+
+
+# M, N, K, the kernel they run: the CTA-pair GEMM with several tiles a pair (a second round of its
+# accumulators, rows and columns that end inside a tile, rows of the output that are no 16-byte
+# multiples), and the cluster kernel's largest tile
+DENSE_LINEAR_SHAPES = [(8192, 4096, 768, -256), (8190, 4096, 784, -256), (4100, 4095, 768, -256), (6400, 640, 768, -128),
+                       (6401, 635, 400, -128), (128, 8192, 8192, 128), (100, 4099, 8192, 128)]
+
+
+@pytest.mark.parametrize("out_dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K,tile", DENSE_LINEAR_SHAPES)
+def test_linear_q8_many_tiles(M, N, K, tile, out_dtype, cuda_device):
+    """Against the exact sums, made in float64 on the GPU."""
+    from hackable_lm_b200 import kernels
+
+    assert _linear_tile(M, N, K, out_dtype) == tile
+    q, scale = (t.to(cuda_device) for t in codes((M, K), seed=M))
+    w, w_scale = (t.to(cuda_device) for t in codes((N, K), seed=N))
+    if out_dtype == torch.float16:
+        scale = scale * 1e-2
+    y = kernels.linear_q8(q, scale, w, w_scale, out_dtype).double()
+    e = quant8.linear_q8(q, scale, w, w_scale)
+    over = (y - e).abs() - e.abs() * (3 * U + half_step(out_dtype)) - half_subnormal(out_dtype)
+    assert float(over.max()) <= 0, f"over the bound by {float(over.max()):.3e}"
+
+
+def test_linear_q8_shapes_reach_every_kernel(cuda_device):
+    for out_dtype in DTYPES:
+        reached = {_linear_tile(*shape[:3], out_dtype) for shape in LINEAR_SHAPES + DENSE_LINEAR_SHAPES}
+        assert reached == {0, 16, 32, 64, 128, -128, -256}
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_linear_q8_largest_sums(M, cuda_device):
     """Codes of the largest magnitude: -128 (which the quantiser never writes) times itself over

@@ -46,6 +46,27 @@ def test_c_entry_points_refuse_bad_arguments_before_any_launch():
     assert lib.hlm_weight_grad_q8(V, odd, V, V, None, 0, 4, 8, 16, BF, None) == -2
 
 
+def test_plan_queries():
+    lib = _lib.load()
+    a, b = ctypes.c_int(-7), ctypes.c_int(-7)
+    assert lib.hlm_linear_q8_plan(1, 4096, 768, _lib.HLM_BF16, None) == -1
+    assert lib.hlm_linear_q8_plan(0, 4096, 768, _lib.HLM_BF16, a) == -1
+    assert lib.hlm_linear_q8_plan(1, 4096, 24, _lib.HLM_BF16, a) == -2
+    assert lib.hlm_linear_q8_plan(1, 4096, 131072, _lib.HLM_BF16, a) == -2
+    assert lib.hlm_linear_q8_plan(1, 4096, 768, 5, a) == -2
+    assert lib.hlm_weight_grad_q8_plan(0, 8, 16, a, b) == -1
+    assert lib.hlm_weight_grad_q8_plan(1, 8, 16, None, b) == -1
+    assert a.value == b.value == -7
+    assert lib.hlm_linear_q8_plan(1, 4096, 768, _lib.HLM_BF16, a) == 0 and a.value == 0
+    assert lib.hlm_linear_q8_plan(32768, 4096, 768, _lib.HLM_F32, a) == 0 and a.value == -256
+    assert lib.hlm_weight_grad_q8_plan(32768, 4096, 768, a, b) == 0 and a.value == 256 and b.value > 1
+    for tokens, N, K in ((1, 8, 16), (1003, 520, 272), (32768, 768, 2048)):
+        assert lib.hlm_weight_grad_q8_plan(tokens, N, K, a, b) == 0 and b.value >= 1
+        parts = 4 * N * K * b.value if b.value > 1 else 0
+        need = lib.hlm_weight_grad_q8_workspace_bytes(tokens, N, K)
+        assert need >= 4 * tokens * K + parts
+
+
 def test_cpu_tensors_are_rejected():
     x = torch.randn(4, 32, dtype=torch.bfloat16)
     q, s = torch.zeros(4, 32, dtype=torch.int8), torch.ones(4)
