@@ -531,6 +531,45 @@ def test_weight_grad_q8_is_as_exact_as_its_result_can_be(tokens, N, K, dtype, cu
     assert float((y - e).norm()) <= 1.05 * float((e.to(dtype).double() - e).norm())
 
 
+# tokens, N, K, columns of a tile, whether the tokens are split (whole: with one and with several tiles a pair)
+PLANNED_WGRAD_SHAPES = [(200, 520, 272, 128, False), (500, 6400, 640, 128, False), (1003, 520, 272, 128, True),
+                        (20000, 264, 272, 128, True), (1000, 2048, 2064, 256, False), (300, 8192, 4096, 256, False),
+                        (4090, 2304, 768, 256, True), (8192, 2304, 768, 256, True), (32768, 768, 2048, 256, True)]
+
+
+def _wgrad_plan(tokens, N, K):
+    import ctypes
+
+    from hackable_lm_b200 import _lib
+
+    columns, splits = ctypes.c_int(), ctypes.c_int()
+    _lib.check(_lib.load().hlm_weight_grad_q8_plan(tokens, N, K, ctypes.byref(columns), ctypes.byref(splits)), "plan")
+    return columns.value, splits.value
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,N,K,columns,split", PLANNED_WGRAD_SHAPES)
+def test_weight_grad_q8_planned_tiles_and_splits(tokens, N, K, columns, split, dtype, cuda_device):
+    """Each tile width with the tokens whole and split, against the product in float64 (made on the
+    GPU): every element within its own bound, and all together as exact as the exact result rounded
+    once (within 5%), so that no part of the tokens is missing or counted twice."""
+    from hackable_lm_b200 import ops
+
+    got_columns, splits = _wgrad_plan(tokens, N, K)
+    assert (got_columns, splits > 1) == (columns, split)
+    q, scale = (t.to(cuda_device) for t in codes((tokens, K), seed=tokens))
+    grad = values((tokens, N), dtype, seed=N, scale=0.1).to(cuda_device)
+    y = ops.weight_grad_q8(grad, q, scale).double()
+    e = quant8.weight_grad_q8(grad, q, scale)
+    size = grad.double().abs().t() @ quant8.read_back(q, scale).abs()
+    E = half_step(dtype)
+    sub = grad.double().abs().sum(dim=0).unsqueeze(1) * 2 * half_subnormal(dtype)
+    bound = size * (2 * E * E + (2 * tokens + 4) * U) + sub
+    over = (y - e).abs() - bound - (e.abs() + bound) * E - half_subnormal(dtype)
+    assert float(over.max()) <= 0, f"over the bound by {float(over.max()):.3e}"
+    assert float((y - e).norm()) <= 1.05 * float((e.to(dtype).double() - e).norm())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("tokens", [50, 3000, 200000])
 @pytest.mark.parametrize("least,most,reach", [(2.0 ** 4, 2.0 ** 11, 2.0 ** -12), (2.0 ** -40, 2.0 ** -30, 2.0 ** 13),
