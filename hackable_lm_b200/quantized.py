@@ -31,6 +31,15 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight", q)
         self.register_buffer("weight_scale", scale)
 
+    def _apply(self, fn, recurse=True):
+        """Moves to another device; a move to another type (``.half()``, ``.to(torch.bfloat16)``) is for
+        the floating tensors around the codes, whose scales stay as they are, in fp32."""
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def forward(self, q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return kernels.linear_q8(q, scale, self.weight, self.weight_scale, out_dtype)
 

@@ -76,6 +76,32 @@ def test_int8_model_weights_and_state(cuda_device):
     assert torch.equal(other(x)[0], quantized(x)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_int8_model_in_another_type(dtype, cuda_device):
+    """A move to another type is for the stream between the projections: the codes and their scales
+    stay.  A wider or other 16-bit stream moves each of its roundings by at most two half steps of
+    bf16, 2^-7 of a value, well inside the 5.4% that the 8-bit rounding itself is given above."""
+    quantized = _model(cuda_device, depth=2).quantize_int8()
+    x, y = _tokens(cuda_device)
+    logits, (_, loss) = quantized(x)[0], quantized(x, y)
+    scales = {n: b.clone() for n, b in quantized.named_buffers() if n.endswith("weight_scale")}
+    moved = quantized.to(dtype)
+    assert moved is quantized and quantized.tok_emb.weight.dtype == dtype
+    for n, b in quantized.named_buffers():
+        if n.endswith("weight_scale"):
+            assert b.dtype == torch.float32 and torch.equal(b, scales[n])
+        elif n.endswith("weight"):
+            assert b.dtype == torch.int8
+    got, _ = quantized(x)
+    _, got_loss = quantized(x, y)
+    assert got.dtype == dtype and _rel(got, logits) < 0.054
+    assert abs(float(got_loss) - float(loss)) <= float((got.double() - logits.double()).abs().max()) + 1e-2
+    back, _ = quantized.to("cpu").to(cuda_device)(x)
+    assert torch.equal(back, got)
+    if dtype == torch.bfloat16:
+        assert torch.equal(got, logits)
+
+
 def test_int8_model_is_a_snapshot(cuda_device):
     """What happens to the model afterwards does not reach the 8-bit one."""
     model = _model(cuda_device, depth=2)

@@ -171,6 +171,21 @@ def test_activation_checkpoint_config():
         LanguageModel(model_config_for_depth(2, vocab_size=64)).quantize_int8()
 
 
+def test_int8_linear_keeps_its_scales_in_32_bits():
+    from hackable_lm_b200.quantized import Int8Linear
+
+    lin = Int8Linear(torch.empty(24, 32, device="meta", dtype=torch.bfloat16))
+    lin = lin.to_empty(device="cpu")
+    scale = torch.rand(24)
+    lin.weight.zero_()
+    lin.weight_scale.copy_(scale)
+    for move in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.float()):
+        move(lin)
+        assert lin.weight.dtype == torch.int8
+        assert lin.weight_scale.dtype == torch.float32 and torch.equal(lin.weight_scale, scale)
+    assert torch.equal(lin.state_dict()["weight_scale"], scale)
+
+
 def test_models_on_meta_tensors_reach_the_operators():
     from hackable_lm_b200.config import model_config_for_depth
     from hackable_lm_b200.model import LanguageModel
