@@ -79,7 +79,7 @@ class QuantizedBlock(nn.Module):
 class QuantizedLanguageModel(nn.Module):
     """``model.LanguageModel`` on 8-bit integer projections.  ``forward(idx, targets)`` returns
     what the model returns: (logits, None) without targets, else (None, mean loss over the
-    targets that are not ignore_index -100).  No gradients.  It holds copies: training the model
+    targets within the vocabulary; -100 and any other are left out).  No gradients.  It holds copies: training the model
     further, or moving it, changes nothing here."""
 
     def __init__(self, model: nn.Module) -> None:
@@ -101,13 +101,17 @@ class QuantizedLanguageModel(nn.Module):
             x, q8, scale = block(x, q8, scale)
         if targets is None:
             return self.lm_head(q8, scale, x.dtype), None
-        q8, scale, t = q8.reshape(-1, q8.shape[-1]), scale.reshape(-1), targets.reshape(-1)
+        q8, scale, t = q8.reshape(-1, q8.shape[-1]), scale.reshape(-1), targets.reshape(-1).to(torch.int64)
+        # as the fused LM-head loss: targets outside the vocabulary are left out (F.cross_entropy
+        # would stop the process's GPU work at one)
+        counted = (t >= 0) & (t < self.config.vocab_size)
+        t = torch.where(counted, t, -100)
         total = torch.zeros((), dtype=torch.float32, device=x.device)
         for s in range(0, t.numel(), self.loss_rows):  # logits of a chunk of tokens at a time, in fp32
             e = s + self.loss_rows
             logits = self.lm_head(q8[s:e], scale[s:e], torch.float32)
             total = total + F.cross_entropy(logits, t[s:e], reduction="sum")
-        return None, total / (t != -100).sum()
+        return None, total / counted.sum()
 
     def dequantized_weights(self, dtype: torch.dtype = torch.bfloat16) -> dict[str, torch.Tensor]:
         """The weights that the codes stand for, by module name."""

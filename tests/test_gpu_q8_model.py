@@ -55,6 +55,24 @@ def test_int8_model_against_bf16_model(length, window, cuda_device):
     assert torch.isnan(per) == torch.isnan(ignored) and (torch.isnan(per) or abs(float(per) - float(ignored)) < 1e-2)
 
 
+def test_int8_model_targets_like_the_bf16_models(cuda_device):
+    """32-bit targets are taken; targets outside the vocabulary are left out of the mean, as the bf16
+    model's fused loss leaves them out."""
+    model = _model(cuda_device, depth=2)
+    quantized = model.quantize_int8()
+    x, y = _tokens(cuda_device)
+    assert torch.equal(quantized(x, y.to(torch.int32))[1], quantized(x, y)[1])
+    ignored, odd = y.clone(), y.clone()
+    ignored[0, :5] = -100
+    odd[0, :5] = torch.tensor([-1, 512, 2 ** 40, -2 ** 40, -100], device=cuda_device)
+    expect = quantized(x, ignored)[1]
+    assert torch.equal(quantized(x, odd)[1], expect) and bool(torch.isfinite(expect))
+    with torch.no_grad():
+        assert torch.equal(model(x, odd)[1], model(x, ignored)[1])
+        none = torch.full_like(y, -1)
+        assert bool(torch.isnan(model(x, none)[1])) and bool(torch.isnan(quantized(x, none)[1]))
+
+
 def test_int8_model_weights_and_state(cuda_device):
     model = _model(cuda_device, depth=2)
     quantized = model.quantize_int8()
