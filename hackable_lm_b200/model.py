@@ -248,7 +248,9 @@ class MLP(nn.Module):
         super().__init__()
         self.gate_up = GateUpProjection(config)
         self.down = DownProjection(config)
-        self.keep_int8 = normalize_activation_checkpoint(config.activation_checkpoint) == "int8"
+        # a config without the field (the reference's own) keeps the activations whole
+        keep = getattr(config, "activation_checkpoint", "none")
+        self.keep_int8 = normalize_activation_checkpoint(keep) == "int8"
         if self.keep_int8 and not (self.gate_up.selected_backend() == self.down.selected_backend() == "b200"):
             raise RuntimeError("activation_checkpoint 'int8' needs the b200 gate_up and down backends")
 

@@ -171,6 +171,22 @@ def test_activation_checkpoint_config():
         LanguageModel(model_config_for_depth(2, vocab_size=64)).quantize_int8()
 
 
+def test_config_without_the_checkpoint_field():
+    """A config object of the reference's fields alone builds the model, as before the field was there."""
+    from types import SimpleNamespace
+
+    from hackable_lm_b200.config import model_config_for_depth
+    from hackable_lm_b200.model import LanguageModel
+
+    fields = model_config_for_depth(2, vocab_size=64, sequence_len=32, backend="torch", attention_backend="torch").to_dict()
+    del fields["activation_checkpoint"], fields["extra"]
+    model = LanguageModel(SimpleNamespace(**fields))
+    idx = torch.zeros(1, 8, dtype=torch.long)
+    _, loss = model(idx, idx)
+    loss.backward()
+    assert bool(torch.isfinite(loss)) and not model.blocks[0].mlp.keep_int8
+
+
 def test_int8_linear_keeps_its_scales_in_32_bits():
     from hackable_lm_b200.quantized import Int8Linear
 
