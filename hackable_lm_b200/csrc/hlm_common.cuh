@@ -628,7 +628,8 @@ HLM_DEVICE uint32_t pack_bf16x2(float lo, float hi) {
 
 HLM_DEVICE float sigmoidf_(float x) { return 1.0f / (1.0f + __expf(-x)); }
 // 1 / (1 + 2^(-x log2 e)) with the hardware ex2 and an approximate divide
-// (two MUFU ops, a few ulp of fp32): for kernels whose outputs are bf16.
+// (two MUFU ops): a few units of fp32, and 2 |x| 2^-24 of the value for negative x from the
+// argument's rounding.  For 16-bit outputs; the SwiGLU kernels use it for fp32 tensors too.
 HLM_DEVICE float sigmoid_fast(float x) {
   return __fdividef(1.0f, 1.0f + ex2_ftz(x * -1.4426950408889634f));
 }

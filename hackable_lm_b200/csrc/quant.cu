@@ -199,8 +199,14 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_scalar_kernel(
         const float g = static_cast<float>(qp[c]) * sg;
         const float u = static_cast<float>(qp[hidden + c]) * su;
         const float d = to_f32(dp[c]);
-        const float s = sigmoid_fast(g);
-        gp[c] = from_f32<T>(d * u * (s * (1.0f + g * (1.0f - s))));
+        float s, rest;
+        if constexpr (sizeof(T) == 4) {
+          sigmoid_exact(g, s, rest);
+        } else {
+          s = sigmoid_fast(g);
+          rest = 1.0f - s;
+        }
+        gp[c] = from_f32<T>(d * u * (s * (1.0f + g * rest)));
         gp[hidden + c] = from_f32<T>(d * (g * s));
       }
     }
@@ -663,9 +669,20 @@ __global__ void __launch_bounds__(256) swiglu_ckpt8_bwd_vec_kernel(
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const F2 gv = g[i] * sg2, uv = u[i] * su2, dd = d[2 * k + i];
-            const F2 s = f2_sigmoid(gv);
+            F2 s, rest;  // sigmoid(g) and 1 - sigmoid(g)
+            if constexpr (sizeof(T) == 4) {
+              float g0, g1, s0, s1, r0, r1;
+              f2_split(gv, g0, g1);
+              sigmoid_exact(g0, s0, r0);
+              sigmoid_exact(g1, s1, r1);
+              s = f2(s0, s1);
+              rest = f2(r0, r1);
+            } else {
+              s = f2_sigmoid(gv);
+              rest = f2_fma(s, minus, one);
+            }
             // d u s (1 + g (1 - s)) and d (g s)
-            rg[2 * k + i] = dd * uv * (s * f2_fma(gv, f2_fma(s, minus, one), one));
+            rg[2 * k + i] = dd * uv * (s * f2_fma(gv, rest, one));
             ru[2 * k + i] = dd * (gv * s);
           }
         }

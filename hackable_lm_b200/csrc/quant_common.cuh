@@ -106,7 +106,10 @@ HLM_DEVICE F2 f2_fma(F2 a, F2 b, F2 c) {
 }
 
 // 1 / (1 + 2^(-x log2 e)) of both values: the bits of sigmoid_fast, whose divide of 1 by a
-// number not below 1 is the approximate reciprocal.
+// number not below 1 is the approximate reciprocal.  The argument is a rounded product with a
+// rounded constant, so a value for negative x is off by up to 2 |x| 2^-24 of itself and a few
+// units: below the rounding of 16-bit results, not of fp32 ones.  The forward uses it for fp32 too,
+// since its output has the bits of the SwiGLU kernel, which does.
 HLM_DEVICE F2 f2_sigmoid(F2 x) {
   float a, b;
   f2_split(x * f2(-1.4426950408889634f), a, b);
@@ -114,6 +117,14 @@ HLM_DEVICE F2 f2_sigmoid(F2 x) {
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
   return f2(a, b);
+}
+
+// For fp32 gradients: sigmoid(x) and 1 - sigmoid(x), each to some 2^-21 of itself whatever x.
+// The complement is made from the exponential where the difference would cancel.
+HLM_DEVICE void sigmoid_exact(float x, float& s, float& rest) {
+  const float e = expf(-x);
+  s = __fdividef(1.0f, 1.0f + e);
+  rest = x < 0.0f ? 1.0f - s : e * s;
 }
 
 // Two packed 16-bit values, or two fp32 ones, as a pair (exact).

@@ -382,6 +382,28 @@ def test_swiglu_ckpt8_far_and_zero_values(dtype, cuda_device):
     _check_swiglu(gate_up, values((4, 300), dtype, seed=6), cuda_device)
 
 
+@pytest.mark.parametrize("hidden", [128, 129, 1000])
+def test_swiglu_ckpt8_fp32_gradient_of_far_gates(hidden, cuda_device):
+    """fp32 gradients keep their bits however far the gate is.  The scales are powers of two, so the
+    values read back are exact.  e^-g is off by an ulp (2 U), s = 1 / (1 + e) by 7 U (the divide
+    by 2 ulp), its complement by 10 U (e s, or 1 - s where s is at most a half), so d g s by 9 U and
+    d u s (1 + g (1 - s)) by 22 U of the magnitudes."""
+    from hackable_lm_b200 import ops
+
+    g = torch.Generator().manual_seed(hidden)
+    rows, groups = 12, -(-hidden // 128)
+    q = torch.randint(-127, 128, (rows, 2 * hidden), generator=g, dtype=torch.int16).to(torch.int8)
+    scale = 2.0 ** torch.randint(-6, 0, (rows, 2 * groups), generator=g).float()
+    d = values((rows, hidden), torch.float32, seed=2, scale=0.1)
+    grad = ops.swiglu_ckpt8_backward(q.to(cuda_device), scale.to(cuda_device), d.to(cuda_device))
+    e = quant8.swiglu_ckpt8_backward(q, scale, d)
+    (qg, qu), (sg, su) = q.chunk(2, dim=-1), scale.chunk(2, dim=-1)
+    gate, up, dd = quant8.group_read_back(qg, sg), quant8.group_read_back(qu, su), d.double()
+    s, rest = torch.sigmoid(gate), torch.sigmoid(-gate)
+    bound = torch.cat(((dd * up * s).abs() * (1 + gate.abs() * rest) * 22 * U, (dd * gate * s).abs() * 9 * U), dim=-1)
+    assert_within(grad, e, bound + 2.0 ** -126, "grad_gate_up")
+
+
 @pytest.mark.parametrize("hidden", [64, 100, 129, 2048])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_swiglu_ckpt8_output_is_swiglu(hidden, dtype, cuda_device):
