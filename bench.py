@@ -345,6 +345,18 @@ D12_KERNELS = {"lm_logits": 1, "lm_dlogits": 1, "lm_dx": 1, "lm_dw": 1, "gate_up
                "proj_norm": 24, "rmsnorm_fwd": 1, "rmsnorm_bwd": 25}
 
 
+def d12_kernels(keep: str) -> dict:
+    """Calls of each timed kernel in a micro-step.  With 8-bit checkpoints the MLP runs unfused: its norm
+    is a kernel of its own (beside the input's), proj_norm is o_proj alone, each of the two projections
+    quantises its input and reads it back for its weight gradient."""
+    if keep == "none":
+        return dict(D12_KERNELS)
+    fused_mlp = ("gate_up", "swiglu_fwd", "swiglu_bwd", "swiglu_down_bwd")
+    return {k: n for k, n in D12_KERNELS.items() if k not in fused_mlp} | {
+        "proj_norm": 12, "rmsnorm_fwd": 13, "quant_rows": 24, "dequant_rows": 24, "swiglu_ckpt8_fwd": 12,
+        "swiglu_ckpt8_bwd": 12, "weight_grad_q8": 24}
+
+
 def d12_flops_per_token(window: int) -> int:
     if not window:
         return D12_FLOPS_PER_TOKEN
@@ -401,10 +413,9 @@ def bench_d12(args, d: Dist, device) -> dict:
             first_loss = float(l.float().item())
     torch.cuda.synchronize()
     # per-kernel timing of the library's own launches during the first timed step
-    # capacity: up to two launches per operator call (LM dlogits / grad_hidden run in row halves)
-    # (the fused MLP kernels do not run with 8-bit checkpoints, and proj_norm then runs for o_proj alone)
-    timers = {k: _lib.KernelTimer(k, 2 * n * s.accum) for k, n in D12_KERNELS.items()
-              if keep == "none" or k != "proj_norm"}
+    # capacity: several launches per operator call (the LM head's run in chunks and row halves)
+    kernel_calls = d12_kernels(keep)
+    timers = {k: _lib.KernelTimer(k, (8 if k.startswith("lm_") else 2) * n * s.accum) for k, n in kernel_calls.items()}
     clocks = ClockSampler(device.index)
     clocks.start()
     d.barrier()
@@ -469,30 +480,40 @@ def bench_d12(args, d: Dist, device) -> dict:
              "qkv_fwd": 2.0 * M * C * Hd, "qkv_dx": 2.0 * M * C * Hd, "qkv_dw": 2.0 * M * C * Hd,
              "gate_up": 2.0 * M * C * 2 * s.config.mlp_hidden,
              # o_proj (K = C) and down (K = H) calls alternate: the mean per call
-             "proj_norm": 2.0 * M * C * (Dq + s.config.mlp_hidden) / 2}
-    n_fwd = D12_KERNELS["rmsnorm_fwd"]
+             "proj_norm": 2.0 * M * C * (Dq + s.config.mlp_hidden) / 2 if keep == "none" else 2.0 * M * C * Dq,
+             # gate_up (2H x C) and down (C x H) alternate
+             "weight_grad_q8": 2.0 * M * C * (2 * Hm + Hm) / 2}
+    n_fwd = kernel_calls["rmsnorm_fwd"]
     bytes_ = {
         "swiglu_fwd": 2.0 * M * 3 * Hm,           # read gate_up [M,2H], write [M,H]
         "swiglu_bwd": 2.0 * M * 5 * Hm,           # read gate_up + grad [M,H], write [M,2H]
         # the input norm (read x, write norm); the residual variants run inside proj_norm
         "rmsnorm_fwd": 2.0 * M * C * (2 + 4 * (n_fwd - 1)) / n_fwd,
         # input norm: read x + grad_norm, write grad; residual variants also read the residual grad
-        "rmsnorm_bwd": 2.0 * M * C * (3 + 4 * (D12_KERNELS["rmsnorm_bwd"] - 1)) / D12_KERNELS["rmsnorm_bwd"],
+        "rmsnorm_bwd": 2.0 * M * C * (3 + 4 * (kernel_calls["rmsnorm_bwd"] - 1)) / kernel_calls["rmsnorm_bwd"],
         "qkv_bwd_norm": 2.0 * M * Dq * 6,         # read q, k, dq, dk; write dq_in, dk_in
         "lm_dlogits": 4.0 * M * V,                # bf16 logits read + dlogits written in place
         # down grad_h GEMM + SwiGLU backward: read grad_y [M,C], gate_up [M,2H], W_down [C,H];
         # write grad_gate_up [M,2H] (HBM-bound: 2*M*C*H FLOP over these bytes is below the ridge)
         "swiglu_down_bwd": 2.0 * (M * C + 4 * M * Hm + C * Hm),
+        # 8-bit checkpoints: inputs of width C and H alternate (2 bytes in, a code and a row's scale out;
+        # read back as two 16-bit values), gate_up and h with a scale for 128 hidden units
+        "quant_rows": M * (3.0 * (C + Hm) / 2 + 4),
+        "dequant_rows": M * (5.0 * (C + Hm) / 2 + 4),
+        "swiglu_ckpt8_fwd": M * 8.0 * (Hm + -(-Hm // 128)),
+        "swiglu_ckpt8_bwd": M * 8.0 * (Hm + -(-Hm // 128)),
     }
     breakdown, totals = {}, {}
     for k, t in timers.items():
+        if t.launches > t.capacity:
+            raise RuntimeError(f"{k}: {t.launches} launches in a step, {t.capacity} were timed: its calls are counted wrongly")
         ts = t.times_ms()
         if not ts:
             continue
         totals[k] = sum(ts)
-        # per operator call (D12_KERNELS calls per micro-step; a call may be two launches)
-        avg = sum(ts) / (D12_KERNELS[k] * s.accum)
-        e = {"launches_in_step": t.launches, "calls_in_step": D12_KERNELS[k] * s.accum,
+        # per operator call (kernel_calls per micro-step; a call may be several launches)
+        avg = sum(ts) / (kernel_calls[k] * s.accum)
+        e = {"launches_in_step": t.launches, "calls_in_step": kernel_calls[k] * s.accum,
              "avg_ms_per_call": round(avg, 4), "total_ms": round(sum(ts), 3),
              "share_of_step": round(sum(ts) / step0_ms, 4)}
         if k in flops:

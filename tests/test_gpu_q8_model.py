@@ -202,6 +202,33 @@ def test_8_bit_checkpoints_halve_what_the_mlp_keeps(cuda_device):
     assert held["int8"] == rows * (C + 2 * H + H + 4 * (1 + 12 + 1) + 2 * C)
 
 
+@pytest.mark.parametrize("keep", ["none", "int8"])
+def test_bench_counts_the_calls_of_a_step(keep, cuda_device):
+    """The bench's table of calls in a micro-step of twelve layers, by which it averages, is what runs."""
+    import bench
+    from hackable_lm_b200 import _lib
+
+    model = _model(cuda_device, depth=12, activation_checkpoint=keep)
+    x, y = _tokens(cuda_device)
+    calls = bench.d12_kernels(keep)
+    timers = {k: _lib.KernelTimer(k, 4 * n) for k, n in calls.items()}
+    for t in timers.values():
+        t.__enter__()
+    try:
+        model(x, y)[1].backward()
+    finally:
+        for t in timers.values():
+            t.__exit__(None, None, None)
+    torch.cuda.synchronize()
+    one_launch = {"gate_up", "proj_norm", "rmsnorm_fwd", "quant_rows", "dequant_rows", "swiglu_ckpt8_fwd",
+                  "swiglu_ckpt8_bwd", "weight_grad_q8"}
+    for k, n in calls.items():
+        if k in one_launch:
+            assert timers[k].launches == n, k
+        else:  # a call may be two launches; the unfused SwiGLU does not run here
+            assert n <= timers[k].launches <= 2 * n or (k in ("swiglu_fwd", "swiglu_bwd") and timers[k].launches == 0), k
+
+
 def test_train_step_with_8_bit_checkpoints(cuda_device):
     from hackable_lm_b200 import train
 
