@@ -31,9 +31,7 @@ bool encode_map(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inn
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return false;
   if (!host_aligned16(base) || (ld * elem_bytes) % 16 != 0 || inner == 0 || outer == 0 || ld < inner) return false;
-  const CUtensorMapDataType type = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                   : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const CUtensorMapDataType type = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {ld * elem_bytes};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem_bytes), box_outer};

@@ -1,7 +1,7 @@
 // Persistent warp-specialised tcgen05 GEMM core for sm_100a.
 //
 //   D[M, N] (+)= A[M, K] * B[N, K]^T      bf16 operands, fp32 accumulation in TMEM
-//                                         (Kind = KindS8: int8 operands, int32 sums)
+//                                         (pair kernel, Kind = KindS8: int8 operands, int32 sums)
 //
 // Roles (one CTA per SM, grid = min(#tiles, #SMs)):
 //   warp 0      : one thread issues TMA loads (cp.async.bulk.tensor, 128-byte
@@ -57,7 +57,8 @@ struct epi_cluster_exchange<E, std::void_t<decltype(E::kClusterExchange)>>
 // `static constexpr bool kRelaxedRelease = true`: the pair kernel then hands the
 // accumulator back without a release, which would wait for those stores to land.
 // What the MMA issuer may overwrite is the accumulator alone, and its tcgen05.ld
-// have completed (tcgen05.wait::ld) before the arrive.
+// have completed (tcgen05.wait::ld) before the arrive.  An epilogue that leaves anything else
+// for the issuer to read or overwrite needs the release.
 template <class E, class = void>
 struct epi_relaxed_release : std::false_type {};
 template <class E>
@@ -163,7 +164,7 @@ HLM_DEVICE bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err) {
   return true;
 }
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
 __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
     gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA0,
                       const __grid_constant__ CUtensorMap tmA1,
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
           armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
           const uint32_t sa = base + stage * L::kStageBytes;
           const uint32_t sb = sa + L::kABytes;
-          const int k0 = kb * Kind::kBlockK;
+          const int k0 = kb * kBK;
           // ---- A
           if constexpr (!A_MN) {
             const CUtensorMap* mp = &tmA0;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      constexpr uint32_t idesc = Kind::idesc(kBM, BN, A_MN, B_MN);
+      constexpr uint32_t idesc = make_idesc_bf16_f32(kBM, BN, A_MN, B_MN);
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(gemm_threads<EPI_WARPS>(), 1)
                                         : make_sw128_desc(sa + kk * 32u, 16u, 1024u);
             const uint64_t bdesc = B_MN ? make_sw128_desc(sb + kk * 2048u, 8192u, 1024u)
                                         : make_sw128_desc(sb + kk * 32u, 16u, 1024u);
-            Kind::mma(d_tmem, adesc, bdesc, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+            tc_mma_f16(d_tmem, adesc, bdesc, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
           }
           tc_commit(EMPTY_BAR(stage));
           if (++stage == STAGES) {
@@ -651,17 +652,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gemm_threads<EPI_WAR
 //   ld: row stride in elements, box = {64, box_outer}.
 bool encode_bf16_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                      uint64_t ld, uint32_t box_outer);
-// The same for elements of elem_bytes (1: bytes, 2: 16-bit, 4: fp32), box = {128 bytes, box_outer}.
+// The same for elements of elem_bytes (1: bytes, 2: 16-bit), box = {128 bytes, box_outer}.
 // The 16-bit map copies fp16 as well as bf16 (no arithmetic on the elements).
 bool encode_map(CUtensorMap* map, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
                 uint64_t ld, uint32_t box_outer);
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
 int launch_gemm_sm100(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                       const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                       cudaStream_t stream, int kernel_id) {
   using L = GemmSmem<BN, STAGES>;
-  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
+  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,
                 "shared memory budget exceeded");
@@ -683,12 +684,12 @@ int launch_gemm_sm100(const CUtensorMap& a0, const CUtensorMap& a1, const CUtens
 // epilogues that exchange data across the cluster.  With p.n_tiles == cluster
 // and p.splits == 1, the CTAs of a cluster take the n tiles of one m tile
 // together (work index w = m_tile * n_tiles + n_tile, stepped by the grid).
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4, class Kind = KindBf16>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS = 4>
 int launch_gemm_cluster(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& a2,
                         const CUtensorMap& b, const GemmParams& p, const typename Epi::Params& ep,
                         int cluster, cudaStream_t stream, int kernel_id) {
   using L = GemmSmem<BN, STAGES>;
-  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS, Kind>;
+  auto kern = gemm_sm100_kernel<BN, STAGES, A_MN, B_MN, Epi, EPI_WARPS>;
   const int smem = L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024;
   static_assert(L::kEpiOffset + Epi::template smem_bytes<EPI_WARPS>() + 1024 <= 232448,
                 "shared memory budget exceeded");

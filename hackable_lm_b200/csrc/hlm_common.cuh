@@ -491,15 +491,12 @@ __host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
          | (static_cast<uint32_t>(M >> 4) << 24); // M / 16
 }
 
-// Operand kinds of the GEMM kernels.  A K block is one 128-byte swizzle row of
+// Operand kinds of the pair GEMM.  A K block is one 128-byte swizzle row of
 // either (64 16-bit values or 128 int8), read by four MMAs of 32 bytes of K each.
 struct KindBf16 {
   static constexpr int kBlockK = 64;
   static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool a_mn, bool b_mn) {
     return make_idesc_bf16_f32(M, N, a_mn, b_mn);
-  }
-  static HLM_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    tc_mma_f16(d, a, b, idesc, acc);
   }
   static HLM_DEVICE void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     tc_mma_f16_pair(d, a, b, idesc, acc);
@@ -514,9 +511,6 @@ struct KindS8 {
   static constexpr int kBlockK = 128;
   static __host__ __device__ constexpr uint32_t idesc(int M, int N, bool, bool) {
     return make_idesc_s8_s32(M, N);
-  }
-  static HLM_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    tc_mma_i8(d, a, b, idesc, acc);
   }
   static HLM_DEVICE void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     tc_mma_i8_pair(d, a, b, idesc, acc);
