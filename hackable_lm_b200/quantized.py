@@ -92,6 +92,8 @@ class QuantizedLanguageModel(nn.Module):
         self.blocks = nn.ModuleList([QuantizedBlock(b) for b in model.blocks])
         self.lm_head = Int8Linear(model.lm_head.lm_head.weight)
         self.loss_rows = model.lm_head.chunk_size or 4096
+        if self.loss_rows < 0:  # as the model's own loss refuses it
+            raise RuntimeError(f"loss_chunk_size must be nonnegative, got {self.loss_rows}")
 
     @torch.no_grad()
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):

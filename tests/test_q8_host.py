@@ -187,6 +187,16 @@ def test_config_without_the_checkpoint_field():
     assert bool(torch.isfinite(loss)) and not model.blocks[0].mlp.keep_int8
 
 
+def test_int8_model_refuses_a_negative_loss_chunk():
+    from hackable_lm_b200.config import model_config_for_depth
+    from hackable_lm_b200.model import LanguageModel
+
+    with torch.device("meta"):
+        model = LanguageModel(model_config_for_depth(2, vocab_size=64, sequence_len=32, loss_chunk_size=-1))
+    with pytest.raises(RuntimeError, match="nonnegative"):
+        model.quantize_int8()
+
+
 def test_int8_linear_keeps_its_scales_in_32_bits():
     from hackable_lm_b200.quantized import Int8Linear
 
